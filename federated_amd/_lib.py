@@ -73,6 +73,20 @@ SIGNATURES = {
     "fc_dft_rotate": (_INT, [_P, _I32, _I64, _INT, _I64, _I64, _P, _I64, _P]),
     "fc_onebit_decode_sum": (_INT, [_P, _P, _I32, _I64, _P, _P]),
     "fc_onebit_decode_sum_range": (_INT, [_P, _P, _I32, _I64, _I64, _I64, _P, _P]),
+    # the clients' local step (client_rows.hip, client_linear.hip)
+    "fc_client_tiles": (_I64, [_P, _I32, _I32, _P, _P]),
+    "fc_layer_norm": (_INT, [_P, _I64, _INT, _P, _I32, _I64, _P, _I64, _P, _I64, _F32, _P, _I64, _P, _P, _P]),
+    "fc_layer_norm_backward": (_INT, [_P, _I64, _P, _I64, _INT, _P, _P, _P, _I32, _P, _I32, _I64, _P, _I64, _P, _I64,
+                                      _P, _I64, _P, _I64, _P, _I64, _INT, _P, _P]),
+    "fc_linear": (_INT, [_P, _I64, _INT, _P, _I32, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64, _INT, _P, _I64, _P,
+                         _I64, _P, _I64, _P]),
+    "fc_linear_backward_input": (_INT, [_P, _I64, _INT, _P, _I32, _I32, _I64, _I64, _P, _I64, _I64, _INT, _P, _I64,
+                                        _P, _I64, _P, _I64, _P]),
+    "fc_linear_backward_weight": (_INT, [_P, _I64, _P, _I64, _INT, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64,
+                                         _INT, _P]),
+    "fc_top_logits": (_INT, [_P, _I64, _INT, _I64, _I64, _I32, _F32, _P, _P, _P, _P]),
+    "fc_distill": (_INT, [_P, _I64, _INT, _I64, _I64, _P, _P, _I32, _P, _P, _I32, _F32, _P, _P, _P, _P, _P, _P, _P,
+                          _I64, _P]),
 }
 
 _lib = None

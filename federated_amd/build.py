@@ -2,10 +2,14 @@
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc", "fedcodec.hip")
 HDR = os.path.join(os.path.dirname(HERE), "include", "fedcodec.h")
+# the clients' local step: ordinary float32 arithmetic (denormals kept, contraction on)
+CLIENT_SRCS = [os.path.join(HERE, "csrc", f) for f in ("client_rows.hip", "client_linear.hip")]
+CLIENT_HDRS = [os.path.join(HERE, "csrc", "client_common.h")]
 OUT = os.path.join(HERE, "libfedcodec.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
@@ -21,15 +25,29 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
          "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
 
 
+# no packed float32 instructions, in any file: some of their forms are not reliable
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+CLIENT_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared"] + NO_PACKED_F32
+
+
 def build(force=False, verbose=False):
-  if (not force and os.path.exists(OUT) and
-      os.path.getmtime(OUT) >= max(os.path.getmtime(SRC), os.path.getmtime(HDR))):
+  sources = [SRC, HDR] + CLIENT_SRCS + CLIENT_HDRS
+  if not force and os.path.exists(OUT) and os.path.getmtime(OUT) >= max(os.path.getmtime(s) for s in sources):
     return OUT
   tmp = OUT + ".tmp.%d" % os.getpid()
-  cmd = [HIPCC] + FLAGS + ["-o", tmp, SRC]
-  if verbose:
-    print(" ".join(cmd), flush=True)
-  subprocess.check_call(cmd)
+  with tempfile.TemporaryDirectory() as d:
+    objs, running = [], []
+    for src, flags in [(SRC, FLAGS)] + [(s, CLIENT_FLAGS) for s in CLIENT_SRCS]:
+      objs.append(os.path.join(d, os.path.basename(src) + ".o"))
+      cmd = [HIPCC, "-c"] + [f for f in flags if f != "-shared"] + ["-o", objs[-1], src]
+      if verbose:
+        print(" ".join(cmd), flush=True)
+      running.append((cmd, subprocess.Popen(cmd)))  # pylint: disable=consider-using-with
+    codes = [p.wait() for _, p in running]
+    for (cmd, _), rc in zip(running, codes):
+      if rc:
+        raise subprocess.CalledProcessError(rc, cmd)
+    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp] + objs)
   os.replace(tmp, OUT)
   return OUT
 

@@ -1,0 +1,449 @@
+"""Operators of the clients' local step, batched over a round's clients.
+
+What a round's codec reads -- one float32 row of P elements per client -- is made by
+every sampled client's local step (trainer.py:286-291 hands the model's deltas to the
+aggregator).  These operators run that step's products, norms and losses for all of
+a round's clients in one launch each:
+
+  - a ``ClientBatch`` says which rows of an activation tensor are whose (any number
+    per client, none included);
+  - weights are [clients, ...] tensors with any client stride: views into the
+    clients' flat parameter rows ([clients, P], one row per client), or one weight
+    broadcast to all clients (``expand``, stride 0: a round's first step);
+  - weight gradients are float32 and can be written straight into views of the
+    [clients, P] rows that ``codec.quantize_encode`` and the aggregators take.
+
+Activations and weights are float32, bfloat16 or float16, of one type per call;
+sums, statistics and gradients of weights are held in float32.  All calls are
+asynchronous on the current stream of the tensors' device, allocate what they return
+(unless given ``out``) and keep nothing.  Rows behind the batch's last are not read;
+in a given output they are left as they were, in an allocated one they are zero.
+
+Forward and backward are separate calls with explicit gradients: a broadcast weight
+still gets one gradient per client, which is what the codec encodes.
+"""
+import ctypes
+
+import numpy as np
+import torch
+
+from federated_amd import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
+_TILES = (16, 64, 128)
+MAX_TOP = 1024  # FC_MAX_TOP
+
+
+class ClientBatch:
+  """Which rows belong to which client: ``counts[c]`` rows for client c, in order.
+
+  Built once per round from the clients' row counts (host integers); holds the
+  offsets and the row-tile tables the kernels read on ``device``.
+  """
+
+  def __init__(self, counts, device=None):
+    _lib.require_gpu()
+    counts = np.ascontiguousarray(np.asarray(counts))
+    if counts.ndim != 1 or counts.size == 0:
+      raise ValueError("counts must be a non-empty list of row counts")
+    if not np.issubdtype(counts.dtype, np.integer):
+      raise ValueError("row counts must be integers, got %s" % counts.dtype)
+    counts = counts.astype(np.int64)
+    if counts.min() < 0:
+      raise ValueError("row counts must not be negative")
+    if int(counts.sum()) >= (1 << 31) - 1024:
+      raise ValueError("a batch holds fewer than 2^31 - 1024 rows")
+    self.device = torch.device("cuda" if device is None else device)
+    if self.device.type != "cuda":
+      raise ValueError("a ClientBatch lives on the GPU, got %s" % self.device)
+    if self.device.index is None:
+      self.device = torch.device("cuda", torch.cuda.current_device())
+    self.counts = counts
+    self.num_clients = int(counts.size)
+    self.num_rows = int(counts.sum())
+    ends = np.cumsum(counts)
+    # one host buffer, one copy: offsets, row -> client, a table entry per client, tiles
+    parts = [np.concatenate([[0], ends]).astype(np.int32),
+             np.repeat(np.arange(counts.size, dtype=np.int32), counts),
+             np.stack([np.arange(counts.size), ends - counts, counts, np.zeros_like(counts)], 1).astype(np.int32)]
+    for rows in _TILES:
+      parts.extend(self._tile_table(rows))
+    starts, at = [], 0
+    for p in parts:
+      starts.append(at)
+      at += (p.size + 3) // 4 * 4  # 16-byte aligned
+    host = np.zeros(at, np.int32)
+    for p, s in zip(parts, starts):
+      host[s:s + p.size] = p.reshape(-1)
+    dev = torch.from_numpy(host).to(self.device)
+    views = [dev[s:s + p.size] for p, s in zip(parts, starts)]
+    self.offsets, self.row_client, self._clients = views[:3]
+    self._tiles = {rows: (views[3 + 2 * i], views[4 + 2 * i], parts[3 + 2 * i].shape[0])
+                   for i, rows in enumerate(_TILES)}
+
+  def _tile_table(self, rows):
+    lib = _lib.load()
+    counts = self.counts.ctypes.data_as(ctypes.c_void_p)
+    n = int(lib.fc_client_tiles(counts, self.num_clients, rows, None, None))
+    if n < 0:
+      _lib.check(n)
+    tiles = np.zeros((n, 4), np.int32)
+    first = np.zeros(self.num_clients + 1, np.int32)
+    lib.fc_client_tiles(counts, self.num_clients, rows, tiles.ctypes.data_as(ctypes.c_void_p),
+                        first.ctypes.data_as(ctypes.c_void_p))
+    return tiles, first
+
+
+# --- argument checks -------------------------------------------------------------
+
+
+def _activations(name, t, batch, width=None, like=None):
+  if not isinstance(t, torch.Tensor) or t.dim() != 2:
+    raise ValueError("%s must be a [rows, width] tensor" % name)
+  if t.dtype not in _DTYPES:
+    raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+  if like is not None and t.dtype != like.dtype:
+    raise ValueError("%s is %s, expected %s" % (name, t.dtype, like.dtype))
+  if t.device != batch.device:
+    raise ValueError("%s is on %s, the batch on %s" % (name, t.device, batch.device))
+  if t.shape[0] < batch.num_rows:
+    raise ValueError("%s has %d rows, the batch %d" % (name, t.shape[0], batch.num_rows))
+  if t.shape[1] == 0 or (width is not None and t.shape[1] != width):
+    raise ValueError("%s has width %d%s" % (name, t.shape[1], "" if width is None else ", expected %d" % width))
+  _rows_ok(name, t)
+  return t
+
+
+def _rows_ok(name, t):
+  if t.shape[-1] > 1 and t.stride(-1) != 1:
+    raise ValueError("%s must be contiguous along its last axis" % name)
+
+
+def _distinct(name, t):
+  """An output whose elements must not overlap."""
+  need = 1
+  for size, stride in sorted(zip(t.shape, t.stride()), key=lambda p: p[1]):
+    if size > 1:
+      if stride < need:
+        raise ValueError("%s has overlapping elements" % name)
+      need = stride * (size - 1) + need
+  return t
+
+
+def _params(name, t, batch, shape, dtype):
+  if not isinstance(t, torch.Tensor) or tuple(t.shape) != (batch.num_clients,) + shape:
+    raise ValueError("%s must be a %s tensor, got %s" % (
+        name, [batch.num_clients] + list(shape), list(t.shape) if isinstance(t, torch.Tensor) else type(t)))
+  if t.dtype != dtype:
+    raise ValueError("%s is %s, expected %s" % (name, t.dtype, dtype))
+  if t.device != batch.device:
+    raise ValueError("%s is on %s, the batch on %s" % (name, t.device, batch.device))
+  _rows_ok(name, t)
+  return t
+
+
+def _grad_out(name, t, batch, shape):
+  if t is None:
+    return torch.empty((batch.num_clients,) + shape, dtype=torch.float32, device=batch.device)
+  return _distinct(name, _params(name, t, batch, shape, torch.float32))
+
+
+def _out(name, out, like, batch, width):
+  if out is not None:
+    return _distinct(name, _activations(name, out, batch, width, like))
+  out = torch.empty((like.shape[0], width), dtype=like.dtype, device=like.device)
+  if like.shape[0] > batch.num_rows:
+    out[batch.num_rows:].zero_()
+  return out
+
+
+def _vector(name, t, rows, device):
+  if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.dtype != torch.float32 or t.shape[0] < rows:
+    raise ValueError("%s must be a float32 vector of at least %d" % (name, rows))
+  if t.device != device:
+    raise ValueError("%s is on %s, expected %s" % (name, t.device, device))
+  if t.shape[0] > 1 and t.stride(0) != 1:
+    raise ValueError("%s must be contiguous" % name)
+  return t
+
+
+def _stats(rows, batch):
+  t = torch.empty(rows, dtype=torch.float32, device=batch.device)
+  if rows > batch.num_rows:
+    t[batch.num_rows:].zero_()
+  return t
+
+
+def _ptr(t):
+  return None if t is None else t.data_ptr()
+
+
+def _ld(t):
+  return 0 if t is None else t.stride(0)
+
+
+def _call(device, name, *args):
+  stream = torch.cuda.current_stream(device).cuda_stream
+  if device.index == torch.cuda.current_device():
+    _lib.call(name, *args, stream)
+  else:
+    with torch.cuda.device(device):
+      _lib.call(name, *args, stream)
+
+
+# --- layer norm ------------------------------------------------------------------
+
+
+def layer_norm(x, weight, bias, batch, eps=1e-5, out=None):
+  """y = (x - mean) rstd weight_c + bias_c over the last axis, client by client.
+
+  ``weight`` / ``bias``: [clients, dim] of x's type, or None.  Returns (y, mean,
+  rstd), the statistics as float32 [rows] for the backward pass.
+  """
+  _activations("x", x, batch)
+  dim = x.shape[1]
+  for name, t in (("weight", weight), ("bias", bias)):
+    if t is not None:
+      _params(name, t, batch, (dim,), x.dtype)
+  out = _out("out", out, x, batch, dim)
+  mean, rstd = _stats(x.shape[0], batch), _stats(x.shape[0], batch)
+  tiles, _, ntiles = batch._tiles[16]  # pylint: disable=protected-access
+  _call(batch.device, "fc_layer_norm", _ptr(x), x.stride(0), _DTYPES[x.dtype], _ptr(tiles), ntiles, dim,
+        _ptr(weight), _ld(weight), _ptr(bias), _ld(bias), float(eps), _ptr(out), out.stride(0), _ptr(mean),
+        _ptr(rstd))
+  return out, mean, rstd
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight, batch, residual=None, dweight=None, dbias=None,
+                        accumulate=False, out=None):
+  """Gradients of ``layer_norm``: (dx, dweight, dbias).
+
+  ``residual``: a gradient added to dx (the branch around the norm).  ``dweight`` /
+  ``dbias``: float32 [clients, dim] outputs (views of the clients' rows), allocated
+  when None; ``accumulate`` adds to the given ones.  A client without rows gets zeros.
+  """
+  _activations("x", x, batch)
+  dim = x.shape[1]
+  _activations("dy", dy, batch, dim, x)
+  _vector("mean", mean, batch.num_rows, batch.device)
+  _vector("rstd", rstd, batch.num_rows, batch.device)
+  if weight is not None:
+    _params("weight", weight, batch, (dim,), x.dtype)
+  if residual is not None:
+    _activations("residual", residual, batch, dim, x)
+  if accumulate and (dweight is None or dbias is None):
+    raise ValueError("accumulate needs dweight and dbias to add to")
+  dweight = _grad_out("dweight", dweight, batch, (dim,))
+  dbias = _grad_out("dbias", dbias, batch, (dim,))
+  out = _out("out", out, x, batch, dim)
+  tiles, first, ntiles = batch._tiles[64]  # pylint: disable=protected-access
+  part = torch.empty(ntiles * 2 * dim, dtype=torch.float32, device=batch.device)
+  _call(batch.device, "fc_layer_norm_backward", _ptr(dy), dy.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
+        _ptr(mean), _ptr(rstd), _ptr(tiles), ntiles, _ptr(first), batch.num_clients, dim, _ptr(weight), _ld(weight),
+        _ptr(residual), _ld(residual), _ptr(out), out.stride(0), _ptr(dweight), dweight.stride(0), _ptr(dbias),
+        dbias.stride(0), int(bool(accumulate)), _ptr(part))
+  return out, dweight, dbias
+
+
+# --- linear ----------------------------------------------------------------------
+
+
+def _activation(activation):
+  if activation not in _ACTIVATIONS:
+    raise ValueError("activation must be None, 'relu', 'gelu' or 'silu', got %r" % (activation,))
+  return _ACTIVATIONS[activation]
+
+
+def _weight(weight, batch, dtype, inner=None, outer=None):
+  if not isinstance(weight, torch.Tensor) or weight.dim() != 3:
+    raise ValueError("weight must be a [clients, out_features, in_features] tensor")
+  m, k = weight.shape[1:]
+  if m == 0 or k == 0 or (inner is not None and k != inner) or (outer is not None and m != outer):
+    raise ValueError("weight is [clients, %d, %d], expected [clients, %s, %s]" % (
+        m, k, "out" if outer is None else outer, "in" if inner is None else inner))
+  _params("weight", weight, batch, (m, k), dtype)
+  return m, k
+
+
+def linear(x, weight, bias, batch, activation=None, residual=None, preactivation=False, out=None):
+  """y = activation(x weight_c^T + bias_c) + residual, client by client.
+
+  ``weight``: [clients, out_features, in_features]; ``bias``: [clients, out_features]
+  or None, both of x's type.  ``activation``: None, "relu", "gelu" (the exact one) or
+  "silu".  With ``preactivation`` returns (y, z), z the value under the activation
+  (rounded to x's type), which the backward pass of the next operator down reads.
+  """
+  _activations("x", x, batch)
+  act = _activation(activation)
+  m, k = _weight(weight, batch, x.dtype, inner=x.shape[1])
+  if bias is not None:
+    _params("bias", bias, batch, (m,), x.dtype)
+  if residual is not None:
+    _activations("residual", residual, batch, m, x)
+  out = _out("out", out, x, batch, m)
+  z = _out("z", None, x, batch, m) if preactivation else None
+  tiles, _, ntiles = batch._tiles[128]  # pylint: disable=protected-access
+  _call(batch.device, "fc_linear", _ptr(x), x.stride(0), _DTYPES[x.dtype], _ptr(tiles), ntiles, batch.num_clients,
+        k, m, _ptr(weight), weight.stride(0), weight.stride(1), _ptr(bias), _ld(bias), act, _ptr(residual),
+        _ld(residual), _ptr(z), _ld(z), _ptr(out), out.stride(0))
+  return (out, z) if preactivation else out
+
+
+def linear_backward_input(dz, weight, batch, preactivation=None, activation=None, residual=None, out=None):
+  """dx = (dz weight_c) * activation'(preactivation) + residual, client by client.
+
+  ``dz``: the gradient at this product's pre-activation.  ``preactivation`` /
+  ``activation``: of the operator below, so that dx is the gradient at ITS
+  pre-activation.
+  """
+  act = _activation(activation)
+  _activations("dz", dz, batch)
+  m, k = _weight(weight, batch, dz.dtype, outer=dz.shape[1])
+  if (act != 0) != (preactivation is not None):
+    raise ValueError("activation and preactivation go together")
+  if preactivation is not None:
+    _activations("preactivation", preactivation, batch, k, dz)
+  if residual is not None:
+    _activations("residual", residual, batch, k, dz)
+  out = _out("out", out, dz, batch, k)
+  tiles, _, ntiles = batch._tiles[128]  # pylint: disable=protected-access
+  _call(batch.device, "fc_linear_backward_input", _ptr(dz), dz.stride(0), _DTYPES[dz.dtype], _ptr(tiles), ntiles,
+        batch.num_clients, k, m, _ptr(weight), weight.stride(0), weight.stride(1), act, _ptr(preactivation),
+        _ld(preactivation), _ptr(residual), _ld(residual), _ptr(out), out.stride(0))
+  return out
+
+
+def linear_backward_weight(dz, x, batch, dweight=None, dbias=None, bias=True, accumulate=False):
+  """(dweight, dbias): dweight_c = sum over client c's rows of dz x^T, dbias_c of dz.
+
+  float32 [clients, out_features, in_features] and [clients, out_features]: given
+  (views of the clients' rows; ``accumulate`` adds to them) or allocated.  ``bias``
+  False leaves dbias out (None).  A client without rows gets zeros.
+  """
+  _activations("x", x, batch)
+  _activations("dz", dz, batch, None, x)
+  m, k = dz.shape[1], x.shape[1]
+  if not bias and dbias is not None:
+    raise ValueError("dbias given with bias=False")
+  if accumulate and (dweight is None or (bias and dbias is None)):
+    raise ValueError("accumulate needs dweight and dbias to add to")
+  dweight = _grad_out("dweight", dweight, batch, (m, k))
+  if bias:
+    dbias = _grad_out("dbias", dbias, batch, (m,))
+  _call(batch.device, "fc_linear_backward_weight", _ptr(dz), dz.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
+        _ptr(batch._clients), batch.num_clients, k, m, _ptr(dweight), dweight.stride(0), dweight.stride(1),  # pylint: disable=protected-access
+        _ptr(dbias), _ld(dbias), int(bool(accumulate)))
+  return dweight, dbias
+
+
+# --- top logits and distillation ---------------------------------------------------
+
+
+def top_logits(logits, k, temperature=1.0):
+  """The k largest logits of every row: (indices int32, values, lse).
+
+  The message of a teacher: ``indices`` [rows, k] in falling order of value (ties to
+  the lowest index; NaN below every number), ``values`` [rows, k] of the logits' type,
+  ``lse`` float32 [rows] = log sum exp(logits / temperature) over the whole row.
+  """
+  if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or not logits.is_cuda:
+    raise ValueError("logits must be a [rows, vocabulary] tensor on the GPU")
+  if logits.dtype not in _DTYPES:
+    raise ValueError("logits must be float32, bfloat16 or float16, got %s" % logits.dtype)
+  _rows_ok("logits", logits)
+  rows, vocab = logits.shape
+  k = int(k)
+  if not 1 <= k <= min(vocab, MAX_TOP):
+    raise ValueError("k must be in [1, %d], got %d" % (min(vocab, MAX_TOP), k))
+  _temperature(temperature)
+  index = torch.empty((rows, k), dtype=torch.int32, device=logits.device)
+  values = torch.empty((rows, k), dtype=logits.dtype, device=logits.device)
+  lse = torch.empty(rows, dtype=torch.float32, device=logits.device)
+  _call(logits.device, "fc_top_logits", _ptr(logits), logits.stride(0), _DTYPES[logits.dtype], rows, vocab, k,
+        float(temperature), _ptr(index), _ptr(values), _ptr(lse))
+  return index, values, lse
+
+
+def _temperature(t):
+  if not 0.0 < float(t) < float("inf"):
+    raise ValueError("temperature must be positive and finite, got %r" % (t,))
+
+
+def _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights):
+  _activations("logits", logits, batch)
+  _temperature(temperature)
+  n = batch.num_rows
+  for name, t, dtype in (("indices", indices, torch.int32), ("values", values, None)):
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] < n or t.shape[1] != indices.shape[1]:
+      raise ValueError("%s must be a [rows, k] tensor of at least %d rows" % (name, n))
+    if t.device != batch.device:
+      raise ValueError("%s is on %s, the batch on %s" % (name, t.device, batch.device))
+    if dtype is not None and t.dtype != dtype:
+      raise ValueError("%s is %s, expected %s" % (name, t.dtype, dtype))
+  if not 1 <= indices.shape[1] <= MAX_TOP:
+    raise ValueError("k must be in [1, %d], got %d" % (MAX_TOP, indices.shape[1]))
+  if values.dtype not in _DTYPES:
+    raise ValueError("values must be float32, bfloat16 or float16, got %s" % values.dtype)
+  for name, t in (("teacher_lse", teacher_lse), ("row_weights", row_weights)):
+    if t is not None:
+      _vector(name, t, n, batch.device)
+  return indices.contiguous(), values.float().contiguous()
+
+
+def _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, lse, grad, want_loss, dloss):
+  loss = torch.empty(batch.num_clients, dtype=torch.float32, device=batch.device) if want_loss else None
+  row_loss = torch.empty(batch.num_rows, dtype=torch.float32, device=batch.device) if want_loss else None
+  _call(batch.device, "fc_distill", _ptr(logits), logits.stride(0), _DTYPES[logits.dtype], batch.num_rows,
+        logits.shape[1], _ptr(indices), _ptr(values), indices.shape[1], _ptr(batch.row_client), _ptr(batch.offsets),
+        batch.num_clients, float(temperature), _ptr(teacher_lse), _ptr(row_weights), _ptr(dloss), _ptr(row_loss),
+        _ptr(lse), _ptr(loss), _ptr(grad), _ld(grad))
+  return loss
+
+
+def distillation(logits, indices, values, batch, temperature=1.0, teacher_lse=None, row_weights=None):
+  """Distillation loss of every client from a teacher's top logits: (loss, lse).
+
+    p_k = exp(values_k / T - L),  q = softmax(logits / T)
+    loss_c = sum over the client's rows of  w_r T^2 sum_k p_k (log p_k - log q[indices_k])
+
+  ``indices`` / ``values``: [rows, k] as ``top_logits`` gives them; an index outside the
+  vocabulary (-1) or a value of -inf is padding, and a row of nothing but padding has
+  no loss and no gradient.  An index that comes twice counts twice.  L is
+  ``teacher_lse`` (float32 [rows], at this temperature: p then sums to less than one,
+  the rest of the teacher's mass is left out) or, when None, makes p sum to one.
+  ``row_weights``: float32 [rows]; None: 1 / (the client's rows), the mean.  A row of
+  weight 0 is not looked at.  ``lse`` (float32 [rows]) is for
+  ``distillation_backward``.
+  """
+  indices, values = _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights)
+  lse = _stats(logits.shape[0], batch)
+  loss = _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, lse, None, True, None)
+  return loss, lse
+
+
+def distillation_backward(logits, lse, indices, values, batch, temperature=1.0, teacher_lse=None, row_weights=None,
+                          dloss=None, out=None):
+  """Gradient of ``distillation`` by the logits; ``dloss``: float32 [clients] or None (ones).
+
+  ``out`` may be ``logits`` itself.
+  """
+  indices, values = _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights)
+  _vector("lse", lse, batch.num_rows, batch.device)
+  if dloss is not None:
+    _vector("dloss", dloss, batch.num_clients, batch.device)
+  out = _out("out", out, logits, batch, logits.shape[1])
+  _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, lse, out, False, dloss)
+  return out
+
+
+def distillation_with_gradient(logits, indices, values, batch, temperature=1.0, teacher_lse=None, row_weights=None,
+                               out=None):
+  """(loss, gradient by the logits) of ``distillation`` in one pass over the logits.
+
+  ``out`` may be ``logits`` itself.
+  """
+  indices, values = _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights)
+  out = _out("out", out, logits, batch, logits.shape[1])
+  loss = _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, None, out, True, None)
+  return loss, out

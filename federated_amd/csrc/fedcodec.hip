@@ -6437,6 +6437,10 @@ int64_t dft_len(int64_t m) {  // FFT length: m itself (power of two) or the Blue
 extern "C" {
 
 const char* fc_last_error(void) { return g_err.c_str(); }
+
+// The client-step operators' files report through the same message.
+__attribute__((visibility("hidden"))) int fc_internal_fail(int code, const char* msg) { return fail(code, msg); }
+__attribute__((visibility("hidden"))) int fc_internal_check_launch(const char* what) { return check_launch(what); }
 const char* fc_version(void) { return "fedcodec 0.1 gfx950"; }
 #ifdef FC_STAMPS
 int fc_debug_stamps(unsigned long long* host8, int reset) {

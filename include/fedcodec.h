@@ -426,6 +426,89 @@ int fc_diag_occupy(uint32_t xcd_mask, int64_t microseconds, int32_t* held, void*
 int fc_quantize_floor(const float* const* xs, int32_t nclients, int64_t P, float step, const int64_t* seeds, int mode,
                       float* dist_part, int32_t* nnz_part, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The clients' local step: what makes the rows the codec reads (the local training
+ * that trainer.py:286-291 runs before the aggregator).  Batched over a round's
+ * clients; activations are [rows, width] with a row stride, weights [clients, ...]
+ * with a client stride (0: one weight for all clients), gradients of weights
+ * float32 with a client stride (views of the clients' float32[P] rows).  Strides
+ * count elements; a pointer needs its type's own alignment only.  Rows no tile
+ * names are neither read nor written.
+ * ------------------------------------------------------------------------- */
+
+/* Types of activations and weights. */
+#define FC_FLOAT32 0
+#define FC_BFLOAT16 1
+#define FC_FLOAT16 2
+
+/* Activations of fc_linear(_backward_input). */
+#define FC_ACT_NONE 0
+#define FC_ACT_RELU 1
+#define FC_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
+#define FC_ACT_SILU 3
+
+#define FC_MAX_TOP 1024 /* top logits of a row */
+
+/* HOST: the row-tile table of a batch whose client c has counts[c] rows, in client
+ * order: per tile int32 {client, first row, rows, 0} with at most tile_rows rows, and
+ * first_tile[nclients + 1] (both nullable: the count alone).  Returns the number of
+ * tiles, or -1.  The kernels read the table from device memory and trust it. */
+int64_t fc_client_tiles(const int64_t* counts, int32_t nclients, int32_t tile_rows, int32_t* tiles,
+                        int32_t* first_tile);
+
+/* y = (x - mean) rstd weight_c + bias_c; weight, bias nullable.  tiles of 16 rows. */
+int fc_layer_norm(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, int32_t ntiles, int64_t dim,
+                  const void* weight, int64_t weight_stride, const void* bias, int64_t bias_stride, float eps,
+                  void* y, int64_t y_stride, float* mean, float* rstd, void* stream);
+
+/* dx (+ residual, nullable), dweight_c, dbias_c (nullable; accumulate: added to).
+ * partials: float[2 * ntiles * dim] device scratch; sums run in tile order. */
+int fc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int dtype,
+                           const float* mean, const float* rstd, const int32_t* tiles, int32_t ntiles,
+                           const int32_t* first_tile, int32_t nclients, int64_t dim, const void* weight,
+                           int64_t weight_stride, const void* residual, int64_t residual_stride, void* dx,
+                           int64_t dx_stride, float* dweight, int64_t dweight_stride, float* dbias,
+                           int64_t dbias_stride, int accumulate, float* partials, void* stream);
+
+/* y = act(x weight_c^T + bias_c) + residual; preactivation (nullable) takes the value
+ * under the activation.  tiles of 128 rows. */
+int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, int32_t ntiles, int32_t nclients,
+              int64_t in_features, int64_t out_features, const void* weight, int64_t weight_client_stride,
+              int64_t weight_stride, const void* bias, int64_t bias_client_stride, int activation,
+              const void* residual, int64_t residual_stride, void* preactivation, int64_t preactivation_stride,
+              void* y, int64_t y_stride, void* stream);
+
+/* dx = (dz weight_c) * act'(preactivation) + residual.  tiles of 128 rows. */
+int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const int32_t* tiles, int32_t ntiles,
+                             int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
+                             int64_t weight_client_stride, int64_t weight_stride, int activation,
+                             const void* preactivation, int64_t preactivation_stride, const void* residual,
+                             int64_t residual_stride, void* dx, int64_t dx_stride, void* stream);
+
+/* dweight_c = sum of dz_r x_r^T, dbias_c (nullable) = sum of dz_r over the client's
+ * rows.  clients: one int32 {client, first row, rows, 0} per client. */
+int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
+                              const int32_t* clients, int32_t nclients, int64_t in_features, int64_t out_features,
+                              float* dweight, int64_t dweight_client_stride, int64_t dweight_stride, float* dbias,
+                              int64_t dbias_client_stride, int accumulate, void* stream);
+
+/* The k largest logits of every row, falling, ties to the lowest index, NaN below every
+ * number; lse = log sum exp(logits / temperature) of the whole row. */
+int fc_top_logits(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t vocab, int32_t k,
+                  float temperature, int32_t* index, void* values, float* lse, void* stream);
+
+/* Distillation from k teacher entries per row (index [rows][k], outside the
+ * vocabulary: padding; values [rows][k]):
+ *   p = exp(values / T - L), L = teacher_lse or log sum exp;  q = softmax(logits / T)
+ *   loss_c = sum_r w_r T^2 sum_k p_k (log p_k - log q);  grad = w_r T (q sum p - p)
+ * loss given: loss [nclients] from row_loss [rows] (scratch), lse (nullable) out, grad
+ * (nullable; may be logits) in the same pass.  loss NULL: grad from the saved lse,
+ * scaled by dloss [nclients] (nullable).  row_weights NULL: 1 / the client's rows. */
+int fc_distill(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t vocab, const int32_t* index,
+               const float* values, int32_t k, const int32_t* row_client, const int32_t* offsets, int32_t nclients,
+               float temperature, const float* teacher_lse, const float* row_weights, const float* dloss,
+               float* row_loss, float* lse, float* loss, void* grad, int64_t grad_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

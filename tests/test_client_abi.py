@@ -1,0 +1,92 @@
+"""The client-step operators' C entry points without a GPU: refusals come before any
+device work, and the host-side row-tile table."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from federated_amd import _lib
+
+NULL = None
+
+
+def _buf():
+  return ctypes.addressof(ctypes.create_string_buffer(64))
+
+
+def refused(rc, word):
+  assert rc != 0 and word in _lib.load().fc_last_error(), (rc, _lib.load().fc_last_error())
+
+
+def test_client_tiles_cover_every_row_once():
+  lib = _lib.load()
+  for counts, height in [([5], 16), ([0, 16, 0, 17, 1], 16), ([0, 0], 64), ([130, 128, 127], 128), ([1] * 300, 64)]:
+    c = np.asarray(counts, np.int64)
+    p = c.ctypes.data_as(ctypes.c_void_p)
+    n = lib.fc_client_tiles(p, c.size, height, None, None)
+    assert n == sum(-(-k // height) for k in counts)
+    tiles, first = np.full((n, 4), -1, np.int32), np.full(c.size + 1, -1, np.int32)
+    assert lib.fc_client_tiles(p, c.size, height, tiles.ctypes.data_as(ctypes.c_void_p),
+                               first.ctypes.data_as(ctypes.c_void_p)) == n
+    seen = []
+    start = np.cumsum(c) - c
+    for k in range(c.size):
+      rows = [r for t in tiles[first[k]:first[k + 1]] for r in range(t[1], t[1] + t[2])]
+      assert all(t[0] == k and 0 < t[2] <= height for t in tiles[first[k]:first[k + 1]])
+      assert rows == list(range(start[k], start[k] + c[k]))
+      seen += rows
+    assert seen == list(range(c.sum())) and first[-1] == n
+
+
+def test_client_tiles_refusals():
+  lib = _lib.load()
+  c = np.array([3, -1], np.int64)
+  p = c.ctypes.data_as(ctypes.c_void_p)
+  assert lib.fc_client_tiles(p, 2, 16, None, None) == -1 and b"negative" in lib.fc_last_error()
+  assert lib.fc_client_tiles(None, 2, 16, None, None) == -1
+  assert lib.fc_client_tiles(p, 0, 16, None, None) == -1
+  assert lib.fc_client_tiles(p, 1, 0, None, None) == -1
+  c[:] = 1 << 31, 1
+  assert lib.fc_client_tiles(p, 2, 1 << 20, None, None) == -1 and b"too many rows" in lib.fc_last_error()
+
+
+def test_layer_norm_refusals():
+  lib, b = _lib.load(), _buf()
+  refused(lib.fc_layer_norm(b, 4, 0, b, 1, 0, b, 4, b, 4, 1e-5, b, 4, b, b, None), b"sizes")
+  refused(lib.fc_layer_norm(b, 4, 0, b, -1, 4, b, 4, b, 4, 1e-5, b, 4, b, b, None), b"sizes")
+  refused(lib.fc_layer_norm(NULL, 4, 0, b, 1, 4, b, 4, b, 4, 1e-5, b, 4, b, b, None), b"null")
+  refused(lib.fc_layer_norm(b, 4, 3, b, 1, 4, b, 4, b, 4, 1e-5, b, 4, b, b, None), b"dtype")
+  assert lib.fc_layer_norm(b, 4, 0, b, 0, 4, b, 4, b, 4, 1e-5, b, 4, b, b, None) == 0  # no rows: nothing to do
+  refused(lib.fc_layer_norm_backward(b, 4, b, 4, 0, b, b, b, 1, NULL, 1, 4, b, 4, NULL, 0, b, 4, b, 4, b, 4, 0, b,
+                                     None), b"null")
+  refused(lib.fc_layer_norm_backward(b, 4, b, 4, 0, b, b, b, 1, b, 0, 4, b, 4, NULL, 0, b, 4, b, 4, b, 4, 0, b,
+                                     None), b"sizes")
+  refused(lib.fc_layer_norm_backward(b, 4, b, 4, 0, b, b, b, 1, b, 1, 4, b, 4, NULL, 0, b, 4, b, 4, b, 4, 0, NULL,
+                                     None), b"null")
+
+
+def test_top_logits_and_distillation_refusals():
+  lib, b = _lib.load(), _buf()
+  for k in (0, 9, 1025):
+    refused(lib.fc_top_logits(b, 8, 0, 1, 8 if k < 100 else 5000, k, 1.0, b, b, b, None), b"bad k")
+  for t in (0.0, -1.0, float("inf"), float("nan")):
+    refused(lib.fc_top_logits(b, 8, 0, 1, 8, 2, t, b, b, b, None), b"temperature")
+  refused(lib.fc_top_logits(b, 8, 0, 1, 8, 2, 1.0, NULL, b, b, None), b"null")
+  refused(lib.fc_top_logits(b, 8, 7, 1, 8, 2, 1.0, b, b, b, None), b"dtype")
+
+  def distill(rows=1, vocab=8, k=2, clients=1, tau=1.0, dloss=NULL, row_loss=b, lse=b, loss=b, grad=NULL, logits=b,
+              dtype=0):
+    return lib.fc_distill(logits, 8, dtype, rows, vocab, b, b, k, b, b, clients, tau, NULL, NULL, dloss, row_loss, lse,
+                          loss, grad, 8, None)
+
+  refused(distill(k=0), b"bad k")
+  refused(distill(k=1025), b"bad k")
+  refused(distill(tau=0.0), b"temperature")
+  refused(distill(vocab=0), b"sizes")
+  refused(distill(clients=0), b"sizes")
+  refused(distill(loss=NULL), b"null")  # neither a loss nor a gradient wanted
+  refused(distill(loss=NULL, grad=b, lse=NULL), b"null")  # the gradient alone needs the saved lse
+  refused(distill(row_loss=NULL), b"null")
+  refused(distill(dloss=b), b"dloss")
+  refused(distill(logits=NULL), b"null")
+  refused(distill(dtype=4), b"dtype")

@@ -1,0 +1,789 @@
+"""The client-step operators against their definitions in float64.
+
+Tolerances are error bounds, not observations.  u = eps / 2 is a type's unit roundoff;
+an output of type T is rounded once (u_T |value|).  A float32 sum of n terms is off by
+at most n u_32 sum |terms|, whatever its order; a matrix instruction may chop where it
+adds, so products count 2 u_32 per term.  exp and log cost a few u_32 of their value,
+and exp turns an absolute error of its argument into a relative one.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from federated_amd import client_ops as ops
+
+pytestmark = pytest.mark.gpu
+
+U32 = torch.finfo(torch.float32).eps / 2
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ["f32", "bf16", "f16"]
+COUNTS = [5, 0, 1, 130, 17]  # an empty client, single rows, tiles that end inside
+
+
+def unit(dtype):
+  return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):  # half the spacing of the subnormals
+  return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+
+
+def rand(rng, shape, dtype, scale=1.0, gpu="cuda"):
+  return (torch.from_numpy(rng.standard_normal(shape).astype(np.float32)) * scale).to(gpu).to(dtype)
+
+
+def flat_params(rng, clients, sizes, dtype, scale, shared=False, pad=3):
+  """Views of `sizes` in flat rows [clients, P] (P odd), as a client's parameters lie."""
+  total = sum(int(np.prod(s)) for s in sizes) + pad
+  total += 1 - total % 2
+  rows = rand(rng, (1 if shared else clients, total), dtype, scale).expand(clients, total)
+  views, at = [], 1  # an odd first offset: no 16-byte alignment
+  for s in sizes:
+    n = int(np.prod(s))
+    views.append(rows[:, at:at + n].unflatten(1, tuple(s)) if len(s) > 1 else rows[:, at:at + n])
+    at += n
+  return views
+
+
+def spans(counts):
+  ends = np.cumsum(counts)
+  return [(int(e - c), int(e)) for e, c in zip(ends, counts)]
+
+
+def check(got, want, tol, what):
+  got = got.detach().double().cpu()
+  want, tol = want.double().cpu(), torch.as_tensor(tol).double().cpu()
+  assert got.shape == want.shape, what
+  bad = ~((got - want).abs() <= tol)
+  assert not bad.any(), "%s: %d of %d off, worst %.3g against %.3g" % (
+      what, int(bad.sum()), bad.numel(), float((got - want).abs().max()),
+      float(torch.broadcast_to(tol, got.shape)[(got - want).abs() == (got - want).abs().max()].max()))
+
+
+# --- layer norm ------------------------------------------------------------------
+
+
+def norm_reference(x, w, b, counts, eps, dy=None, residual=None):
+  x = x.double().cpu()
+  n, d = x.shape
+  mu = x.mean(1)
+  s = 1.0 / torch.sqrt(((x - mu[:, None]) ** 2).mean(1) + eps)
+  xh = (x - mu[:, None]) * s[:, None]
+  client = torch.from_numpy(np.repeat(np.arange(len(counts)), counts))
+  g = torch.ones(n, d, dtype=torch.float64) if w is None else w.double().cpu()[client]
+  y = xh * g + (0 if b is None else b.double().cpu()[client])
+  out = dict(y=y, mean=mu, rstd=s, xh=xh, g=g)
+  if dy is not None:
+    dy = dy.double().cpu()
+    a = dy * g
+    dx = s[:, None] * (a - a.mean(1, keepdim=True) - xh * (a * xh).mean(1, keepdim=True))
+    out["dx"] = dx if residual is None else dx + residual.double().cpu()
+    out["dw"] = torch.stack([(dy * xh)[lo:hi].sum(0) for lo, hi in spans(counts)])
+    out["db"] = torch.stack([dy[lo:hi].sum(0) for lo, hi in spans(counts)])
+  return out
+
+
+def norm_tolerances(ref, x, b, dim, dtype, counts=None, dy=None, residual=None):
+  x = x.double().cpu()
+  # a thread adds at most dim / 64 + 16 terms, and the threads join in 8 steps
+  depth = dim / 64 + 24
+  s = ref["rstd"]
+  e_mean = depth * U32 * x.abs().mean(1) + U32 * ref["mean"].abs()
+  # xh = (x - mu) s: the mean's error, a subtraction, and s (relative error: half the
+  # variance's, which is depth + 2 roundings plus the mean's error to first order, and
+  # four roundings of division, root, sum, product)
+  rel_s = (depth + 8) * U32 + s * e_mean
+  e_xh = s[:, None] * (e_mean[:, None] + U32 * (x - ref["mean"][:, None]).abs()) + ref["xh"].abs() * (
+      rel_s[:, None] + 2 * U32)
+  bias = 0 if b is None else float(b.abs().max())
+  tol = dict(mean=e_mean, rstd=s * rel_s,
+             y=ref["g"].abs() * e_xh + (unit(dtype) + 3 * U32) * (ref["y"].abs() + bias * 2 * U32) + tiny(dtype) +
+             2 * U32 * ((ref["xh"] * ref["g"]).abs() + bias))
+  if dy is not None:
+    dy = dy.double().cpu()
+    a = (dy * ref["g"]).abs()
+    res = 0 if residual is None else residual.double().cpu().abs()
+    xh = ref["xh"].abs()
+    # a, its mean and xh mean(a xh) each with their own roundings
+    e_m0 = (depth + 2) * U32 * a.mean(1, keepdim=True)
+    e_m1 = (depth + 3) * U32 * (a * xh).mean(1, keepdim=True) + (a * e_xh).mean(1, keepdim=True)
+    m0, m1 = a.mean(1, keepdim=True), (a * xh).mean(1, keepdim=True)
+    inner = a + m0 + xh * m1
+    e_dx = s[:, None] * (e_m0 + xh * e_m1 + e_xh * m1 + 5 * U32 * inner) + rel_s[:, None] * s[:, None] * inner
+    tol["dx"] = e_dx + unit(dtype) * ref["dx"].abs() + 2 * U32 * (res + ref["dx"].abs()) + tiny(dtype)
+    tol["dw"] = torch.stack([((hi - lo + 4) * U32 * (dy.abs() * xh)[lo:hi] + (dy.abs() * e_xh)[lo:hi]).sum(0)
+                             for lo, hi in spans(counts)])
+    tol["db"] = torch.stack([((hi - lo + 4) * U32 * dy.abs()[lo:hi]).sum(0) for lo, hi in spans(counts)])
+  return tol
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("dim", [1, 7, 96, 511, 670, 1024, 1027, 2048, 4096, 5000, 8193, 17000])
+def test_layer_norm_forward_and_backward(gpu, dtype, dim):
+  rng = np.random.default_rng(dim)
+  counts = COUNTS if dim < 4096 else [3, 0, 70]
+  n = sum(counts)
+  batch = ops.ClientBatch(counts)
+  x = rand(rng, (n, dim), dtype) + rand(rng, (n, 1), dtype)
+  w, b = flat_params(rng, len(counts), [(dim,), (dim,)], dtype, 0.5)
+  dy, res = rand(rng, (n, dim), dtype, 0.3), rand(rng, (n, dim), dtype)
+  y, mean, rstd = ops.layer_norm(x, w, b, batch)
+  rows = torch.full((len(counts), 2 * dim + 1), 7.0, device=gpu)
+  dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, w, batch, residual=res, dweight=rows[:, 1:dim + 1],
+                                       dbias=rows[:, dim + 1:])
+  ref = norm_reference(x, w, b, counts, 1e-5, dy, res)
+  tol = norm_tolerances(ref, x, b, dim, dtype, counts, dy, res)
+  for name, got in dict(y=y, mean=mean, rstd=rstd, dx=dx, dw=dw, db=db).items():
+    check(got, ref[name], tol[name], name)
+  assert (rows[:, 0] == 7.0).all()  # the row's other parameters are not touched
+  assert (dw[1] == 0).all() and (db[1] == 0).all()  # the client without rows
+
+
+@pytest.mark.parametrize("shared", [False, True], ids=["own", "shared"])
+def test_layer_norm_options(gpu, shared):
+  """Row strides, one weight for all clients, no weight or bias, accumulation, rows behind."""
+  rng = np.random.default_rng(3)
+  dim, counts = 130, [4, 9]
+  n = sum(counts)
+  batch = ops.ClientBatch(counts)
+  wide = rand(rng, (n + 5, dim + 7), torch.bfloat16)
+  wide[n:] = math.nan
+  x = wide[:, 3:3 + dim]
+  w, b = flat_params(rng, 2, [(dim,), (dim,)], torch.bfloat16, 0.5, shared=shared)
+  out = torch.full((n + 5, dim + 1), 5.0, dtype=torch.bfloat16, device=gpu)
+  y, mean, rstd = ops.layer_norm(x, w, b, batch, out=out[:, :dim])
+  ref = norm_reference(x[:n], w, b, counts, 1e-5)
+  check(y[:n], ref["y"], norm_tolerances(ref, x[:n], b, dim, torch.bfloat16)["y"], "y")
+  assert (out[n:] == 5.0).all() and (out[:, dim] == 5.0).all()
+  y2, _, _ = ops.layer_norm(x, None, None, batch)
+  ref2 = norm_reference(x[:n], None, None, counts, 1e-5)
+  check(y2[:n], ref2["y"], norm_tolerances(ref2, x[:n], None, dim, torch.bfloat16)["y"], "bare")
+  assert (y2[n:] == 0).all()
+  dy = rand(rng, (n, dim), torch.bfloat16)
+  _, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, w, batch)
+  dw2, db2 = dw.clone(), db.clone()
+  ops.layer_norm_backward(dy, x, mean, rstd, w, batch, dweight=dw2, dbias=db2, accumulate=True)
+  check(dw2, 2 * dw, 4 * n * U32 * dw.abs().double().cpu().max() + 1e-30, "accumulated")
+  check(db2, 2 * db, 4 * n * U32 * db.abs().double().cpu().max() + 1e-30, "accumulated bias")
+
+
+def test_layer_norm_constant_rows_and_nan(gpu):
+  """A constant row's variance is zero (y = bias); a NaN stays in its row and client."""
+  batch = ops.ClientBatch([2, 2])
+  x = torch.full((4, 64), 3.0, device=gpu)
+  x[3, 5] = math.nan
+  w = torch.ones(2, 64, device=gpu)
+  b = torch.full((2, 64), 0.5, device=gpu)
+  y, mean, rstd = ops.layer_norm(x, w, b, batch)
+  assert (y[:3] == 0.5).all() and y[3].isnan().all()
+  _, dw, _ = ops.layer_norm_backward(torch.ones_like(x), x, mean, rstd, w, batch)
+  assert (dw[0] == 0).all() and dw[1].isnan().all()
+
+
+# --- linear ----------------------------------------------------------------------
+
+ACTS = {
+    None: (lambda z: z, lambda z: torch.ones_like(z)),
+    "relu": (lambda z: z.clamp(min=0), lambda z: (z > 0).double()),
+    "gelu": (lambda z: 0.5 * z * torch.special.erfc(-z / math.sqrt(2)),
+             lambda z: 0.5 * torch.special.erfc(-z / math.sqrt(2)) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)),
+    "silu": (lambda z: z * torch.sigmoid(z),
+             lambda z: torch.sigmoid(z) * (1 + z * (1 - torch.sigmoid(z)))),
+}
+
+
+def linear_reference(x, w, counts):
+  """(z, bound of its float32 sum) per row."""
+  x, w = x.double().cpu(), w.double().cpu()
+  z, mag = [], []
+  for c, (lo, hi) in enumerate(spans(counts)):
+    z.append(x[lo:hi] @ w[c].t())
+    mag.append(x[lo:hi].abs() @ w[c].abs().t())
+  return torch.cat(z), torch.cat(mag) * (2 * x.shape[1] * U32)
+
+
+def check_linear(gpu, rng, counts, k, m, dtype, act, shared=False, scale=None, behind=0):
+  n = sum(counts)
+  batch = ops.ClientBatch(counts)
+  x = rand(rng, (n + behind, k), dtype)
+  dz = rand(rng, (n + behind, m), dtype, 0.5)
+  if behind:
+    x[n:], dz[n:] = math.nan, math.nan
+  w, b = flat_params(rng, len(counts), [(m, k), (m,)], dtype, scale or 1 / math.sqrt(k), shared=shared)
+  res, before = rand(rng, (n, m), dtype), rand(rng, (n, k), dtype)
+  below = rand(rng, (n, k), dtype)
+  client = torch.from_numpy(np.repeat(np.arange(len(counts)), counts))
+  f, slope = ACTS[act]
+  u = unit(dtype)
+
+  y, z = ops.linear(x, w, b, batch, activation=act, residual=res if behind == 0 else None, preactivation=True)
+  zr, ez = linear_reference(x[:n], w, counts)
+  zr = zr + b.double().cpu()[client]
+  ez = ez + 2 * U32 * zr.abs()
+  check(z[:n], zr, ez + u * (zr.abs() + ez) + tiny(dtype), "z")
+  yr = f(zr) + (res.double().cpu() if behind == 0 else 0)
+  # the activations' slopes stay below 1.13; their own evaluation a few roundings of z
+  ey = 1.13 * ez + 16 * U32 * zr.abs() + 2 * U32 * (yr.abs() + 4)
+  check(y[:n], yr, ey + u * (yr.abs() + ey) + tiny(dtype), "y")
+  if behind:
+    assert (y[n:] == 0).all() and (z[n:] == 0).all()
+
+  dx = ops.linear_backward_input(dz, w, batch, preactivation=before if act else None, activation=act,
+                                 residual=below if behind == 0 else None)
+  wt = w.double().cpu().transpose(1, 2)
+  gr, eg = linear_reference(dz[:n], wt, counts)
+  sl = slope(before.double().cpu()) if act else torch.ones(n, k, dtype=torch.float64)
+  want = gr * sl + (below.double().cpu() if behind == 0 else 0)
+  e = eg * sl.abs() + 16 * U32 * gr.abs() * (1 + before.double().cpu().abs()) + 2 * U32 * want.abs()
+  check(dx[:n], want, e + u * (want.abs() + e) + tiny(dtype), "dx")
+
+  rows = torch.full((len(counts), m * k + m + 2), 3.0, device=gpu)
+  dw, db = ops.linear_backward_weight(dz, x, batch, dweight=rows[:, 1:1 + m * k].unflatten(1, (m, k)),
+                                      dbias=rows[:, 1 + m * k:1 + m * k + m])
+  for c, (lo, hi) in enumerate(spans(counts)):
+    d, xx = dz[lo:hi].double().cpu(), x[lo:hi].double().cpu()
+    check(dw[c], d.t() @ xx, 2 * max(1, hi - lo) * U32 * (d.abs().t() @ xx.abs()), "dw of client %d" % c)
+    check(db[c], d.sum(0), 2 * max(1, hi - lo) * U32 * d.abs().sum(0), "db of client %d" % c)
+  assert (rows[:, 0] == 3.0).all() and (rows[:, -1] == 3.0).all()
+  return rows
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("k,m", [(1, 1), (5, 3), (64, 128), (96, 131), (130, 64), (257, 300), (670, 96), (1024, 17)])
+def test_linear_sizes(gpu, dtype, k, m):
+  rng = np.random.default_rng(k * 1000 + m)
+  check_linear(gpu, rng, COUNTS, k, m, dtype, [None, "relu", "gelu", "silu"][(k + m) % 4])
+
+
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_activations(gpu, dtype, act):
+  check_linear(gpu, np.random.default_rng(11), [33, 2], 40, 72, dtype, act, scale=0.7)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("counts", [[1], [1] * 40, [0, 0, 3], [16, 15, 17], [129], [300, 1], [700]])
+def test_linear_row_counts(gpu, dtype, counts):
+  check_linear(gpu, np.random.default_rng(sum(counts)), counts, 136, 200, dtype, "silu")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_long_contractions(gpu, dtype):
+  """Few rows over a long axis, and many rows into a small weight (splits, where taken)."""
+  check_linear(gpu, np.random.default_rng(1), [2, 1], 4100, 36, dtype, "gelu")
+  check_linear(gpu, np.random.default_rng(2), [1], 72, 4099, dtype, None)
+  check_linear(gpu, np.random.default_rng(3), [5000, 3], 24, 40, dtype, "relu")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_shared_weight_and_rows_behind(gpu, dtype):
+  rng = np.random.default_rng(21)
+  check_linear(gpu, rng, [20, 0, 45], 150, 70, dtype, "gelu", shared=True)
+  check_linear(gpu, rng, [20, 0, 45], 150, 70, dtype, None, behind=9)
+
+
+def test_linear_strides_and_accumulation(gpu):
+  rng = np.random.default_rng(5)
+  counts, k, m = [7, 140], 48, 56
+  n = sum(counts)
+  batch = ops.ClientBatch(counts)
+  xw, wide = rand(rng, (n, k + 5), torch.bfloat16), rand(rng, (2, m + 1, k + 9), torch.bfloat16, 0.2)
+  x, w = xw[:, 2:2 + k], wide[:, 1:, 3:3 + k]
+  out = torch.full((n, m + 3), 9.0, dtype=torch.bfloat16, device=gpu)
+  y = ops.linear(x, w, None, batch, out=out[:, 1:1 + m])
+  assert torch.equal(y, ops.linear(x.contiguous(), w.contiguous(), None, batch))
+  assert (out[:, 0] == 9.0).all() and (out[:, m + 1:] == 9.0).all()
+  dz = rand(rng, (n, m), torch.bfloat16)
+  dw, db = ops.linear_backward_weight(dz, x, batch)
+  dw2, db2 = dw.clone(), db.clone()
+  ops.linear_backward_weight(dz, x, batch, dweight=dw2, dbias=db2, accumulate=True)
+  assert torch.equal(dw2, 2 * dw) and torch.equal(db2, 2 * db)
+  dw3, none = ops.linear_backward_weight(dz, x, batch, bias=False)
+  assert none is None and torch.equal(dw3, dw)
+
+
+def test_linear_nan_and_infinity_stay_in_their_rows(gpu):
+  batch = ops.ClientBatch([3, 3])
+  x = torch.ones(6, 40, device=gpu)
+  x[1, 3], x[4, 0] = math.nan, math.inf
+  w = torch.ones(2, 50, 40, device=gpu)
+  y = ops.linear(x, w, None, batch, activation="relu")
+  assert y[1].isnan().all() and (y[4] == math.inf).all()
+  assert (y[[0, 2, 3, 5]] == 40).all()
+  dw, db = ops.linear_backward_weight(torch.ones(6, 50, device=gpu), x, batch)
+  assert dw[0, :, 3].isnan().all() and (dw[0, :, :3] == 3).all() and (dw[1, :, 0] == math.inf).all()
+  assert (db == 3).all()
+
+
+# --- top logits --------------------------------------------------------------------
+
+
+def top_reference(logits, k, temperature=1.0):
+  a = logits.double().cpu()
+  key = torch.where(a.isnan(), -math.inf, a)
+  # NaN below every number, -inf included: two stable passes
+  order = torch.sort(torch.where(a.isnan(), 1, 0), dim=1, stable=True).indices
+  by = torch.sort(torch.gather(key, 1, order), dim=1, descending=True, stable=True).indices
+  return torch.gather(order, 1, by)[:, :k], torch.logsumexp(a / temperature, 1)
+
+
+def check_top(logits, k, temperature=1.0):
+  index, values, lse = ops.top_logits(logits, k, temperature)
+  want, want_lse = top_reference(logits, k, temperature)
+  assert torch.equal(index.long().cpu(), want)
+  got = torch.gather(logits, 1, index.long())
+  assert torch.equal(values.nan_to_num(nan=7e4), got.nan_to_num(nan=7e4))
+  finite = want_lse.isfinite()
+  assert torch.equal(lse.cpu()[~finite].double().nan_to_num(nan=5.0), want_lse[~finite].nan_to_num(nan=5.0))
+  a = logits.double().cpu()[finite]
+  if a.numel():
+    # the sum: vocab / 1024 + 16 + 20 additions of terms whose exponents are off by two
+    # roundings of at most the row's span; then the maximum's product and the log
+    span = torch.where(a.isinf(), 0.0, a / temperature).abs().amax(1)
+    tol = (a.shape[1] / 1024 + 48 + 4 * span) * 2 * U32
+    check(lse[finite.to(lse.device)], want_lse[finite], tol, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("vocab,k", [(1, 1), (7, 7), (100, 3), (1000, 64), (1025, 1024), (10004, 10), (10004, 1000),
+                                     (40000, 128), (131072, 64)])
+def test_top_logits_sizes(gpu, dtype, vocab, k):
+  rng = np.random.default_rng(vocab + k)
+  check_top(rand(rng, (5, vocab), dtype, 3.0), k, 1.0 if k % 2 else 1.7)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_top_logits_ties_infinities_nan(gpu, dtype):
+  """Whole rows of ties (more than are ranked at once), signed zeros, -inf, NaN, +inf."""
+  rng = np.random.default_rng(4)
+  v = 9001
+  x = rand(rng, (12, v), dtype)
+  x[0] = 1.0
+  x[1] = -math.inf
+  x[2] = math.nan
+  x[3, 100:] = -math.inf
+  x[4] = 0.0
+  x[4, ::2] = -0.0
+  x[5] = torch.round(x[5].float()).to(dtype)
+  x[6, 17] = math.nan
+  x[7, 50], x[7, 4000] = math.inf, math.inf
+  x[8] = -math.inf
+  x[8, 8999] = 2.0
+  x[9] = torch.arange(v, device=gpu).flip(0).to(dtype) / 64
+  x[10, :5000] = math.nan
+  x[11] = (torch.arange(v, device=gpu) % 2).to(dtype)
+  for k in (1, 33, 700):
+    check_top(x, k)
+
+
+def test_top_logits_strides_and_no_rows(gpu):
+  rng = np.random.default_rng(9)
+  wide = rand(rng, (6, 3000), torch.bfloat16)
+  check_top(wide[::2, 5:2505], 20)
+  index, values, lse = ops.top_logits(wide[:0], 4)
+  assert index.shape == (0, 4) and values.shape == (0, 4) and lse.shape == (0,)
+
+
+# --- distillation --------------------------------------------------------------------
+
+
+def distill_reference(logits, index, values, counts, tau, teacher_lse=None, weights=None, dloss=None):
+  """(loss, gradient, bound of each) in float64, row by row."""
+  n = sum(counts)
+  s = logits[:n].double().cpu() / tau
+  v = s.shape[1]
+  loss = torch.zeros(len(counts), dtype=torch.float64)
+  e_loss = torch.zeros(len(counts), dtype=torch.float64)
+  grad, e_grad = torch.zeros_like(s), torch.zeros_like(s)
+  for c, (lo, hi) in enumerate(spans(counts)):
+    for r in range(lo, hi):
+      w = 1.0 / (hi - lo) if weights is None else float(weights[r])
+      entries = [(int(j), float(t) / tau) for j, t in zip(index[r].cpu(), values[r].double().cpu())
+                 if 0 <= int(j) < v and float(t) != -math.inf]
+      if not entries or w == 0:
+        continue
+      t = torch.tensor([t for _, t in entries], dtype=torch.float64)
+      j = torch.tensor([j for j, _ in entries])
+      L = torch.logsumexp(t, 0) if teacher_lse is None else float(teacher_lse[r])
+      p = torch.exp(t - L)
+      lse = torch.logsumexp(s[r], 0)
+      q = torch.exp(s[r] - lse)
+      term = p * (torch.log(p) - (s[r][j] - lse))
+      loss[c] += w * tau * tau * term.sum()
+      pr = torch.zeros(v, dtype=torch.float64).index_add(0, j, p)
+      scale = w * tau * (1.0 if dloss is None else float(dloss[c]))
+      grad[r] = scale * (p.sum() * q - pr)
+      # errors of exponents: the arguments' roundings (a few u of their size), the
+      # log-sum-exp's own sum (vocab / 256 + 32 additions)
+      size = float(s[r][s[r].isfinite()].abs().max() + t.abs().max() + lse.abs() + abs(float(L)))
+      d = (6 * size + v / 256 + 2 * len(t) + 48) * 2 * U32
+      mag = (p * (torch.log(p).abs() + (s[r][j] - lse).abs())).sum() + 2 * p.sum()
+      e_loss[c] += w * tau * tau * float(mag) * (2 * d + (hi - lo + 8) * U32)
+      e_grad[r] = abs(scale) * (p.sum() * q + pr) * (2 * d + 8 * U32)
+  return loss, grad, e_loss, e_grad
+
+
+def teacher_rows(rng, n, v, k, pad=0.25, gpu="cuda"):
+  index = torch.stack([torch.from_numpy(rng.permutation(v)[:k] if k <= v else rng.integers(0, v, k)) for _ in range(n)])
+  values = torch.from_numpy(np.sort(rng.standard_normal((n, k)) * 3)[:, ::-1].copy()).float()
+  if pad:
+    index[torch.from_numpy(rng.random((n, k)) < pad)] = -1
+  return index.int().to(gpu), values.to(gpu)
+
+
+def check_distill(logits, index, values, counts, tau=1.0, **kw):
+  batch = ops.ClientBatch(counts)
+  dtype, n = logits.dtype, sum(counts)
+  weights, teacher_lse = kw.get("row_weights"), kw.get("teacher_lse")
+  loss, grad, el, eg = distill_reference(logits, index, values, counts, tau, teacher_lse, weights)
+  el, eg = el + 1e-30, eg + unit(dtype) * (grad.abs() + eg) + tiny(dtype)
+  got, lse = ops.distillation(logits, index, values, batch, temperature=tau, **kw)
+  check(got, loss, el, "loss")
+  fused, dfused = ops.distillation_with_gradient(logits, index, values, batch, temperature=tau, **kw)
+  check(fused, loss, el, "fused loss")
+  check(dfused[:n], grad, eg, "fused gradient")
+  dback = ops.distillation_backward(logits, lse, index, values, batch, temperature=tau, **kw)
+  check(dback[:n], grad, eg, "gradient")
+  dloss = torch.linspace(-1.0, 2.0, len(counts), device=logits.device)
+  _, grad2, _, eg2 = distill_reference(logits, index, values, counts, tau, teacher_lse, weights, dloss)
+  check(ops.distillation_backward(logits, lse, index, values, batch, temperature=tau, dloss=dloss, **kw)[:n], grad2,
+        eg2 + unit(dtype) * (grad2.abs() + eg2) + tiny(dtype), "scaled gradient")
+  copy = logits.clone()
+  _, inplace = ops.distillation_with_gradient(copy, index, values, batch, temperature=tau, out=copy, **kw)
+  assert torch.equal(inplace[:n], dfused[:n])
+  copy = logits.clone()
+  assert torch.equal(ops.distillation_backward(copy, lse, index, values, batch, temperature=tau, out=copy, **kw)[:n],
+                     dback[:n])
+  return dfused
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("vocab,k", [(1, 1), (5, 5), (50, 8), (1000, 32), (10004, 64), (33333, 1)])
+def test_distillation_sizes(gpu, dtype, vocab, k):
+  rng = np.random.default_rng(vocab * 7 + k)
+  counts = [3, 0, 4, 1]
+  logits = rand(rng, (8, vocab), dtype, 2.0)
+  index, values = teacher_rows(rng, 8, vocab, k)
+  check_distill(logits, index, values, counts, tau=2.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_distillation_options(gpu, dtype):
+  """The teacher's own lse, row weights (one of them zero over NaN logits), -inf values."""
+  rng = np.random.default_rng(31)
+  counts, v, k = [2, 5], 700, 16
+  logits = rand(rng, (7, v), dtype, 2.0)
+  index, values = teacher_rows(rng, 7, v, k)
+  values[1, 3:] = -math.inf
+  lse = torch.logsumexp(values / 1.5, 1) + 0.3
+  check_distill(logits, index, values, counts, tau=1.5, teacher_lse=lse)
+  weights = torch.tensor([0.5, 0.0, 1.0, 2.0, 0.0, 1.0, 0.25], device=gpu)
+  logits[1] = math.nan
+  grad = check_distill(logits, index, values, counts, tau=0.7, row_weights=weights)
+  assert (grad[1] == 0).all() and (grad[4] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_distillation_empty_rows_repeats_and_masks(gpu, dtype):
+  """Rows of nothing but padding (over NaN logits), an index that comes twice, indices
+  outside the vocabulary, student logits of -inf."""
+  rng = np.random.default_rng(8)
+  counts, v, k = [4, 1, 3], 300, 8
+  logits = rand(rng, (8, v), dtype, 2.0)
+  index, values = teacher_rows(rng, 8, v, k, pad=0)
+  index[0] = -1
+  logits[0] = math.nan
+  index[4] = v  # the second client has nothing
+  index[1, 2], index[1, 6] = index[1, 0], index[1, 0]
+  index[2, :4] = torch.tensor([v, -7, 2**31 - 1, -2**31])
+  mask = torch.ones(v, dtype=torch.bool, device=gpu)
+  mask[index[3].long()] = False
+  logits[3] = torch.where(mask, -math.inf, logits[3])
+  grad = check_distill(logits, index, values, counts)
+  assert (grad[0] == 0).all() and (grad[4] == 0).all()
+  # an index repeated: the same as one entry of the summed probability
+  batch = ops.ClientBatch([1])
+  one = torch.tensor([[5, 5]], dtype=torch.int32, device=gpu)
+  l2, _ = ops.distillation_with_gradient(logits[5:6], one, torch.zeros(1, 2, device=gpu), batch)
+  g1 = ops.distillation_with_gradient(logits[5:6], one[:, :1].contiguous(), torch.zeros(1, 1, device=gpu), batch)
+  assert abs(float(l2) - (float(g1[0]) - math.log(2))) < 1e-5
+
+
+def test_distillation_student_without_distribution(gpu):
+  """All of a row's logits -inf: an infinite loss, and the teacher's side of the gradient."""
+  batch = ops.ClientBatch([1])
+  logits = torch.full((1, 40), -math.inf, device=gpu)
+  index = torch.tensor([[3, 9]], dtype=torch.int32, device=gpu)
+  loss, grad = ops.distillation_with_gradient(logits, index, torch.zeros(1, 2, device=gpu), batch)
+  assert float(loss) == math.inf
+  want = torch.zeros(1, 40)
+  want[0, [3, 9]] = -0.5
+  check(grad, want, 4 * U32, "gradient")
+
+
+def test_distillation_gradient_by_differences(gpu):
+  """Central differences of the float32 loss: step h = 2^-6 leaves h^2 / 6 of a third
+  derivative below 2 w tau^2 / tau^3, and 2 u |loss| / h from the loss's own rounding."""
+  rng = np.random.default_rng(77)
+  v, tau, h = 24, 1.5, 2.0**-6
+  batch = ops.ClientBatch([1, 1])
+  logits = rand(rng, (2, v), torch.float32)
+  index, values = teacher_rows(rng, 2, v, 4, pad=0)
+  loss, grad = ops.distillation_with_gradient(logits, index, values, batch, temperature=tau)
+  for j in range(v):
+    up, down = logits.clone(), logits.clone()
+    up[:, j] += h
+    down[:, j] -= h
+    a = ops.distillation(up, index, values, batch, temperature=tau)[0].double()
+    b = ops.distillation(down, index, values, batch, temperature=tau)[0].double()
+    tol = 2 / tau * h * h / 6 + (64 * U32 * (loss.double().abs() + 10)) / h
+    check((a - b) / (2 * h), grad[:, j], tol.cpu(), "column %d" % j)
+
+
+# --- together ------------------------------------------------------------------------
+
+
+class Step:
+  """One client step of a residual block and a head under a teacher's top logits: the
+  operators as they are used, gradients in the clients' flat rows."""
+
+  def __init__(self, rng, counts, dtype, d=40, hidden=88, v=121, shared=False, gpu="cuda"):
+    self.counts, self.dtype = counts, dtype
+    self.sizes = [(d,), (d,), (hidden, d), (hidden,), (d, hidden), (d,), (v, d), (v,)]
+    self.P = sum(int(np.prod(s)) for s in self.sizes)
+    c = len(counts)
+    rows = rand(rng, (1 if shared else c, self.P), dtype, 0.2).expand(c, self.P)
+    self.params = self.views(rows)
+    self.update = torch.zeros(c, self.P, device=gpu)
+    self.grads = self.views(self.update)
+    n = sum(counts)
+    self.batch = ops.ClientBatch(counts)
+    self.x = rand(rng, (n, d), dtype)
+    teacher = rand(rng, (n, v), torch.float32, 3.0)
+    self.index, self.values, self.lse = ops.top_logits(teacher, 12, temperature=2.0)
+
+  def views(self, rows):
+    out, at = [], 0
+    for s in self.sizes:
+      k = int(np.prod(s))
+      out.append(rows[:, at:at + k].unflatten(1, s) if len(s) > 1 else rows[:, at:at + k])
+      at += k
+    return out
+
+  def run(self):
+    g, b, w1, b1, w2, b2, w3, b3 = self.params
+    dg, db, dw1, db1, dw2, db2, dw3, db3 = self.grads
+    batch = self.batch
+    h, mean, rstd = ops.layer_norm(self.x, g, b, batch)
+    a, z = ops.linear(h, w1, b1, batch, activation="gelu", preactivation=True)
+    y = ops.linear(a, w2, b2, batch, residual=self.x)
+    logits = ops.linear(y, w3, b3, batch)
+    loss, dlogits = ops.distillation_with_gradient(logits, self.index, self.values, batch, temperature=2.0,
+                                                   teacher_lse=self.lse, out=logits)
+    ops.linear_backward_weight(dlogits, y, batch, dweight=dw3, dbias=db3)
+    dy = ops.linear_backward_input(dlogits, w3, batch)
+    ops.linear_backward_weight(dy, a, batch, dweight=dw2, dbias=db2)
+    dz = ops.linear_backward_input(dy, w2, batch, preactivation=z, activation="gelu")
+    ops.linear_backward_weight(dz, h, batch, dweight=dw1, dbias=db1)
+    dh = ops.linear_backward_input(dz, w1, batch)
+    dx, _, _ = ops.layer_norm_backward(dh, self.x, mean, rstd, g, batch, residual=dy, dweight=dg, dbias=db)
+    return loss, dx
+
+  def autograd(self):
+    """The same step in float64 by torch's own differentiation, client by client."""
+    params = [p.double().cpu().clone().requires_grad_() for p in self.params]
+    x = self.x.double().cpu().requires_grad_()
+    losses = []
+    for c, (lo, hi) in enumerate(spans(self.counts)):
+      if lo == hi:
+        losses.append(torch.zeros((), dtype=torch.float64))
+        continue
+      g, b, w1, b1, w2, b2, w3, b3 = [p[c] for p in params]
+      xc = x[lo:hi]
+      hc = torch.nn.functional.layer_norm(xc, (xc.shape[1],), g, b)
+      y = torch.nn.functional.gelu(hc @ w1.t() + b1) @ w2.t() + b2 + xc
+      logq = torch.log_softmax((y @ w3.t() + b3) / 2.0, 1)
+      p = torch.exp(self.values[lo:hi].double().cpu() / 2.0 - self.lse[lo:hi].double().cpu()[:, None])
+      losses.append(4.0 * (p * (torch.log(p) - torch.gather(logq, 1, self.index[lo:hi].long().cpu()))).sum(1).mean())
+    loss = torch.stack(losses)
+    grads = torch.autograd.grad(loss.sum(), params + [x])
+    return loss, grads[-1], grads[:-1]
+
+
+@pytest.mark.parametrize("shared", [False, True], ids=["own", "shared"])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_step_gradients(gpu, dtype, shared):
+  """The whole step against float64 autograd.  Every stored activation and gradient is
+  rounded to the type once; a parameter's gradient passes at most 10 such roundings,
+  each relative to its own tensor, so 10 u (plus float32's sums) of the gradient's
+  norm, four times for the products of perturbed factors, bounds its error's norm."""
+  step = Step(np.random.default_rng(6), [12, 0, 33, 1], dtype, shared=shared)
+  loss, dx = step.run()
+  want_loss, want_dx, want = step.autograd()
+  bound = 4 * (10 * unit(dtype) + 400 * U32)
+  for got, ref in [(loss, want_loss), (dx, want_dx)] + list(zip(step.grads, want)):
+    ref = ref.double()
+    err = (got.double().cpu() - ref).norm()
+    assert float(err) <= bound * float(ref.norm()), (got.shape, float(err), float(ref.norm()))
+  assert (step.update[1] == 0).all()
+
+
+def test_step_feeds_the_codec(gpu):
+  """The step's rows go through the default aggregator as they lie, bit for bit the
+  oracle's round."""
+  from federated_amd.aggregators import quantize_encode  # pylint: disable=g-import-not-at-top
+  from oracle import aggregators as oagg  # pylint: disable=g-import-not-at-top
+  step = Step(np.random.default_rng(16), [9, 4, 20], torch.bfloat16)
+  step.run()
+  step.update.mul_(50.0)
+  seeds = np.array([[1, 2], [3, 4], [5, 6]], np.int64)
+  process = quantize_encode.QuantizeEncodeFactory(0.05, rounding_type="stochastic").create((np.float32, (step.P,)))
+  out = process.next(process.initialize(), step.update, seeds=seeds)
+  want, meas, _ = oagg.quantize_encode_next([r.cpu().numpy() for r in step.update], 0.05, "stochastic", seeds=seeds)
+  assert np.array_equal(out.result.cpu().numpy(), want)
+  assert out.measurements["avg_bitrate"] == meas["avg_bitrate"]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_step_twice_is_bitwise_equal_and_graph_replays(gpu, dtype):
+  """Two eager runs agree bit for bit; a captured step replays with new inputs in
+  place, eager work between the replays; two graphs share nothing."""
+  step = Step(np.random.default_rng(26), [40, 3, 0, 77], dtype)
+  other = Step(np.random.default_rng(27), [15, 60], dtype)
+
+  def eager(s):
+    loss, dx = s.run()
+    torch.cuda.synchronize()
+    return [t.clone() for t in (loss, dx, s.update)]
+
+  a, b = eager(step), eager(step)
+  assert all(torch.equal(p, q) for p, q in zip(a, b))
+  stream = torch.cuda.Stream()
+  stream.wait_stream(torch.cuda.current_stream())
+  graphs = []
+  with torch.cuda.stream(stream):
+    for s in (step, other):
+      s.run()
+    torch.cuda.synchronize()
+    for s in (step, other):
+      g = torch.cuda.CUDAGraph()
+      with torch.cuda.graph(g, stream=stream):
+        out = s.run()
+      graphs.append((g, s, out))
+  torch.cuda.synchronize()
+  rng = np.random.default_rng(5)
+  for _ in range(4):
+    for g, s, out in graphs:
+      s.x.copy_(rand(rng, tuple(s.x.shape), dtype))
+      want = eager(s)
+      s.update.fill_(-1.0)
+      g.replay()
+      graphs[1 - [h[0] for h in graphs].index(g)][0].replay()  # the other graph right behind it
+      torch.cuda.synchronize()
+      assert all(torch.equal(p, q) for p, q in zip((out[0], out[1], s.update), want))
+
+
+def test_step_on_another_stream(gpu):
+  step = Step(np.random.default_rng(36), [25, 31], torch.bfloat16)
+  loss, dx = step.run()
+  want = [t.clone() for t in (loss, dx, step.update)]
+  step.update.zero_()
+  s = torch.cuda.Stream()
+  s.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(s):
+    loss, dx = step.run()
+  s.synchronize()
+  assert all(torch.equal(p, q) for p, q in zip((loss, dx, step.update), want))
+
+
+def test_batches_without_rows(gpu):
+  batch = ops.ClientBatch([0, 0])
+  x = torch.empty(0, 8, device=gpu)
+  w = torch.ones(2, 5, 8, device=gpu)
+  y, _, _ = ops.layer_norm(x, None, None, batch)
+  assert y.shape == (0, 8) and ops.linear(x, w, None, batch).shape == (0, 5)
+  dw, db = ops.linear_backward_weight(torch.empty(0, 5, device=gpu), x, batch)
+  assert (dw == 0).all() and (db == 0).all() and dw.shape == (2, 5, 8)
+  assert ops.linear_backward_input(torch.empty(0, 5, device=gpu), w, batch).shape == (0, 8)
+  idx = torch.empty(0, 3, dtype=torch.int32, device=gpu)
+  loss, grad = ops.distillation_with_gradient(x, idx, torch.empty(0, 3, device=gpu), batch)
+  assert (loss == 0).all() and grad.shape == (0, 8)
+  st = torch.empty(0, device=gpu)
+  _, dg, dbt = ops.layer_norm_backward(x, x, st, st, None, batch)
+  assert (dg == 0).all() and (dbt == 0).all()
+
+
+# --- refusals ------------------------------------------------------------------------
+
+
+def test_batch_refusals(gpu):
+  for bad in ([], [[1, 2]], [1.5], [-1, 2], [1 << 31]):
+    with pytest.raises(ValueError):
+      ops.ClientBatch(bad)
+  with pytest.raises(ValueError):
+    ops.ClientBatch([1], device="cpu")
+
+
+def test_operator_refusals(gpu):
+  batch = ops.ClientBatch([3, 2])
+  x = torch.zeros(5, 8, device=gpu)
+  w, b = torch.zeros(2, 6, 8, device=gpu), torch.zeros(2, 6, device=gpu)
+  dz = torch.zeros(5, 6, device=gpu)
+  idx = torch.zeros(5, 2, dtype=torch.int32, device=gpu)
+  val = torch.zeros(5, 2, device=gpu)
+  one = torch.zeros(1, device=gpu)
+  st = torch.zeros(5, device=gpu)
+  calls = [
+      lambda: ops.layer_norm(x[:4], None, None, batch),  # too few rows
+      lambda: ops.layer_norm(x.cpu(), None, None, batch),
+      lambda: ops.layer_norm(x.double(), None, None, batch),
+      lambda: ops.layer_norm(x.t().contiguous().t(), None, None, batch),
+      lambda: ops.layer_norm(x[None], None, None, batch),
+      lambda: ops.layer_norm(x, torch.zeros(2, 7, device=gpu), None, batch),
+      lambda: ops.layer_norm(x, torch.zeros(3, 8, device=gpu), None, batch),
+      lambda: ops.layer_norm(x, torch.zeros(2, 8, device=gpu).half(), None, batch),
+      lambda: ops.layer_norm(x, None, None, batch, out=one.expand(5, 8)),
+      lambda: ops.layer_norm_backward(x, x, st[:4], st, None, batch),
+      lambda: ops.layer_norm_backward(x.half(), x, st, st, None, batch),
+      lambda: ops.layer_norm_backward(x, x, st, st, None, batch, accumulate=True),
+      lambda: ops.layer_norm_backward(x, x, st, st, None, batch, dweight=torch.zeros(8, device=gpu).expand(2, 8)),
+      lambda: ops.linear(x, w, b, batch, activation="tanh"),
+      lambda: ops.linear(x, w[:, :, :7], b, batch),
+      lambda: ops.linear(x, w[:1], b, batch),
+      lambda: ops.linear(x, w.half(), b, batch),
+      lambda: ops.linear(x, w.transpose(1, 2).contiguous().transpose(1, 2), b, batch),
+      lambda: ops.linear(x, w, b[:, :5], batch),
+      lambda: ops.linear(x, w, b, batch, residual=x),
+      lambda: ops.linear(x, w, b, batch, out=torch.zeros(5, 7, device=gpu)),
+      lambda: ops.linear_backward_input(dz, w, batch, activation="relu"),
+      lambda: ops.linear_backward_input(dz, w, batch, preactivation=x),
+      lambda: ops.linear_backward_input(x, w, batch),
+      lambda: ops.linear_backward_weight(dz, x.half(), batch),
+      lambda: ops.linear_backward_weight(dz, x, batch, dweight=w.half()),
+      lambda: ops.linear_backward_weight(dz, x, batch, dweight=w[:1].expand(2, 6, 8)),
+      lambda: ops.linear_backward_weight(dz, x, batch, accumulate=True),
+      lambda: ops.linear_backward_weight(dz, x, batch, bias=False, dbias=b),
+      lambda: ops.top_logits(x, 0),
+      lambda: ops.top_logits(x, 9),
+      lambda: ops.top_logits(torch.zeros(1, 2000, device=gpu), 1025),
+      lambda: ops.top_logits(x, 2, temperature=0.0),
+      lambda: ops.top_logits(x.cpu(), 2),
+      lambda: ops.top_logits(x.int(), 2),
+      lambda: ops.distillation(x, idx.long(), val, batch),
+      lambda: ops.distillation(x, idx[:4], val, batch),
+      lambda: ops.distillation(x, idx, val[:, :1], batch),
+      lambda: ops.distillation(x, idx, val, batch, temperature=float("inf")),
+      lambda: ops.distillation(x, idx, val, batch, teacher_lse=st[:3]),
+      lambda: ops.distillation(x, idx, val, batch, row_weights=st.double()),
+      lambda: ops.distillation(x, idx.cpu(), val, batch),
+      lambda: ops.distillation(x, idx.repeat(1, 600), val.repeat(1, 600), batch),
+      lambda: ops.distillation_backward(x, st[:2], idx, val, batch),
+      lambda: ops.distillation_backward(x, st, idx, val, batch, dloss=one),
+      lambda: ops.distillation_with_gradient(x, idx, val, batch, out=dz),
+  ]
+  for i, call in enumerate(calls):
+    with pytest.raises(ValueError):
+      call()
+      pytest.fail("call %d was not refused" % i)
