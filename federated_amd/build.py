@@ -12,6 +12,8 @@ CLIENT_SRCS = [os.path.join(HERE, "csrc", f) for f in ("client_rows.hip", "clien
 CLIENT_HDRS = [os.path.join(HERE, "csrc", "client_common.h")]
 OUT = os.path.join(HERE, "libfedcodec.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+# no packed float32 instructions, in any file: some of their forms are not reliable
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
          # TF-CPU numerics: FTZ/DAZ on float32, no FMA contraction
          "-fgpu-flush-denormals-to-zero", "-ffp-contract=off",
@@ -22,11 +24,9 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
          # after the atomic) made k_encode wait for each ticket atomic -- and every
          # vector memory operation before it -- where it is issued instead of where
          # the ticket is used, a tile later
-         "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
+         "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"] + NO_PACKED_F32
 
 
-# no packed float32 instructions, in any file: some of their forms are not reliable
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 CLIENT_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared"] + NO_PACKED_F32
 
 
