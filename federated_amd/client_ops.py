@@ -23,6 +23,7 @@ Forward and backward are separate calls with explicit gradients: a broadcast wei
 still gets one gradient per client, which is what the codec encodes.
 """
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -31,7 +32,7 @@ from federated_amd import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
-_TILES = (16, 64, 128)
+_TILES = (16, 32, 64, 128, 256)
 MAX_TOP = 1024  # FC_MAX_TOP
 
 
@@ -62,6 +63,7 @@ class ClientBatch:
     self.counts = counts
     self.num_clients = int(counts.size)
     self.num_rows = int(counts.sum())
+    self.longest = int(counts.max())
     ends = np.cumsum(counts)
     # one host buffer, one copy: offsets, row -> client, a table entry per client, tiles
     parts = [np.concatenate([[0], ends]).astype(np.int32),
@@ -266,6 +268,62 @@ def _weight(weight, batch, dtype, inner=None, outer=None):
   return m, k
 
 
+# How long a product takes with tiles of `rows` rows, from one card's measurements (us):
+# a CU's time for one 128-byte k-step of one tile (16-bit types: 1.03 us for two 128 x
+# 128 tiles side by side, 1.8 for one of 256 x 256, 1.2 for four of 32 x 128; float32
+# runs at a fourth of the rate), a tile's start and end, and how many tiles a CU holds.
+# A k-step that waits for memory takes about 0.7 however little it computes.
+_TILE_COSTS = {32: (0.3, 5.0, 4), 128: (0.52, 9.0, 2), 256: (1.8, 12.0, 1)}
+_STEP_LATENCY = 0.7
+_CUS = 256
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan(tiles, steps, longest, size, aligned):
+  """(tile rows, splits of the contraction) of a product, by the lowest estimate.
+
+  ``tiles``: output tiles for each of _TILE_COSTS' heights; ``steps`` / ``longest``: the
+  mean and the largest number of k-steps of a tile.  Splitting pays where there are
+  fewer tiles than the chip holds: 1 x 4096 by 14336 x 4096 (bfloat16) takes 38 us whole
+  and 26 in four parts; where the tiles fill it, it only costs (8 x 2048 rows, 4096 to
+  8192: 2.1 ms whole, 2.9 in four).
+  """
+  best = None
+  for (rows, (step, ends, resident)), count in zip(_TILE_COSTS.items(), tiles):
+    if rows == 256 and (size == 4 or not aligned):
+      continue  # the kernel's limits
+    step *= 4 if size == 4 else 1
+    splits = 1
+    while splits <= 16 and (splits == 1 or 2 * splits <= longest):
+      blocks = max(1, count * splits)
+      per_cu = -(-blocks // _CUS) if blocks < 4 * _CUS else blocks / _CUS
+      rounds = max(1.0, blocks / (_CUS * resident))
+      t = max(per_cu * step * steps, rounds * _STEP_LATENCY * longest) / splits + rounds * ends
+      if splits > 1:  # the parts' write and read, and the joining launch
+        t += 4.0 + 2 * blocks * rows * max(128, rows) * 4 / 4e6
+      if best is None or t < best[0]:
+        best = (t, rows, splits)
+      splits *= 2
+  return best[1:]
+
+
+def _workspace(blocks, rows, splits, device):
+  if splits == 1:
+    return None
+  need = int(_lib.load().fc_linear_workspace_bytes(blocks, rows, splits))
+  return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def _dword_aligned(*tensors):
+  return all((t.data_ptr() | t.stride(0) * t.element_size() | t.stride(-2) * t.element_size()) % 4 == 0 for t in tensors)
+
+
+def _row_plan(batch, columns, contraction, a, weight):
+  tiles = tuple(batch._tiles[h][2] * -(-columns // max(128, h)) for h in _TILE_COSTS)  # pylint: disable=protected-access
+  steps = -(-contraction * a.element_size() // 128)
+  return _plan(tiles, steps, steps, a.element_size(), _dword_aligned(a, weight))
+
+
 def linear(x, weight, bias, batch, activation=None, residual=None, preactivation=False, out=None):
   """y = activation(x weight_c^T + bias_c) + residual, client by client.
 
@@ -283,10 +341,13 @@ def linear(x, weight, bias, batch, activation=None, residual=None, preactivation
     _activations("residual", residual, batch, m, x)
   out = _out("out", out, x, batch, m)
   z = _out("z", None, x, batch, m) if preactivation else None
-  tiles, _, ntiles = batch._tiles[128]  # pylint: disable=protected-access
-  _call(batch.device, "fc_linear", _ptr(x), x.stride(0), _DTYPES[x.dtype], _ptr(tiles), ntiles, batch.num_clients,
-        k, m, _ptr(weight), weight.stride(0), weight.stride(1), _ptr(bias), _ld(bias), act, _ptr(residual),
-        _ld(residual), _ptr(z), _ld(z), _ptr(out), out.stride(0))
+  rows, splits = _row_plan(batch, m, k, x, weight)
+  tiles, _, ntiles = batch._tiles[rows]  # pylint: disable=protected-access
+  ws = _workspace(ntiles * -(-m // max(128, rows)), rows, splits, batch.device)
+  _call(batch.device, "fc_linear", _ptr(x), x.stride(0), _DTYPES[x.dtype], _ptr(tiles), ntiles, rows,
+        batch.num_clients, k, m, _ptr(weight), weight.stride(0), weight.stride(1), _ptr(bias), _ld(bias), act,
+        _ptr(residual), _ld(residual), _ptr(z), _ld(z), _ptr(out), out.stride(0), splits, _ptr(ws),
+        0 if ws is None else ws.numel())
   return (out, z) if preactivation else out
 
 
@@ -307,10 +368,13 @@ def linear_backward_input(dz, weight, batch, preactivation=None, activation=None
   if residual is not None:
     _activations("residual", residual, batch, k, dz)
   out = _out("out", out, dz, batch, k)
-  tiles, _, ntiles = batch._tiles[128]  # pylint: disable=protected-access
-  _call(batch.device, "fc_linear_backward_input", _ptr(dz), dz.stride(0), _DTYPES[dz.dtype], _ptr(tiles), ntiles,
+  rows, splits = _row_plan(batch, k, m, dz, weight)
+  tiles, _, ntiles = batch._tiles[rows]  # pylint: disable=protected-access
+  ws = _workspace(ntiles * -(-k // max(128, rows)), rows, splits, batch.device)
+  _call(batch.device, "fc_linear_backward_input", _ptr(dz), dz.stride(0), _DTYPES[dz.dtype], _ptr(tiles), ntiles, rows,
         batch.num_clients, k, m, _ptr(weight), weight.stride(0), weight.stride(1), act, _ptr(preactivation),
-        _ld(preactivation), _ptr(residual), _ld(residual), _ptr(out), out.stride(0))
+        _ld(preactivation), _ptr(residual), _ld(residual), _ptr(out), out.stride(0), splits, _ptr(ws),
+        0 if ws is None else ws.numel())
   return out
 
 
@@ -331,9 +395,15 @@ def linear_backward_weight(dz, x, batch, dweight=None, dbias=None, bias=True, ac
   dweight = _grad_out("dweight", dweight, batch, (m, k))
   if bias:
     dbias = _grad_out("dbias", dbias, batch, (m,))
+  size = x.element_size()
+  tiles = tuple(batch.num_clients * -(-m // h) * -(-k // max(128, h)) for h in _TILE_COSTS)
+  per = 128 // size
+  rows, splits = _plan(tiles, -(-batch.num_rows // (per * batch.num_clients)), -(-batch.longest // per), size,
+                       _dword_aligned(dz, x))
+  ws = _workspace(batch.num_clients * -(-m // rows) * -(-k // max(128, rows)), rows, splits, batch.device)
   _call(batch.device, "fc_linear_backward_weight", _ptr(dz), dz.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
         _ptr(batch._clients), batch.num_clients, k, m, _ptr(dweight), dweight.stride(0), dweight.stride(1),  # pylint: disable=protected-access
-        _ptr(dbias), _ld(dbias), int(bool(accumulate)))
+        _ptr(dbias), _ld(dbias), int(bool(accumulate)), rows, splits, _ptr(ws), 0 if ws is None else ws.numel())
   return dweight, dbias
 
 

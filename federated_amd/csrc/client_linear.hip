@@ -10,6 +10,8 @@
 // ("KC": a row of 16-byte chunks along k) or along their own index ("XC").
 #include "client_common.h"
 
+#include <type_traits>
+
 namespace {
 
 using namespace fc;
@@ -18,24 +20,54 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kThreads = 256;
-constexpr int kRowBytes = 128;  // a KC tile's row: one k-step of a staged tile
-
 enum Act { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
 
+// The normal distribution function and exp(-z^2 / 2).  float32: erff.  16-bit outputs:
+// Abramowitz & Stegun 7.1.26 (absolute error of erf below 1.5e-7, far under their
+// rounding), a reciprocal, an exponential and five multiply-adds.
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float z, float& bell) {
+  if constexpr (sizeof(T) == 4) {
+    bell = expf(-0.5f * z * z);
+    return 0.5f * (1.0f + erff(z * 0.70710678f));
+  } else {
+    const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+    bell = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+    float q = 1.061405429f;
+    q = q * t - 1.453152027f;
+    q = q * t + 1.421413741f;
+    q = q * t - 0.284496736f;
+    q = q * t + 0.254829592f;
+    q *= 0.5f * t * bell;  // half of erfc(|z| / sqrt 2)
+    return z < 0.0f ? q : 1.0f - q;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float logistic(float z) {
+  if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
+  else return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * z));
+}
+
+template <typename T>
 __device__ __forceinline__ float act_value(int act, float z) {
+  float bell;
   if (act == kRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  if (act == kGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-  if (act == kSilu) return z / (1.0f + expf(-z));
+  if (act == kGelu) return z * normal_cdf<T>(z, bell);
+  if (act == kSilu) return z * logistic<T>(z);
   return z;
 }
 
+template <typename T>
 __device__ __forceinline__ float act_slope(int act, float z) {
   if (act == kRelu) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-  if (act == kGelu)
-    return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
+  if (act == kGelu) {
+    float bell;
+    const float cdf = normal_cdf<T>(z, bell);
+    return cdf + z * 0.39894228f * bell;
+  }
   if (act == kSilu) {
-    const float s = 1.0f / (1.0f + expf(-z));
+    const float s = logistic<T>(z);
     return s * (1.0f + z * (1.0f - s));
   }
   return 1.0f;
@@ -59,16 +91,41 @@ template <> __device__ __forceinline__ f32x4 mma<float>(VecOf<float>::type j, Ve
   return acc;
 }
 
-// A staged operand tile of X indices by one k-step (128 bytes of k).
-//  KC: [X][128 B], 16-byte chunk c of row x at chunk c ^ (x & 7).
+// 16 bytes per lane from base + off straight to LDS (dword-aligned source): lane l's land
+// at lds + 16 l.  Untracked by the compiler: the caller waits for vmcnt(0).
+__device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+               : "memory");
+}
+
+__device__ __forceinline__ void load_lds16_at(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+}
+
+// The thread's number, to the compiler a new value each time: addresses made from it
+// are not carried in registers through the main loop.
+__device__ __forceinline__ int hidden_thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// A staged operand tile of X indices by one k-step of 128 bytes of k, NT threads.
+//  KC: [X][128 bytes], 16-byte chunk c of row x at chunk c ^ turn(x).
 //  XC: [k][X], groups of 16 indices of row k at group g ^ swz(k).
-template <typename T, int X, bool KC>
+template <typename T, int X, bool KC, int NT>
 struct Stage {
+  static constexpr int ROW = 128;
   static constexpr int kVec = Elem<T>::kVec;
-  static constexpr int kK = kRowBytes / (int)sizeof(T);  // k per staged tile
-  static constexpr int kChunks = X * 8 / kThreads;       // 16-byte chunks per thread (either layout)
-  static constexpr int kBytes = X * kRowBytes;
+  static constexpr int kK = ROW / (int)sizeof(T);   // k per staged tile
+  static constexpr int kPer = ROW / 16;             // chunks per KC row
+  static constexpr int kChunks = X * kPer / NT;  // 16-byte chunks per thread (either layout)
+  static constexpr int kBytes = X * ROW;
   typedef typename VecOf<T>::type vec;
+
+  // A 16-byte read takes lanes {0-3, 12-15, 20-23, 24-27}, then {4-7, 8-11, 16-19, 28-31},
+  // and so on in the upper half, at once (measured): their 16 chunks then cover all banks.
+  static __device__ __forceinline__ int turn(int x) { return x & 7; }
 
   static __device__ __forceinline__ int swz(int k) {
     // the rows one read instruction touches differ in these bits
@@ -77,8 +134,8 @@ struct Stage {
   }
 
   static __device__ __forceinline__ int slot(int s) {  // byte offset of this thread's chunk s
-    const int q = threadIdx.x + s * kThreads;
-    if (KC) return (q >> 3) * kRowBytes + (((q & 7) ^ ((q >> 3) & 7)) << 4);
+    const int q = threadIdx.x + s * NT;
+    if (KC) return (q / kPer) * ROW + (((q % kPer) ^ turn(q / kPer)) << 4);
     constexpr int kPerRow = X / kVec;  // chunks per k row
     const int k = q / kPerRow, c = q % kPerRow;
     constexpr int kPerGroup = 16 / kVec;
@@ -89,10 +146,10 @@ struct Stage {
   static __device__ __forceinline__ void load(vec (&r)[kChunks], const T* base, int64_t ld, int nx, int64_t nk) {
 #pragma unroll
     for (int s = 0; s < kChunks; ++s) {
-      const int q = threadIdx.x + s * kThreads;
+      const int q = threadIdx.x + s * NT;
       if (KC) {
-        const int x = min(q >> 3, nx - 1);  // rows past the end repeat the last: their outputs are not stored
-        const int k = (q & 7) * kVec;
+        const int x = min(q / kPer, nx - 1);  // rows past the end repeat the last: their outputs are not stored
+        const int k = (q % kPer) * kVec;
         r[s] = load_vec(base + x * ld + k, nk - k);
       } else {
         constexpr int kPerRow = X / kVec;
@@ -107,32 +164,120 @@ struct Stage {
     for (int s = 0; s < kChunks; ++s) *(vec*)(lds + slot(s)) = r[s];
   }
 
-  // Fragment of indices [x0, x0 + 16), k chunk-step ks (64 bytes of k: 4 chunks).
-  static __device__ __forceinline__ vec frag(const char* lds, int x0, int ks) {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    if (KC) {
-      const int x = x0 + (lane & 15);
-      return *(const vec*)(lds + x * kRowBytes + (((ks * 4 + g) ^ (x & 7)) << 4));
+  // Direct to LDS: wave w's instruction s fills bytes [NT 16 s + 1024 w, + 1024) in lane
+  // order, so the swizzle is applied to the source.  Byte offsets of this thread's
+  // chunks from the tile's base; indices past the end repeat a valid one.  An XC tile
+  // whose chunks lie a multiple of 16 ks apart (swz's period) needs the first alone.
+  static constexpr int kChunkRows = KC ? NT / kPer : NT * kVec / X;
+  static constexpr int kOffsets = !KC && kChunkRows % 16 == 0 ? 1 : kChunks;
+  static __device__ __forceinline__ void offsets(uint32_t (&o)[kOffsets], int64_t ld, int nx) {
+#pragma unroll
+    for (int s = 0; s < kOffsets; ++s) {
+      int x, k;
+      source(s, threadIdx.x, x, k);
+      if (KC) x = min(x, nx - 1);
+      else if (x >= nx) x = 0;
+      o[s] = (uint32_t)((KC ? x * ld + k : k * ld + x) * (int64_t)sizeof(T));
     }
+  }
+
+  // Index and k of the chunk that lands in this thread's LDS slot s.
+  static __device__ __forceinline__ void source(int s, int tid, int& x, int& k) {
+    const int q = tid + s * NT;
+    if (KC) {
+      x = q / kPer;
+      k = ((q % kPer) ^ turn(x)) * kVec;
+    } else {
+      constexpr int kPerRow = X / kVec, kPerGroup = 16 / kVec;
+      const int c = q % kPerRow;
+      k = q / kPerRow;
+      x = (((c / kPerGroup) ^ swz(k)) * kPerGroup + c % kPerGroup) * kVec;
+    }
+  }
+
+  static __device__ __forceinline__ void direct(const uint32_t (&o)[kOffsets], const T* base, int64_t ld,
+                                                const char* lds) {
+    const uint32_t at = wave_base(lds);
+#pragma unroll
+    for (int s = 0; s < kChunks; ++s) {
+      if (kOffsets == 1) load_lds16(base + s * kChunkRows * ld, o[0], at + s * NT * 16);
+      else load_lds16(base, o[s], at + s * NT * 16);
+    }
+  }
+
+  // LDS address of this wave's first instruction in the buffer `lds`.
+  static __device__ __forceinline__ uint32_t wave_base(const char* lds) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds +
+                                          (threadIdx.x >> 6) * 1024);
+  }
+
+  // The same where k or the indices end inside the tile: part chunks go through
+  // registers, ks past the end are zero.  Rolled, with its own addresses: few steps take
+  // it, and the main loop keeps its registers.
+  static __device__ __forceinline__ void direct_edge(const T* base, int64_t ld, int nx, int64_t nk, char* lds) {
+    const uint32_t at = wave_base(lds);
+    const int tid = hidden_thread();
+#pragma unroll 1
+    for (int s = 0; s < kChunks; ++s) {
+      int x, k;
+      source(s, tid, x, k);
+      const int64_t valid = KC ? nk - k : k < nk ? nx - x : 0;
+      const bool whole = valid >= kVec || (!KC && k < nk && valid <= 0 && nx >= kVec);
+      if (KC) x = min(x, nx - 1);
+      else if (x >= nx) x = 0;  // past the end: any valid index
+      const T* p = base + (KC ? x * ld + k : k * ld + x);
+      if (whole) load_lds16_at(p, at + s * NT * 16);
+      else *(vec*)(lds + (tid + s * NT) * 16) = load_vec(p, valid);
+    }
+  }
+
+  // Column sums of an XC tile: thread t adds up the 4-byte column group t % kCols4 of
+  // every kSumRows-th k row (v: one float per element of the group).
+  static constexpr int kCols4 = X * (int)sizeof(T) / 4, kSumGroups = NT / kCols4;
+  static __device__ __forceinline__ void add_rows(const char* lds, float (&v)[4 / sizeof(T)]) {
+    typedef T group __attribute__((ext_vector_type(4 / sizeof(T))));
+    const int tid = hidden_thread(), c = tid % kCols4, i = c * (4 / (int)sizeof(T));
+#pragma unroll 4
+    for (int k = tid / kCols4; k < kK; k += kSumGroups) {
+      const group q =
+          *(const group*)(lds + k * X * (int)sizeof(T) + (((i >> 4) ^ swz(k)) * 16 + (i & 15)) * (int)sizeof(T));
+#pragma unroll
+      for (int e = 0; e < 4 / (int)sizeof(T); ++e) v[e] += (float)q[e];
+    }
+  }
+
+  // Byte offset of this lane's part of the fragment at indices x0.., first half step (64
+  // bytes of k).  Fragment f further on (f 16 indices; f and x0 / 16 share no bits) and
+  // the second half are at at(base, f, 1).
+  static __device__ __forceinline__ uint32_t lane_base(int x0) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    if (KC) return (x0 + r) * ROW + ((g ^ turn(x0 + r)) << 4);
+    // transposing read: 16 lanes read 4 k rows of 16 indices, lane i gets index i's 4 ks
+    if (sizeof(T) == 2) {
+      const int k = g * 8 + (r >> 2);
+      return k * X * 2 + (((x0 >> 4) ^ swz(k)) << 5) + (r & 3) * 8;
+    }
+    return g * 4 * X * 4 + (((x0 >> 4) ^ swz(g * 4)) << 6) + r * 4;
+  }
+
+  static __device__ __forceinline__ vec frag(const char* lds, uint32_t base, int f, int ks) {
+    if (KC) return *(const vec*)(lds + (base ^ (ks << 6)) + f * 16 * ROW);
     if constexpr (sizeof(T) == 2) {
-      // the transposing read: 16 lanes read 4 k rows of 16 indices, lane i gets index i's 4 ks
+      const char* p = lds + (base ^ (f << 5)) + ks * 32 * X * 2;
       s16x8 v;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = ks * 32 + g * 8 + h * 4 + ((lane & 15) >> 2);
-        const char* p = lds + k * X * 2 + (((x0 >> 4) ^ swz(k)) << 5) + (lane & 3) * 8;
-        const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        const s16x4 t =
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + h * 4 * X * 2));
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[h * 4 + e] = t[e];
       }
       return __builtin_bit_cast(vec, v);
     } else {
+      const char* p = lds + (base ^ (f << 6)) + ks * 16 * X * 4;
       vec v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = ks * 16 + g * 4 + e;
-        v[e] = *(const T*)(lds + k * X * 4 + (((x0 >> 4) ^ swz(k)) << 6) + (lane & 15) * 4);
-      }
+      for (int e = 0; e < 4; ++e) v[e] = *(const T*)(p + e * X * 4);
       return v;
     }
   }
@@ -164,200 +309,393 @@ struct Args {
   int32_t accumulate;
   int32_t act;
   int32_t tiles_i, tiles_j;
+  int32_t splits;      // parts of the contraction, joined through `part`
+  float* part;         // [tile][split][BM BN + BM]
 };
 
-// 128-byte k-steps, staged through registers into two LDS buffers: the next step's
-// global loads are in flight while this one's matrix instructions run.
-template <typename T, int KIND, int BM, int BN>
-__global__ __launch_bounds__(kThreads) void k_linear(const Args p) {
-  constexpr bool kA_KC = KIND != kWeight, kB_KC = KIND == kForward;
-  typedef Stage<T, BM, kA_KC> SA;
-  typedef Stage<T, BN, kB_KC> SB;
-  constexpr int kK = SA::kK;
-  constexpr int MF = BM / 32, NF = BN / 32;  // 2 x 2 waves, 16 x 16 fragments
-  __shared__ __attribute__((aligned(16))) char lds[2][SA::kBytes + SB::kBytes];
+// Workgroups go round the 8 XCDs; tiles are dealt to them kRun at a time, so that what
+// an XCD's blocks read at once (8 row tiles by kRun / 8 column tiles) lies in its own
+// L2, and clients of uneven size still spread over all XCDs.
+__device__ __forceinline__ int xcd_order(int b, int total) {
+  constexpr int kRun = 32;
+  const int turn = b / (8 * kRun) * (8 * kRun);
+  if (turn + 8 * kRun > total) return b;  // the last, partial turn
+  const int r = b - turn;
+  return turn + (r & 7) * kRun + (r >> 3);
+}
 
-  const int ti = blockIdx.x / p.tiles_j, tj = blockIdx.x % p.tiles_j;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wi = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
-  const int64_t j0 = (int64_t)tj * BN;
-  const int nj = (int)min((int64_t)BN, p.nj - j0);
+__device__ __forceinline__ void tile_of(int b, int tiles_i, int tiles_j, int& ti, int& tj) {
+  constexpr int kGroup = 8;
+  const int per = kGroup * tiles_j, g = b / per, first = g * kGroup;
+  const int rows = min(kGroup, tiles_i - first), r = b - g * per;
+  ti = first + r % rows;
+  tj = r / rows;
+}
 
-  int client, ni;
-  int64_t i0, nk;
-  const T *a, *b;
-  if (KIND == kWeight) {
-    client = blockIdx.y;
-    const RowTile t = p.tiles[client];
-    i0 = (int64_t)ti * BM;
-    ni = (int)min((int64_t)BM, p.ni - i0);
-    nk = t.rows;
-    a = (const T*)p.a + t.begin * p.lda + i0;
-    b = (const T*)p.b + t.begin * p.ldb + j0;
-  } else {
-    const RowTile t = p.tiles[ti];
-    client = t.client;
-    i0 = t.begin;
-    ni = t.rows;
-    nk = p.nk;
-    a = (const T*)p.a + i0 * p.lda;
-    b = (const T*)p.b + client * p.b_client + (KIND == kForward ? j0 * p.ldb : j0);
+// Output elements of a row, columns [j, j + VEC), from float32 accumulators, the bias (or
+// pre-activation) and residual vectors already read.
+template <typename T, int KIND>
+__device__ __forceinline__ void finish(const Args& p, float (&v)[Elem<T>::kVec], typename VecOf<T>::type bias,
+                                       typename VecOf<T>::type pre, typename VecOf<T>::type extra, int64_t row,
+                                       int64_t j, int left) {
+  constexpr int VEC = Elem<T>::kVec;
+  typename VecOf<T>::type o;
+  if (KIND == kForward) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] += (float)bias[e];
+    if (p.z) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = (T)v[e];
+      store_vec((T*)p.z + row * p.ld_z + j, o, left);
+    }
+    if (p.act) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = act_value<T>(p.act, v[e]);
+    }
+  } else if (p.pre) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] *= act_slope<T>(p.act, (float)pre[e]);
   }
+  if (p.extra) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] += (float)extra[e];
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) o[e] = (T)v[e];
+  store_vec((T*)p.out + row * p.ld_out + j, o, left);
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_weight(const Args& p, const float (&v)[VEC], int client, int64_t i, int64_t j,
+                                             int left) {
+  float* o = (float*)p.out + client * p.out_client + i * p.ld_out + j;
+#pragma unroll
+  for (int h = 0; h < VEC / 4; ++h) {
+    VecOf<float>::type q = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+    if (p.accumulate) q += load_vec(o + 4 * h, left - 4 * h);
+    store_vec(o + 4 * h, q, left - 4 * h);
+  }
+}
+
+// Which tile of the output a workgroup makes, and of which rows and client.
+struct Place {
+  int client, ni, nj;   // rows and columns of the tile
+  int64_t i0, j0;       // forward, input: activation row; weight: out feature
+  int64_t nk;           // contraction
+  int32_t row0;         // weight: the client's first row
+  bool first_column;
+};
+
+template <int KIND, int BM, int BN>
+__device__ __forceinline__ Place place_of(const Args& p, int b) {
+  Place o;
+  int ti, tj, client = 0;
+  if (KIND == kWeight) {
+    const int per = p.tiles_i * p.tiles_j;
+    client = b / per;
+    b -= client * per;
+  }
+  tile_of(b, p.tiles_i, p.tiles_j, ti, tj);
+  const RowTile rt = p.tiles[KIND == kWeight ? client : ti];
+  o.j0 = (int64_t)tj * BN;
+  o.nj = (int)min((int64_t)BN, p.nj - o.j0);
+  o.first_column = tj == 0;
+  o.row0 = rt.begin;
+  if (KIND == kWeight) {
+    o.client = client;
+    o.i0 = (int64_t)ti * BM;
+    o.ni = (int)min((int64_t)BM, p.ni - o.i0);
+    o.nk = rt.rows;
+  } else {
+    o.client = rt.client;
+    o.i0 = rt.begin;
+    o.ni = rt.rows;
+    o.nk = p.nk;
+  }
+  return o;
+}
+
+// 128-byte k-steps staged to two LDS buffers: straight from memory where every address
+// is a multiple of 4 bytes, else (REG: 16-bit rows of odd length) through registers.
+// During a half step's products the next half's fragments are read, so a buffer is free
+// half a step before its products are done: there, at the step's one barrier, the next
+// buffer has landed and the load of the step after it starts.
+template <typename T, int KIND, int BM, int BN, int WM, int WN, bool REG>
+__global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Args p) {
+  constexpr bool kA_KC = KIND != kWeight, kB_KC = KIND == kForward;
+  constexpr int NT = WM * WN * 64;
+  typedef Stage<T, BM, kA_KC, NT> SA;
+  typedef Stage<T, BN, kB_KC, NT> SB;
+  constexpr int kK = SA::kK, kStage = SA::kBytes + SB::kBytes, VEC = SA::kVec;
+  constexpr int MF = BM / WM / 16, NF = BN / WN / 16;  // fragments per wave
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wi = wave / WN * (BM / WM), wj = wave % WN * (BN / WN);
+  const int tile = xcd_order(blockIdx.x, gridDim.x);
+  const Place at = place_of<KIND, BM, BN>(p, tile);
+  const int ni = at.ni, nj = at.nj, client = at.client;
+  const int64_t i0 = at.i0, j0 = at.j0;
   const int64_t step_a = kA_KC ? kK : kK * p.lda, step_b = kB_KC ? kK : kK * p.ldb;
+  const T* pa = (const T*)p.a + (KIND == kWeight ? at.row0 * p.lda + i0 : i0 * p.lda);
+  const T* pb = (const T*)p.b + (KIND == kWeight ? at.row0 * p.ldb + j0
+                                                 : client * p.b_client + (KIND == kForward ? j0 * p.ldb : j0));
+  int64_t nk = at.nk;
+  if (p.splits > 1) {
+    const int64_t per = ((nk + kK - 1) / kK + p.splits - 1) / p.splits, first = blockIdx.y * per;
+    nk = max((int64_t)0, min(nk - first * kK, per * kK));
+    pa += first * step_a;
+    pb += first * step_b;
+  }
+  const bool edge_a = !kA_KC && ni < BM && ni % VEC, edge_b = !kB_KC && nj < BN && nj % VEC;
+  uint32_t oa[SA::kOffsets], ob[SB::kOffsets];
+  if (!REG) {
+    SA::offsets(oa, p.lda, ni);
+    SB::offsets(ob, p.ldb, nj);
+  }
+  const int steps = (int)((nk + kK - 1) / kK);
+  const int full = edge_a || edge_b ? 0 : (int)(nk / kK);  // steps whose loads are all direct
+  typename SA::vec ra[REG ? SA::kChunks : 1];
+  typename SB::vec rb[REG ? SB::kChunks : 1];
+
+  auto load = [&](int t) {
+    char* d = lds + (t & 1) * kStage;
+    const T *a = pa + t * step_a, *b = pb + t * step_b;
+    const int64_t left = nk - (int64_t)t * kK;
+    if constexpr (REG) {
+      if (t < steps) {
+        SA::load(ra, a, p.lda, ni, left);
+        SB::load(rb, b, p.ldb, nj, left);
+      }
+    } else if (t < full) {
+      SA::direct(oa, a, p.lda, d);
+      SB::direct(ob, b, p.ldb, d + SA::kBytes);
+    } else if (t < steps) {
+      SA::direct_edge(a, p.lda, ni, left, d);
+      SB::direct_edge(b, p.ldb, nj, left, d + SA::kBytes);
+    }
+  };
+  auto put = [&](int t) {
+    if constexpr (REG) {
+      if (t < steps) {
+        SA::put(ra, lds + (t & 1) * kStage);
+        SB::put(rb, lds + (t & 1) * kStage + SA::kBytes);
+      }
+    }
+  };
+  // every wave is here, its fragments read and its loads landed
+  auto arrive = []() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
   f32x4 acc[MF][NF] = {};
-  f32x4 colsum[MF] = {};
-  const bool want_db = KIND == kWeight && p.db && tj == 0 && (wave & 1) == 0;
-  typename SA::vec ones;
-#pragma unroll
-  for (int e = 0; e < SA::kVec; ++e) ones[e] = (T)1.0f;
+  float colsum[4 / sizeof(T)] = {};  // of dz (the first column tile's blocks)
+  const bool want_db = KIND == kWeight && p.db && at.first_column;
+  typename SA::vec fa[2][MF];
+  typename SB::vec fb[2][NF];
+  uint32_t base_a = SA::lane_base(wi), base_b = SB::lane_base(wj);
 
-  typename SA::vec ra[SA::kChunks];
-  typename SB::vec rb[SB::kChunks];
-  const int steps = (int)((nk + kK - 1) / kK);
-  if (steps > 0) {
-    SA::load(ra, a, p.lda, ni, nk);
-    SB::load(rb, b, p.ldb, nj, nk);
-    SA::put(ra, lds[0]);
-    SB::put(rb, lds[0] + SA::kBytes);
-  }
-  __syncthreads();
-  for (int t = 0; t < steps; ++t) {
-    const bool more = t + 1 < steps;
-    if (more) {
-      const int64_t left = nk - (int64_t)(t + 1) * kK;
-      SA::load(ra, a + (t + 1) * step_a, p.lda, ni, left);
-      SB::load(rb, b + (t + 1) * step_b, p.ldb, nj, left);
-    }
-    const char* la = lds[t & 1];
-    const char* lb = la + SA::kBytes;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      typename SA::vec fa[MF];
-      typename SB::vec fb[NF];
-#pragma unroll
-      for (int m = 0; m < MF; ++m) fa[m] = SA::frag(la, wi + m * 16, ks);
-#pragma unroll
-      for (int n = 0; n < NF; ++n) fb[n] = SB::frag(lb, wj + n * 16, ks);
-#pragma unroll
-      for (int m = 0; m < MF; ++m)
-#pragma unroll
-        for (int n = 0; n < NF; ++n) acc[m][n] = mma<T>(fb[n], fa[m], acc[m][n]);
-      if (want_db) {  // column sums as a product with ones: float32, in row order
-#pragma unroll
-        for (int m = 0; m < MF; ++m) colsum[m] = mma<T>(ones, fa[m], colsum[m]);
-      }
-    }
-    if (more) {
-      char* w = lds[(t + 1) & 1];
-      SA::put(ra, w);
-      SB::put(rb, w + SA::kBytes);
-    }
-    __syncthreads();
-  }
-
-  // lane: output row wi + 16 m + lane % 16, columns wj + 16 n + 4 (lane / 16) + 0..3
-#pragma unroll
-  for (int m = 0; m < MF; ++m) {
-    const int i = wi + m * 16 + (lane & 15);
-    if (i >= ni) continue;
+  auto half = [&](auto which, const char* next) {
+    constexpr int cur = decltype(which)::value, nxt = cur ^ 1;
+    asm volatile("" : "+v"(base_a), "+v"(base_b));  // fragments' addresses are made as needed, not kept in registers
 #pragma unroll
     for (int n = 0; n < NF; ++n) {
-      const int jt = wj + n * 16 + (lane >> 4) * 4;
-      const int left = nj - jt;
-      if (left <= 0) continue;
-      const int64_t j = j0 + jt;
-      f32x4 v = acc[m][n];
-      if (KIND == kWeight) {
-        float* o = (float*)p.out + client * p.out_client + (i0 + i) * p.ld_out + j;
-        if (left >= 4) {
-          VecOf<float>::loose_quad* q = (VecOf<float>::loose_quad*)o;
-          *q = p.accumulate ? *q + v : v;
-        } else {
+      fb[nxt][n] = SB::frag(next + SA::kBytes, base_b, n, nxt);
 #pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (e < left) o[e] = p.accumulate ? o[e] + v[e] : v[e];
-        }
-        continue;
-      }
-      const int64_t row = i0 + i;
-      typedef typename VecOf<T>::quad quad;
-      typedef typename VecOf<T>::loose_quad loose_quad;
-      auto get = [&](const void* base, int64_t at) -> quad {
-        const T* s = (const T*)base + at;
-        quad q = {};
-        if (left >= 4) {
-          q = *(const loose_quad*)s;
-        } else {
+      for (int m = n * MF / NF; m < (n + 1) * MF / NF; ++m) fa[nxt][m] = SA::frag(next, base_a, m, nxt);
 #pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (e < left) q[e] = s[e];
-        }
-        return q;
-      };
-      auto set = [&](void* base, int64_t at, quad q) {
-        T* s = (T*)base + at;
-        if (left >= 4) {
-          *(loose_quad*)s = q;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (e < left) s[e] = q[e];
-        }
-      };
-      quad o;
-      if (KIND == kForward) {
-        if (p.bias) {
-          const quad q = get(p.bias, client * p.bias_client + j);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += (float)q[e];
-        }
-        if (p.z) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
-          set(p.z, row * p.ld_z + j, o);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = act_value(p.act, v[e]);
-      } else if (p.pre) {
-        const quad q = get(p.pre, row * p.ld_pre + j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= act_slope(p.act, (float)q[e]);
-      }
-      if (p.extra) {
-        const quad q = get(p.extra, row * p.ld_extra + j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += (float)q[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
-      set(p.out, row * p.ld_out + j, o);
+      for (int m = 0; m < MF; ++m) acc[m][n] = mma<T>(fb[cur][n], fa[cur][m], acc[m][n]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (want_db && lane < 16) {
-      float* o = p.db + client * p.db_client + i0 + i;
-      *o = p.accumulate ? *o + colsum[m][0] : colsum[m][0];
+  };
+  if (steps > 0) {
+    load(0);
+    put(0);
+    arrive();
+    load(1);
+    put(1);
+#pragma unroll
+    for (int m = 0; m < MF; ++m) fa[0][m] = SA::frag(lds, base_a, m, 0);
+#pragma unroll
+    for (int n = 0; n < NF; ++n) fb[0][n] = SB::frag(lds + SA::kBytes, base_b, n, 0);
+#pragma unroll 1
+    for (int t = 0; t < steps; ++t) {
+      if constexpr (KIND == kWeight)
+        if (want_db) SA::add_rows(lds + (t & 1) * kStage, colsum);
+      half(std::integral_constant<int, 0>(), lds + (t & 1) * kStage);
+      arrive();
+      load(t + 2);
+      half(std::integral_constant<int, 1>(), lds + (~t & 1) * kStage);
+      put(t + 2);
     }
   }
+
+  // The accumulators leave through LDS, each wave through its own part, so that global
+  // memory sees whole row segments of 16 bytes per lane.
+  constexpr int kRows = BM / WM, kCols = BN / WN, kRowB = kCols * 4, kPart = 2 * kStage / (WM * WN);
+  constexpr int kFit = kPart / kRowB >= kRows ? kRows : kPart / kRowB >= 64 ? 64 : kPart / kRowB >= 32 ? 32 : 16;
+  constexpr int kLanes = kCols / VEC, kPass = 64 / kLanes;  // lanes per row, rows per read
+  constexpr int kChunkMask = kCols / 4 < 16 ? kCols / 4 - 1 : 15;
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  float* part = p.part + ((int64_t)tile * p.splits + blockIdx.y) * (BM * BN + BM);
+  if constexpr (KIND == kWeight) {
+    if (want_db) {
+      constexpr int kPer = 4 / (int)sizeof(T);
+      float* sums = (float*)lds;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        sums[threadIdx.x / SA::kCols4 * BM + threadIdx.x % SA::kCols4 * kPer + e] = colsum[e];
+      __syncthreads();
+      if ((int)threadIdx.x < ni) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int g = 0; g < SA::kSumGroups; ++g) sum += sums[g * BM + threadIdx.x];
+        if (p.splits > 1) {
+          part[BM * BN + threadIdx.x] = sum;
+        } else {
+          float* o = p.db + client * p.db_client + i0 + threadIdx.x;
+          *o = p.accumulate ? *o + sum : sum;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  char* mine = lds + wave * kPart;
+  const int jt = (lane % kLanes) * VEC, left = nj - wj - jt;  // this lane's columns
+  const int64_t jg = j0 + wj + jt;
+  typename VecOf<T>::type bias = {};
+  if (KIND == kForward && p.bias) bias = load_vec((const T*)p.bias + client * p.bias_client + jg, left);
+#pragma unroll
+  for (int half = 0; half < kRows / kFit; ++half) {
+#pragma unroll
+    for (int m = 0; m < kFit / 16; ++m)
+#pragma unroll
+      for (int n = 0; n < NF; ++n) {
+        const int r = m * 16 + (lane & 15), c = n * 4 + (lane >> 4);
+        *(f32x4*)(mine + r * kRowB + ((c ^ (r & kChunkMask)) << 4)) = acc[half * (kFit / 16) + m][n];
+      }
+    __builtin_amdgcn_wave_barrier();
+    // kUnroll rows at a time, what they read from memory first
+    constexpr int kUnroll = kFit / kPass >= 4 ? 4 : kFit / kPass;
+#pragma unroll 1
+    for (int r0 = lane / kLanes; r0 < kFit; r0 += kPass * kUnroll) {
+      typename VecOf<T>::type pre[kUnroll] = {}, extra[kUnroll] = {};
+      if (KIND != kWeight && p.splits == 1) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int i = wi + half * kFit + r0 + u * kPass;
+          const int64_t row = i0 + i;
+          if (KIND == kInput && p.pre) pre[u] = load_vec((const T*)p.pre + row * p.ld_pre + jg, i < ni ? left : 0);
+          if (p.extra) extra[u] = load_vec((const T*)p.extra + row * p.ld_extra + jg, i < ni ? left : 0);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int r = r0 + u * kPass, i = wi + half * kFit + r;
+        if (i >= ni || left <= 0) continue;
+        float v[VEC];
+#pragma unroll
+        for (int h = 0; h < VEC / 4; ++h) {
+          const f32x4 q = *(const f32x4*)(mine + r * kRowB + (((jt / 4 + h) ^ (r & kChunkMask)) << 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * h + e] = q[e];
+        }
+        if (p.splits > 1) {
+          float* o = part + i * BN + wj + jt;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o[e] = v[e];
+        } else if (KIND == kWeight) {
+          store_weight<VEC>(p, v, client, i0 + i, jg, left);
+        } else {
+          finish<T, KIND>(p, v, bias, pre[u], extra[u], i0 + i, jg, left);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// A split contraction's parts, added up in their order, and the way out.
+template <typename T, int KIND, int BM, int BN>
+__global__ __launch_bounds__(256) void k_linear_join(const Args p) {
+  constexpr int VEC = Elem<T>::kVec, kLanes = BN / VEC;
+  const Place at = place_of<KIND, BM, BN>(p, blockIdx.x);
+  const float* part = p.part + (int64_t)blockIdx.x * p.splits * (BM * BN + BM);
+  constexpr int64_t kNext = BM * BN + BM;
+  const int i = (blockIdx.y * 256 + threadIdx.x) / kLanes, jt = threadIdx.x % kLanes * VEC, left = at.nj - jt;
+  if (KIND == kWeight && p.db && at.first_column && blockIdx.y == 0)
+    for (int r = threadIdx.x; r < at.ni; r += 256) {
+      float* o = p.db + at.client * p.db_client + at.i0 + r;
+      float sum = p.accumulate ? *o : 0.0f;
+      for (int s = 0; s < p.splits; ++s) sum += part[s * kNext + BM * BN + r];
+      *o = sum;
+    }
+  if (i >= at.ni || left <= 0) return;
+  float v[VEC] = {};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float* q = part + s * kNext + i * BN + jt;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] += q[e];
+  }
+  const int64_t row = at.i0 + i, j = at.j0 + jt;
+  if (KIND == kWeight) {
+    store_weight<VEC>(p, v, at.client, row, j, left);
+  } else {
+    typename VecOf<T>::type bias = {}, pre = {}, extra = {};
+    if (KIND == kForward && p.bias) bias = load_vec((const T*)p.bias + at.client * p.bias_client + j, left);
+    if (KIND == kInput && p.pre) pre = load_vec((const T*)p.pre + row * p.ld_pre + j, left);
+    if (p.extra) extra = load_vec((const T*)p.extra + row * p.ld_extra + j, left);
+    finish<T, KIND>(p, v, bias, pre, extra, row, j, left);
+  }
+}
+
+// Every address of the operand a multiple of 4 bytes: row stride, client stride, base.
+bool dword_aligned(const void* base, int64_t ld, int64_t client, size_t size) {
+  return ((uintptr_t)base | (uintptr_t)(ld * (int64_t)size) | (uintptr_t)(client * (int64_t)size)) % 4 == 0;
+}
+
+template <typename T, int KIND, int BM, int BN, int WM, int WN>
+int launch(Args p, int32_t ntiles, int64_t workspace_bytes, hipStream_t s) {
+  p.tiles_j = (int32_t)((p.nj + BN - 1) / BN);
+  p.tiles_i = KIND == kWeight ? (int32_t)((p.ni + BM - 1) / BM) : ntiles;
+  const int64_t blocks = (int64_t)p.tiles_i * p.tiles_j * (KIND == kWeight ? p.nclients : 1);
+  if (blocks > 0x7fffffffLL) return fc_internal_fail(-1, "too many tiles");
+  if (p.splits > 1 && (!p.part || workspace_bytes < blocks * p.splits * (BM * BN + BM) * (int64_t)sizeof(float)))
+    return fc_internal_fail(-1, "workspace too small");
+  const dim3 grid((unsigned)blocks, (unsigned)p.splits), block(WM * WN * 64);
+  const bool direct = dword_aligned(p.a, p.lda, 0, sizeof(T)) && dword_aligned(p.b, p.ldb, p.b_client, sizeof(T)) &&
+                      p.lda < (1 << 22) && p.ldb < (1 << 22);  // offsets inside a tile in 32 bits
+  if (direct) {
+    hipLaunchKernelGGL((k_linear<T, KIND, BM, BN, WM, WN, false>), grid, block, 0, s, p);
+  } else if constexpr (BM < 256) {
+    hipLaunchKernelGGL((k_linear<T, KIND, BM, BN, WM, WN, true>), grid, block, 0, s, p);
+  } else {
+    return fc_internal_fail(-1, "256-row tiles need operands at multiples of 4 bytes");
+  }
+  if (const int rc = fc_internal_check_launch("k_linear")) return rc;
+  if (p.splits == 1) return 0;
+  hipLaunchKernelGGL((k_linear_join<T, KIND, BM, BN>), dim3((unsigned)blocks, BM * BN / Elem<T>::kVec / 256), dim3(256),
+                     0, s, p);
+  return fc_internal_check_launch("k_linear_join");
 }
 
 template <typename T, int KIND>
-int launch(Args p, int32_t ntiles, hipStream_t s) {
-  constexpr int BM = 128, BN = 128;
-  p.tiles_j = (int32_t)((p.nj + BN - 1) / BN);
-  p.tiles_i = KIND == kWeight ? (int32_t)((p.ni + BM - 1) / BM) : ntiles;
-  const int64_t blocks = (int64_t)p.tiles_i * p.tiles_j;
-  if (blocks > 0x7fffffffLL) return fc_internal_fail(-1, "too many tiles");
-  hipLaunchKernelGGL((k_linear<T, KIND, BM, BN>), dim3((unsigned)blocks, KIND == kWeight ? p.nclients : 1),
-                     dim3(kThreads), 0, s, p);
-  return fc_internal_check_launch("k_linear");
+int pick(const Args& p, int32_t ntiles, int tile_rows, int64_t workspace_bytes, hipStream_t s) {
+  switch (tile_rows) {
+    case 32: return launch<T, KIND, 32, 128, 1, 4>(p, ntiles, workspace_bytes, s);
+    case 128: return launch<T, KIND, 128, 128, 2, 2>(p, ntiles, workspace_bytes, s);
+    case 256:
+      if constexpr (sizeof(T) == 2) return launch<T, KIND, 256, 256, 2, 4>(p, ntiles, workspace_bytes, s);
+  }
+  return fc_internal_fail(-1, "bad tile_rows");
 }
 
 template <int KIND>
-int dispatch(int dtype, const Args& p, int32_t ntiles, hipStream_t s) {
+int dispatch(int dtype, const Args& p, int32_t ntiles, int tile_rows, int64_t workspace_bytes, hipStream_t s) {
+  if (p.splits < 1 || p.splits > 1024) return fc_internal_fail(-1, "bad splits");
   switch (dtype) {
-    case FC_FLOAT32: return launch<float, KIND>(p, ntiles, s);
-    case FC_BFLOAT16: return launch<bf16, KIND>(p, ntiles, s);
-    case FC_FLOAT16: return launch<f16, KIND>(p, ntiles, s);
+    case FC_FLOAT32: return pick<float, KIND>(p, ntiles, tile_rows, workspace_bytes, s);
+    case FC_BFLOAT16: return pick<bf16, KIND>(p, ntiles, tile_rows, workspace_bytes, s);
+    case FC_FLOAT16: return pick<f16, KIND>(p, ntiles, tile_rows, workspace_bytes, s);
   }
   return fc_internal_fail(-1, "bad dtype");
 }
@@ -366,11 +704,18 @@ int dispatch(int dtype, const Args& p, int32_t ntiles, hipStream_t s) {
 
 extern "C" {
 
-int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, int32_t ntiles, int32_t nclients,
-              int64_t in_features, int64_t out_features, const void* weight, int64_t weight_client_stride,
-              int64_t weight_stride, const void* bias, int64_t bias_client_stride, int activation,
-              const void* residual, int64_t residual_stride, void* preactivation, int64_t preactivation_stride,
-              void* y, int64_t y_stride, void* stream) {
+int64_t fc_linear_workspace_bytes(int64_t blocks, int tile_rows, int splits) {
+  if (blocks < 0 || (tile_rows != 32 && tile_rows != 128 && tile_rows != 256) || splits < 1 || splits > 1024)
+    return fc_internal_fail(-1, "bad tile_rows or splits");
+  const int64_t columns = tile_rows == 256 ? 256 : 128;
+  return splits == 1 ? 0 : blocks * splits * (tile_rows * columns + tile_rows) * (int64_t)sizeof(float);
+}
+
+int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, int32_t ntiles, int tile_rows,
+              int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
+              int64_t weight_client_stride, int64_t weight_stride, const void* bias, int64_t bias_client_stride,
+              int activation, const void* residual, int64_t residual_stride, void* preactivation,
+              int64_t preactivation_stride, void* y, int64_t y_stride, int splits, void* workspace, int64_t workspace_bytes, void* stream) {
   if (ntiles < 0 || nclients <= 0 || in_features <= 0 || out_features <= 0) return fc_internal_fail(-1, "bad sizes");
   if (activation < 0 || activation > 3) return fc_internal_fail(-1, "bad activation");
   if (ntiles == 0) return 0;
@@ -385,14 +730,16 @@ int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, 
   p.z = preactivation; p.ld_z = preactivation_stride;
   p.out = y; p.ld_out = y_stride;
   p.act = activation;
-  return dispatch<kForward>(dtype, p, ntiles, (hipStream_t)stream);
+  p.splits = splits; p.part = (float*)workspace;
+  return dispatch<kForward>(dtype, p, ntiles, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 
 int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const int32_t* tiles, int32_t ntiles,
-                             int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
+                             int tile_rows, int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
                              int64_t weight_client_stride, int64_t weight_stride, int activation,
                              const void* preactivation, int64_t preactivation_stride, const void* residual,
-                             int64_t residual_stride, void* dx, int64_t dx_stride, void* stream) {
+                             int64_t residual_stride, void* dx, int64_t dx_stride, int splits, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
   if (ntiles < 0 || nclients <= 0 || in_features <= 0 || out_features <= 0) return fc_internal_fail(-1, "bad sizes");
   if (activation < 0 || activation > 3) return fc_internal_fail(-1, "bad activation");
   if (ntiles == 0) return 0;
@@ -407,13 +754,15 @@ int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const
   p.out = dx; p.ld_out = dx_stride;
   p.act = activation;
   if (activation && !preactivation) return fc_internal_fail(-1, "an activation needs its pre-activation");
-  return dispatch<kInput>(dtype, p, ntiles, (hipStream_t)stream);
+  p.splits = splits; p.part = (float*)workspace;
+  return dispatch<kInput>(dtype, p, ntiles, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 
 int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
                               const int32_t* clients, int32_t nclients, int64_t in_features, int64_t out_features,
                               float* dweight, int64_t dweight_client_stride, int64_t dweight_stride, float* dbias,
-                              int64_t dbias_client_stride, int accumulate, void* stream) {
+                              int64_t dbias_client_stride, int accumulate, int tile_rows, int splits, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
   if (nclients <= 0 || nclients > 65535 || in_features <= 0 || out_features <= 0)
     return fc_internal_fail(-1, "bad sizes");
   if (!clients || !dweight) return fc_internal_fail(-1, "null pointer");
@@ -425,7 +774,8 @@ int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, 
   p.out = dweight; p.ld_out = dweight_stride; p.out_client = dweight_client_stride;
   p.db = dbias; p.db_client = dbias_client_stride;
   p.accumulate = accumulate;
-  return dispatch<kWeight>(dtype, p, 0, (hipStream_t)stream);
+  p.splits = splits; p.part = (float*)workspace;
+  return dispatch<kWeight>(dtype, p, 0, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

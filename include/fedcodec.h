@@ -470,27 +470,42 @@ int fc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
                            int64_t dx_stride, float* dweight, int64_t dweight_stride, float* dbias,
                            int64_t dbias_stride, int accumulate, float* partials, void* stream);
 
-/* y = act(x weight_c^T + bias_c) + residual; preactivation (nullable) takes the value
- * under the activation.  tiles of 128 rows. */
-int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, int32_t ntiles, int32_t nclients,
-              int64_t in_features, int64_t out_features, const void* weight, int64_t weight_client_stride,
-              int64_t weight_stride, const void* bias, int64_t bias_client_stride, int activation,
-              const void* residual, int64_t residual_stride, void* preactivation, int64_t preactivation_stride,
-              void* y, int64_t y_stride, void* stream);
+/* The matrix products take the output in tiles of tile_rows rows (32 or 128: by 128
+ * columns; 256: by 256 columns, 16-bit types whose operands' addresses and strides are
+ * multiples of 4 bytes), from a table made with that tile_rows; and can split the
+ * contraction into `splits` (1..1024) parts, joined in order through a device
+ * workspace of fc_linear_workspace_bytes.  Both change speed, and results by the
+ * rounding of float32 sums. */
 
-/* dx = (dz weight_c) * act'(preactivation) + residual.  tiles of 128 rows. */
+/* Workspace for `blocks` output tiles: row tiles x ceil(columns / tile columns)
+ * (the weight gradient: clients x ceil(out / tile_rows) x ceil(in / tile columns)). */
+int64_t fc_linear_workspace_bytes(int64_t blocks, int tile_rows, int splits);
+
+/* y = act(x weight_c^T + bias_c) + residual; preactivation (nullable) takes the value
+ * under the activation. */
+int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, int32_t ntiles, int tile_rows,
+              int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
+              int64_t weight_client_stride, int64_t weight_stride, const void* bias, int64_t bias_client_stride,
+              int activation, const void* residual, int64_t residual_stride, void* preactivation,
+              int64_t preactivation_stride, void* y, int64_t y_stride, int splits, void* workspace,
+              int64_t workspace_bytes, void* stream);
+
+/* dx = (dz weight_c) * act'(preactivation) + residual. */
 int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const int32_t* tiles, int32_t ntiles,
-                             int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
-                             int64_t weight_client_stride, int64_t weight_stride, int activation,
+                             int tile_rows, int32_t nclients, int64_t in_features, int64_t out_features,
+                             const void* weight, int64_t weight_client_stride, int64_t weight_stride, int activation,
                              const void* preactivation, int64_t preactivation_stride, const void* residual,
-                             int64_t residual_stride, void* dx, int64_t dx_stride, void* stream);
+                             int64_t residual_stride, void* dx, int64_t dx_stride, int splits, void* workspace,
+                             int64_t workspace_bytes, void* stream);
 
 /* dweight_c = sum of dz_r x_r^T, dbias_c (nullable) = sum of dz_r over the client's
- * rows.  clients: one int32 {client, first row, rows, 0} per client. */
+ * rows.  clients: one int32 {client, first row, rows, 0} per client; tile_rows: of the
+ * gradient's tiles. */
 int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
                               const int32_t* clients, int32_t nclients, int64_t in_features, int64_t out_features,
                               float* dweight, int64_t dweight_client_stride, int64_t dweight_stride, float* dbias,
-                              int64_t dbias_client_stride, int accumulate, void* stream);
+                              int64_t dbias_client_stride, int accumulate, int tile_rows, int splits, void* workspace,
+                              int64_t workspace_bytes, void* stream);
 
 /* The k largest logits of every row, falling, ties to the lowest index, NaN below every
  * number; lse = log sum exp(logits / temperature) of the whole row. */

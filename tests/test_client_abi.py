@@ -90,3 +90,52 @@ def test_top_logits_and_distillation_refusals():
   refused(distill(dloss=b), b"dloss")
   refused(distill(logits=NULL), b"null")
   refused(distill(dtype=4), b"dtype")
+
+
+def test_linear_refusals():
+  lib, b = _lib.load(), _buf()
+
+  def forward(dtype=1, ntiles=1, rows=128, clients=1, k=8, m=8, act=0, splits=1, ws=NULL, nbytes=0, x=b, stride=8):
+    return lib.fc_linear(x, stride, dtype, b, ntiles, rows, clients, k, m, b, 64, 8, NULL, 0, act, NULL, 0, NULL, 0, b,
+                         8, splits, ws, nbytes, None)
+
+  refused(forward(k=0), b"sizes")
+  refused(forward(clients=0), b"sizes")
+  refused(forward(ntiles=-1), b"sizes")
+  refused(forward(act=4), b"activation")
+  refused(forward(x=NULL), b"null")
+  refused(forward(dtype=9), b"dtype")
+  refused(forward(rows=64), b"tile_rows")
+  refused(forward(dtype=0, rows=256), b"tile_rows")
+  refused(forward(rows=256, stride=9), b"multiples of 4 bytes")
+  refused(forward(splits=0), b"splits")
+  refused(forward(splits=1025), b"splits")
+  refused(forward(splits=2), b"workspace")
+  refused(forward(splits=2, ws=b, nbytes=64), b"workspace")
+  assert forward(ntiles=0) == 0
+
+  def backward_input(act=0, pre=NULL, dz=b):
+    return lib.fc_linear_backward_input(dz, 8, 1, b, 1, 128, 1, 8, 8, b, 64, 8, act, pre, 8, NULL, 0, b, 8, 1, NULL, 0,
+                                        None)
+
+  refused(backward_input(act=1), b"pre-activation")
+  refused(backward_input(act=7), b"activation")
+  refused(backward_input(dz=NULL), b"null")
+
+  def weight(clients=1, m=8, dw=b, splits=1):
+    return lib.fc_linear_backward_weight(b, 8, b, 8, 1, b, clients, 8, m, dw, 64, 8, NULL, 0, 0, 128, splits, NULL, 0,
+                                         None)
+
+  refused(weight(clients=0), b"sizes")
+  refused(weight(m=0), b"sizes")
+  refused(weight(dw=NULL), b"null")
+  refused(weight(splits=3), b"workspace")
+
+
+def test_linear_workspace():
+  lib = _lib.load()
+  assert lib.fc_linear_workspace_bytes(7, 128, 1) == 0
+  assert lib.fc_linear_workspace_bytes(7, 32, 3) == 7 * 3 * (32 * 128 + 32) * 4
+  assert lib.fc_linear_workspace_bytes(2, 256, 2) == 2 * 2 * (256 * 256 + 256) * 4
+  for args in [(1, 64, 1), (1, 128, 0), (-1, 128, 1), (1, 128, 2000)]:
+    assert lib.fc_linear_workspace_bytes(*args) == -1
