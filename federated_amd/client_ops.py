@@ -32,7 +32,7 @@ from federated_amd import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
-_TILES = (16, 32, 64, 128, 256)
+_TILES = (16, 32, 128, 256)
 MAX_TOP = 1024  # FC_MAX_TOP
 
 
@@ -239,7 +239,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight, batch, residual=None, dweight
   dweight = _grad_out("dweight", dweight, batch, (dim,))
   dbias = _grad_out("dbias", dbias, batch, (dim,))
   out = _out("out", out, x, batch, dim)
-  tiles, first, ntiles = batch._tiles[64]  # pylint: disable=protected-access
+  tiles, first, ntiles = batch._tiles[32]  # pylint: disable=protected-access
   part = torch.empty(ntiles * 2 * dim, dtype=torch.float32, device=batch.device)
   _call(batch.device, "fc_layer_norm_backward", _ptr(dy), dy.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
         _ptr(mean), _ptr(rstd), _ptr(tiles), ntiles, _ptr(first), batch.num_clients, dim, _ptr(weight), _ld(weight),

@@ -23,36 +23,36 @@ template <> struct Elem<float> { static constexpr int kVec = 4; };
 template <> struct Elem<bf16> { static constexpr int kVec = 8; };
 template <> struct Elem<f16> { static constexpr int kVec = 8; };
 
-// 16 bytes of T, at T's own alignment: parameters live at any element offset of a
-// client's flat row, and global memory takes unaligned dwordx4.
-template <typename T> struct VecOf {
-  typedef T type __attribute__((ext_vector_type(Elem<T>::kVec)));
-  typedef T loose __attribute__((ext_vector_type(Elem<T>::kVec), aligned(sizeof(T))));
-  typedef T quad __attribute__((ext_vector_type(4)));
-  typedef T loose_quad __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+// N elements of T (16 bytes unless said otherwise), and the same at T's own alignment:
+// parameters live at any element offset of a client's flat row, and global memory takes
+// unaligned dwordx4 (at multiples of 4 bytes for nothing, at odd 16-bit elements at about
+// two thirds of the rate, measured).
+template <typename T, int N = Elem<T>::kVec> struct VecOf {
+  typedef T type __attribute__((ext_vector_type(N)));
+  typedef T loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 
-// `valid` (<= kVec, may be <= 0) elements from p, zeros behind them.
-template <typename T>
-__device__ __forceinline__ typename VecOf<T>::type load_vec(const T* p, int64_t valid) {
-  typename VecOf<T>::type v = {};
-  if (valid >= Elem<T>::kVec) {
-    v = *(const typename VecOf<T>::loose*)p;
+// `valid` (<= N, may be <= 0) elements from p, zeros behind them.
+template <typename T, int N = Elem<T>::kVec>
+__device__ __forceinline__ typename VecOf<T, N>::type load_vec(const T* p, int64_t valid) {
+  typename VecOf<T, N>::type v = {};
+  if (valid >= N) {
+    v = *(const typename VecOf<T, N>::loose*)p;
   } else {
 #pragma unroll
-    for (int e = 0; e < Elem<T>::kVec; ++e)
+    for (int e = 0; e < N; ++e)
       if (e < valid) v[e] = p[e];
   }
   return v;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_vec(T* p, typename VecOf<T>::type v, int64_t valid) {
-  if (valid >= Elem<T>::kVec) {
-    *(typename VecOf<T>::loose*)p = v;
+template <typename T, int N = Elem<T>::kVec>
+__device__ __forceinline__ void store_vec(T* p, typename VecOf<T, N>::type v, int64_t valid) {
+  if (valid >= N) {
+    *(typename VecOf<T, N>::loose*)p = v;
   } else {
 #pragma unroll
-    for (int e = 0; e < Elem<T>::kVec; ++e)
+    for (int e = 0; e < N; ++e)
       if (e < valid) p[e] = v[e];
   }
 }
@@ -62,16 +62,33 @@ struct RowTile {
   int32_t client, begin, rows, pad;
 };
 
+// The DPP value of v under control CTRL: lanes it does not reach hold `old`.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float old, float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v),
+                                                               CTRL, ROWS, 0xf, false));
+}
+
+// Over the 64 lanes, the result in all of them: shifts inside rows of 16 lanes, then the
+// rows' last lanes broadcast, and lane 63 read back (six adds, no LDS).
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+  v += dpp<0x111>(0.0f, v);
+  v += dpp<0x112>(0.0f, v);
+  v += dpp<0x114>(0.0f, v);
+  v += dpp<0x118>(0.0f, v);
+  v += dpp<0x142, 0xa>(0.0f, v);
+  v += dpp<0x143, 0xc>(0.0f, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+  v = fmaxf(v, dpp<0x111>(v, v));
+  v = fmaxf(v, dpp<0x112>(v, v));
+  v = fmaxf(v, dpp<0x114>(v, v));
+  v = fmaxf(v, dpp<0x118>(v, v));
+  v = fmaxf(v, dpp<0x142, 0xa>(v, v));
+  v = fmaxf(v, dpp<0x143, 0xc>(v, v));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 }  // namespace fc

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -55,31 +56,50 @@ struct NormArgs {
   float* part;  // [ntiles][2][dim]
 };
 
-// TPR threads per row, NV 16-byte vectors per thread: the row stays in registers.
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(256) void k_norm(const NormArgs p) {
-  constexpr int VEC = Elem<T>::kVec, G = 256 / TPR;
-  typedef typename VecOf<T>::type vec;
-  __shared__ float slots[2][2 * 4];
+// TPR threads per row, NV vectors of VEC elements per thread: the row stays in registers, the next
+// row's are on their way while this one is summed, and the client's weights stay too.
+template <typename T, int TPR, int NV, int VEC>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm(const NormArgs p) {
+  constexpr int G = TPR > 256 ? 1 : 256 / TPR;
+  typedef typename VecOf<T, VEC>::type vec;
+  __shared__ float slots[2][2 * 8];
   const RowTile t = p.tiles[blockIdx.x];
   const int lane = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const float inv = 1.0f / (float)p.dim;
-  const T* w = (const T*)p.weight + t.client * p.ld_w;
-  const T* b = (const T*)p.bias + t.client * p.ld_b;
+  vec gw[NV], gb[NV], next[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + lane) * VEC, left = p.dim - c;
+    gw[i] = gb[i] = vec{};
+    if (p.weight) {
+      gw[i] = load_vec<T, VEC>((const T*)p.weight + t.client * p.ld_w + c, left);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) gw[i][e] = (T)1.0f;
+    }
+    if (p.bias) gb[i] = load_vec<T, VEC>((const T*)p.bias + t.client * p.ld_b + c, left);
+    next[i] = load_vec<T, VEC>((const T*)p.x + (t.begin + min(g, t.rows - 1)) * p.ld_x + c, left);
+  }
   // every group walks the same number of rows: barriers are uniform
   for (int r = 0; r < t.rows; r += G) {
     const int64_t row = t.begin + min(r + g, t.rows - 1);
     const bool live = r + g < t.rows;
-    const T* x = (const T*)p.x + row * p.ld_x;
     vec v[NV];
     float f[1] = {0.0f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      v[i] = load_vec(x + c, (int64_t)p.dim - c);
+    for (int i = 0; i < NV; ++i) v[i] = next[i];
+    if (r + G < t.rows) {
+      const T* x = (const T*)p.x + (t.begin + min(r + G + g, t.rows - 1)) * p.ld_x;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + lane) * VEC;
+        next[i] = load_vec<T, VEC>(x + c, p.dim - c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[0] += (float)v[i][e];
-    }
     group_sum<TPR>(f, slots[0]);
     const float mu = f[0] * inv;
     f[0] = 0.0f;
@@ -102,83 +122,89 @@ __global__ __launch_bounds__(256) void k_norm(const NormArgs p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
-      const int64_t left = (int64_t)p.dim - c;
-      vec gw = {}, gb = {};
-      if (p.weight) gw = load_vec(w + c, left);
-      if (p.bias) gb = load_vec(b + c, left);
       vec o;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float y = ((float)v[i][e] - mu) * s;
-        if (p.weight) y *= (float)gw[e];
-        if (p.bias) y += (float)gb[e];
-        o[e] = (T)y;
-      }
-      store_vec((T*)p.out + row * p.ld_out + c, o, left);
+      for (int e = 0; e < VEC; ++e) o[e] = (T)(((float)v[i][e] - mu) * s * (float)gw[i][e] + (float)gb[i][e]);
+      store_vec<T, VEC>((T*)p.out + row * p.ld_out + c, o, p.dim - c);
     }
   }
 }
 
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(256) void k_norm_backward(const NormArgs p) {
-  constexpr int VEC = Elem<T>::kVec, G = 256 / TPR;
-  typedef typename VecOf<T>::type vec;
-  __shared__ float slots[2][2 * 4];
+template <typename T, int TPR, int NV, int VEC>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(const NormArgs p) {
+  constexpr int G = TPR > 256 ? 1 : 256 / TPR;
+  typedef typename VecOf<T, VEC>::type vec;
+  __shared__ float slots[2][2 * 8];
   __shared__ float join[G > 1 ? TPR * VEC * NV : 1];
   const RowTile t = p.tiles[blockIdx.x];
   const int lane = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const float inv = 1.0f / (float)p.dim;
-  const T* w = (const T*)p.weight + t.client * p.ld_w;
   float dg[NV][VEC] = {}, db[NV][VEC] = {};
+  vec gw[NV], nx[NV], nd[NV];
+  float nmu, ns;
+  // Row r of this group; a group past the tile's rows reads zeros, and adds none.
+  auto fetch = [&](int r) {
+    const int64_t row = t.begin + min(r + g, t.rows - 1);
+    const bool live = r + g < t.rows;
+    nmu = p.mean[row];
+    ns = p.rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC, left = live ? p.dim - c : 0;
+      nx[i] = load_vec<T, VEC>((const T*)p.x + row * p.ld_x + c, left);
+      nd[i] = load_vec<T, VEC>((const T*)p.dy + row * p.ld_dy + c, left);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + lane) * VEC;
+    if (p.weight) {
+      gw[i] = load_vec<T, VEC>((const T*)p.weight + t.client * p.ld_w + c, p.dim - c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) gw[i][e] = (T)(c + e < p.dim ? 1.0f : 0.0f);
+    }
+  }
+  fetch(0);
   int turn = 0;
   for (int r = 0; r < t.rows; r += G, turn ^= 1) {
     const int64_t row = t.begin + min(r + g, t.rows - 1);
     const bool live = r + g < t.rows;
-    const float mu = p.mean[row], s = p.rstd[row];
-    const T* x = (const T*)p.x + row * p.ld_x;
-    const T* dy = (const T*)p.dy + row * p.ld_dy;
+    const float mu = live ? nmu : 0.0f, s = live ? ns : 0.0f;
     vec vx[NV], vd[NV];
-    float f[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      const int64_t left = live ? (int64_t)p.dim - c : 0;
-      vx[i] = load_vec(x + c, left);
-      vd[i] = load_vec(dy + c, left);
-      vec gw = {};
-      if (p.weight) gw = load_vec(w + c, left);
+      vx[i] = nx[i];
+      vd[i] = nd[i];
+    }
+    if (r + G < t.rows) fetch(r + G);
+    float f[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        // columns past the end (and rows past the tile) have dy = 0: they add nothing
-        const float d = (float)vd[i][e], xh = ((float)vx[i][e] - mu) * s;
-        const float a = p.weight ? d * (float)gw[e] : d;
-        const bool in = e < left;
-        f[0] += in ? a : 0.0f;
-        f[1] += in ? a * xh : 0.0f;
-        dg[i][e] += in ? d * xh : 0.0f;
-        db[i][e] += in ? d : 0.0f;
+        // columns past the end have dy = weight = 0: 0 times a finite xh
+        const float d = (float)vd[i][e], xh = ((float)vx[i][e] - mu) * s, a = d * (float)gw[i][e];
+        f[0] += a;
+        f[1] += (i * TPR + lane) * VEC + e < p.dim ? a * xh : 0.0f;
+        dg[i][e] += d * xh;
+        db[i][e] += d;
       }
-    }
     group_sum<TPR>(f, slots[turn]);
     const float m0 = f[0] * inv, m1 = f[1] * inv;
     if (!live) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
-      const int64_t left = (int64_t)p.dim - c;
-      vec gw = {}, res = {};
-      if (p.weight) gw = load_vec(w + c, left);
-      if (p.residual) res = load_vec((const T*)p.residual + row * p.ld_res + c, left);
+      vec res = {};
+      if (p.residual) res = load_vec<T, VEC>((const T*)p.residual + row * p.ld_res + c, p.dim - c);
       vec o;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = (float)vd[i][e], xh = ((float)vx[i][e] - mu) * s;
-        const float a = p.weight ? d * (float)gw[e] : d;
-        float v = s * (a - m0 - xh * m1);
-        if (p.residual) v += (float)res[e];
-        o[e] = (T)v;
+        const float xh = ((float)vx[i][e] - mu) * s, a = (float)vd[i][e] * (float)gw[i][e];
+        o[e] = (T)(s * (a - m0 - xh * m1) + (float)res[e]);
       }
-      store_vec((T*)p.out + row * p.ld_out + c, o, left);
+      store_vec<T, VEC>((T*)p.out + row * p.ld_out + c, o, p.dim - c);
     }
   }
   if (!p.part) return;
@@ -290,40 +316,122 @@ __global__ __launch_bounds__(256) void k_norm_backward_long(const NormArgs p) {
   }
 }
 
-// dg_c, db_c: the client's tiles' partial rows, summed in tile order.
+// dg_c, db_c: the client's tiles' partial rows.  A block adds up 64 columns, its four waves
+// every fourth tile each, joined in wave order.
 __global__ __launch_bounds__(256) void k_norm_join(const float* part, const int32_t* first_tile, int32_t dim,
                                                    float* dw, int64_t ld_dw, float* db, int64_t ld_db,
                                                    int accumulate) {
-  const int c = blockIdx.y * 256 + threadIdx.x, client = blockIdx.x, which = blockIdx.z;
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.y * 64 + lane, client = blockIdx.x, which = blockIdx.z;
   float* o = which ? db : dw;
-  if (c >= dim || !o) return;
-  o += client * (which ? ld_db : ld_dw) + c;
-  const int lo = first_tile[client], hi = first_tile[client + 1];
-  float s = accumulate ? *o : 0.0f;
-  float t[8];
-  int k = lo;
-  for (; k + 8 <= hi; k += 8) {
+  if (!o) return;
+  const int hi = first_tile[client + 1];
+  float s = 0.0f;
+  if (c < dim) {
+    int k = first_tile[client] + wave;
+    for (; k + 28 < hi; k += 32) {
+      float t[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) t[u] = part[((int64_t)(k + u) * 2 + which) * dim + c];
+      for (int u = 0; u < 8; ++u) t[u] = part[((int64_t)(k + 4 * u) * 2 + which) * dim + c];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) s += t[u];
+      for (int u = 0; u < 8; ++u) s += t[u];
+    }
+    for (; k < hi; k += 4) s += part[((int64_t)k * 2 + which) * dim + c];
   }
-  for (; k < hi; ++k) s += part[((int64_t)k * 2 + which) * dim + c];
-  *o = s;
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < dim) {
+    o += client * (which ? ld_db : ld_dw) + c;
+    s = accumulate ? *o : 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) s += sums[w][lane];
+    *o = s;
+  }
 }
 
 // ---------------------------------------------------------------------------
 // Top logits: the k largest of a row (ties to the lowest index, NaN below every
 // number), and log sum exp(l / tau).
 //
-// The k-th largest of the threads' own maxima is a lower bound of the k-th largest
-// logit, so only the few threads whose maximum reaches it look at their elements
-// again; what they hold at or above it is ranked by counting.  When too many
-// elements tie there, the bound is made exact by a radix select first.
+// One read of the row: each thread keeps its elements' maximum, running maximum and sum.
+// The k-th largest of the threads' maxima is a lower bound of the k-th largest logit, so
+// only the elements of the few threads whose maximum reaches it are looked at again, and
+// what is at or above it is ranked by counting.  When too many elements tie there, the
+// bound is made exact by a radix select first.
 // ---------------------------------------------------------------------------
 
-constexpr int kTopThreads = 1024;
-constexpr int kTopCap = 2048;  // candidates ranked in LDS
+// A row of n elements as N-element vectors at multiples of their size: it starts `head`
+// elements into its first vector, so a row at an odd address (an odd row length) is still
+// read in aligned vectors.  Offsets c count from that vector's start, `end` = head + n;
+// elements outside the row come as -inf and are not stored.
+template <typename T, int N>
+struct Row {
+  typedef typename VecOf<T, N>::type vec;
+  const T* base;  // not to be read before head
+  uint32_t head, end;
+
+  __device__ __forceinline__ Row(const T* row, uint32_t n) {
+    head = (uint32_t)((uintptr_t)row / sizeof(T)) % N;
+    base = row - head;
+    end = head + n;
+  }
+
+  __device__ __forceinline__ bool whole(uint32_t c) const { return c >= head && c + N <= end; }
+
+  __device__ __forceinline__ vec load(uint32_t c) const {
+    if (whole(c)) return *(const vec*)(base + c);
+    vec v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = c + e >= head && c + e < end ? base[c + e] : (T)-INFINITY;
+    return v;
+  }
+
+  // to another row of the same length, element 0 at `to`
+  __device__ __forceinline__ void store(T* to, uint32_t c, vec v) const {
+    T* p = to + (int64_t)c - head;
+    if (whole(c)) {
+      *(typename VecOf<T, N>::loose*)p = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (c + e >= head && c + e < end) p[e] = v[e];
+    }
+  }
+};
+
+// A running maximum m of f and sum of exp2(f scale - r), r = m scale (0 while nothing but
+// -inf and NaN came by).  r is rounded once and then exact: each term is one multiply-add
+// and one exp2.  A NaN makes the sum NaN, and so does +inf.
+struct Softmax {
+  float m = -INFINITY, r = 0.0f, sum = 0.0f;
+
+  __device__ __forceinline__ void raise(float to, float scale) {
+    if (to > m) {
+      const float next = to * scale;
+      sum *= m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(r - next);
+      m = to;
+      r = next;
+    }
+  }
+
+  template <int N>
+  __device__ __forceinline__ void add(const float (&f)[N], float scale) {
+    float high = f[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) high = fmaxf(high, f[e]);
+    raise(high, scale);
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], scale, -r));
+  }
+
+  // log sum exp(f / tau), scale = log2(e) / tau
+  __device__ __forceinline__ float lse(float inv_tau, float scale) const {
+    if (m == -INFINITY) return sum == 0.0f ? -INFINITY : sum;
+    return m * inv_tau + (__builtin_fmaf(-m, scale, r) * kLn2 + logf(sum));
+  }
+};
+
 
 // Orders as the float does; -0 = +0; NaN lowest.
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -332,95 +440,119 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kTopThreads) void k_top_logits(const T* logits, int64_t ld, int32_t vocab, int32_t k,
-                                                            float scale, int32_t* index, T* values, float* lse) {
-  constexpr int VEC = Elem<T>::kVec;
-  typedef typename VecOf<T>::type vec;
-  __shared__ uint32_t maxima[kTopThreads];
+__device__ __forceinline__ unsigned long long candidate(uint32_t key, int64_t c) {
+  return (unsigned long long)key << 32 | (uint32_t)~(uint32_t)c;
+}
+
+template <typename T, int NT, int VEC>
+__global__ __launch_bounds__(NT) void k_top_logits(const T* logits, int64_t ld, int32_t vocab, int32_t k, float inv_tau,
+                                                   int32_t* index, T* values, float* lse) {
+  constexpr int W = NT / 64, kProbes = 16 / W;
+  constexpr int kTopCap = NT == 64 ? 512 : 2048;  // candidates ranked in LDS
+  typedef typename VecOf<T, VEC>::type vec;
+  __shared__ uint32_t maxima[NT], active[NT];
   __shared__ unsigned long long cand[kTopCap];
   __shared__ uint32_t hist[256];
-  __shared__ float red[2][kTopThreads / 64];
-  __shared__ uint32_t bound, ncand, want, ties;
+  __shared__ float red[2][W];
+  __shared__ uint32_t count[2][16];
+  __shared__ uint32_t bound, ncand, nactive, want, ties;
   const int64_t row = blockIdx.x;
   const T* x = logits + row * ld;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float scale = kLog2e * inv_tau;
 
-  uint32_t best = 0;
-  bool nan = false;
-  float mx = -INFINITY, sum = 0.0f;  // running maximum and sum of exp2((l - mx) scale)
-  for (int64_t c = (int64_t)tid * VEC; c < vocab; c += (int64_t)kTopThreads * VEC) {
-    const vec v = load_vec(x + c, vocab - c);
-    float m = -INFINITY;
+  const Row<T, VEC> at_row(x, vocab);
+  Softmax sm;
+  auto add = [&](const vec& v) {
+    float f[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float f = c + e < vocab ? (float)v[e] : -INFINITY;
-      nan |= f != f;
-      m = fmaxf(m, f);
-      if (c + e < vocab) best = max(best, order_key(f));
-    }
-    if (m > mx) {
-      sum *= exp2f((mx - m) * scale);
-      mx = m;
-    }
-    if (mx > -INFINITY)
+    for (int e = 0; e < VEC; ++e) f[e] = (float)v[e];
+    sm.add(f, scale);
+  };
+  constexpr uint32_t kStride = NT * VEC;
+  uint32_t c0 = tid * VEC;
+  for (; c0 + 3 * kStride < at_row.end; c0 += 4 * kStride) {
+    vec v[4];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum += c + e < vocab ? exp2f(((float)v[e] - mx) * scale) : 0.0f;
+    for (int u = 0; u < 4; ++u) v[u] = at_row.load(c0 + u * kStride);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add(v[u]);
   }
+  for (; c0 < at_row.end; c0 += kStride) add(at_row.load(c0));
+
+  // 16-bit types: the key's low half follows from its high half
+  constexpr int kBits = 8 * (int)sizeof(T);
+  const uint32_t best = sm.m == -INFINITY ? 0 : order_key(sm.m);  // nothing but -inf and NaN bounds nothing
   maxima[tid] = best;
-  const float wm = wave_max(mx);
+  const float wm = wave_max(sm.m);
   if (lane == 0) red[0][wave] = wm;
-  if (tid == 0) ncand = ties = 0;
-  const bool any_nan = __syncthreads_or(nan);
+  if (tid == 0) ncand = nactive = ties = 0;
+  __syncthreads();
   float bm = red[0][0];
 #pragma unroll
-  for (int w = 1; w < kTopThreads / 64; ++w) bm = fmaxf(bm, red[0][w]);
-  const float ws = wave_sum(mx > -INFINITY ? sum * exp2f((mx - bm) * scale) : 0.0f);
+  for (int w = 1; w < W; ++w) bm = fmaxf(bm, red[0][w]);
+  sm.raise(bm, scale);
+  const float ws = wave_sum(sm.sum);
   if (lane == 0) red[1][wave] = ws;
-  if (wave == 0) {
-    // the k-th largest of the maxima, bit by bit (0 when fewer threads than k hold any)
-    uint32_t m[kTopThreads / 64];
+
+  // the k-th largest of the maxima, four bits a round: the waves count 16 probes
+  // (0 when fewer threads than k hold any)
+  uint32_t t0 = 0;
+  {
+    uint32_t m[W];
 #pragma unroll
-    for (int i = 0; i < kTopThreads / 64; ++i) m[i] = maxima[i * 64 + lane];
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t probe = t | (1u << bit);
-      int n = 0;
+    for (int i = 0; i < W; ++i) m[i] = maxima[i * 64 + lane];
+#pragma unroll 1
+    for (int shift = 28, turn = 0; shift >= 32 - kBits; shift -= 4, turn ^= 1) {
 #pragma unroll
-      for (int i = 0; i < kTopThreads / 64; ++i) n += __popcll(__ballot(m[i] >= probe));
-      if (n >= k) t = probe;
-    }
-    if (lane == 0) bound = t;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    float s = 0.0f;
+      for (int q = 0; q < kProbes; ++q) {
+        const uint32_t probe = t0 | (uint32_t)(wave * kProbes + q) << shift;
+        int n = 0;
 #pragma unroll
-    for (int w = 0; w < kTopThreads / 64; ++w) s += red[1][w];
-    lse[row] = any_nan ? NAN : fabsf(bm) == INFINITY ? bm : bm * scale * kLn2 + logf(s);
-  }
-  const uint32_t t0 = bound;
-  if (best >= t0)
-    for (int64_t c = (int64_t)tid * VEC; c < vocab; c += (int64_t)kTopThreads * VEC) {
-      const vec v = load_vec(x + c, vocab - c);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (c + e >= vocab) break;
-        const uint32_t key = order_key((float)v[e]);
-        if (key < t0) continue;
-        const uint32_t at = atomicAdd(&ncand, 1u);
-        if (at < kTopCap) cand[at] = (unsigned long long)key << 32 | (uint32_t)~(uint32_t)(c + e);
+        for (int i = 0; i < W; ++i) n += __popcll(__ballot(m[i] >= probe));
+        if (lane == 0) count[turn][wave * kProbes + q] = n;
       }
+      __syncthreads();
+      const unsigned long long ok = __ballot(lane < 16 && (lane == 0 || (int)count[turn][lane & 15] >= k));
+      t0 |= (uint32_t)(63 - __clzll((long long)ok)) << shift;
     }
+  }
+  if (bm == INFINITY) {  // the sum is NaN; the row's is +inf unless it holds a NaN
+    bool nan = false;
+    for (int64_t c = tid; c < vocab; c += NT) nan |= (float)x[c] != (float)x[c];
+    nan = __syncthreads_or(nan);
+    if (tid == 0) lse[row] = nan ? NAN : INFINITY;
+  } else if (tid == 0) {
+    sm.sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sm.sum += red[1][w];
+    lse[row] = sm.lse(inv_tau, scale);
+  }
+  const int chunks = (int)((at_row.end + kStride - 1) / kStride);  // per thread
+  if (best >= t0) active[atomicAdd(&nactive, 1u)] = tid;
+  __syncthreads();
+  const int total = (int)nactive * chunks;
+  for (int q = tid; q < total; q += NT) {
+    const uint32_t c = active[q / chunks] * VEC + q % chunks * kStride;
+    if (c >= at_row.end) continue;
+    const vec v = at_row.load(c);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const uint32_t key = order_key((float)v[e]);
+      if (key < t0 || c + e < at_row.head || c + e >= at_row.end) continue;
+      const uint32_t at = atomicAdd(&ncand, 1u);
+      if (at < kTopCap) cand[at] = candidate(key, c + e - at_row.head);
+    }
+  }
   __syncthreads();
   uint32_t n = ncand;
   if (n > kTopCap) {
     // exact k-th key by four 8-bit digits, then everything above it and the first ties
     uint32_t prefix = 0, need = k;
     for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+      for (int i = tid; i < 256; i += NT) hist[i] = 0;
       __syncthreads();
-      for (int64_t c = tid; c < vocab; c += kTopThreads) {
+      for (int64_t c = tid; c < vocab; c += NT) {
         const uint32_t key = order_key((float)x[c]);
         if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1u);
       }
@@ -440,32 +572,37 @@ __global__ __launch_bounds__(kTopThreads) void k_top_logits(const T* logits, int
     if (tid == 0) ncand = 0;
     __syncthreads();
     // ties are taken in index order: `need` of them
-    for (int64_t c0 = 0; c0 < vocab; c0 += kTopThreads) {
-      const int64_t c = c0 + tid;
+    for (int64_t c1 = 0; c1 < vocab; c1 += NT) {
+      const int64_t c = c1 + tid;
       const uint32_t key = c < vocab ? order_key((float)x[c]) : 0;
       const bool tie = c < vocab && key == prefix;
-      if (c < vocab && key > prefix) cand[atomicAdd(&ncand, 1u)] = (unsigned long long)key << 32 | (uint32_t)~(uint32_t)c;
+      if (c < vocab && key > prefix) cand[atomicAdd(&ncand, 1u)] = candidate(key, c);
       const unsigned long long b = __ballot(tie);
       if (lane == 0) hist[wave] = __popcll(b);
       __syncthreads();
       uint32_t before = ties + __popcll(b & ((1ull << lane) - 1)), all = 0;
 #pragma unroll
-      for (int w = 0; w < kTopThreads / 64; ++w) {
+      for (int w = 0; w < W; ++w) {
         if (w < wave) before += hist[w];
         all += hist[w];
       }
-      if (tie && before < need) cand[atomicAdd(&ncand, 1u)] = (unsigned long long)key << 32 | (uint32_t)~(uint32_t)c;
+      if (tie && before < need) cand[atomicAdd(&ncand, 1u)] = candidate(key, c);
       __syncthreads();
       if (tid == 0) ties += all;
       __syncthreads();
     }
     n = ncand;
   }
-  for (uint32_t i = tid; i < n; i += kTopThreads) {
-    const unsigned long long mine = cand[i];
+  // a candidate's rank: how many are greater, counted by 8 lanes
+  for (uint32_t i0 = 0; i0 < n; i0 += NT / 8) {
+    const uint32_t i = i0 + tid / 8;
+    const unsigned long long mine = i < n ? cand[i] : 0;
     int rank = 0;
-    for (uint32_t j = 0; j < n; ++j) rank += cand[j] > mine;
-    if (rank < k) {
+    for (uint32_t j = tid & 7; j < n; j += 8) rank += cand[j] > mine;
+    rank += __shfl_xor(rank, 1);
+    rank += __shfl_xor(rank, 2);
+    rank += __shfl_xor(rank, 4);
+    if (i < n && rank < k && (tid & 7) == 0) {
       const uint32_t at = ~(uint32_t)mine;
       index[row * k + rank] = (int32_t)at;
       values[row * k + rank] = x[at];
@@ -480,7 +617,6 @@ __global__ __launch_bounds__(kTopThreads) void k_top_logits(const T* logits, int
 //   ds_j = w_r tau (m q_j - sum_{k: i_k = j} p_k)
 // ---------------------------------------------------------------------------
 
-constexpr int kDistillThreads = 256;
 constexpr int kDistillMax = 1024;  // teacher entries per row
 
 struct DistillArgs {
@@ -501,10 +637,11 @@ struct DistillArgs {
   int64_t ld_grad;
 };
 
+// Over the block's NT threads, through `red` (NT / 64 floats of this call's own: one barrier).
 template <int NT>
 __device__ __forceinline__ float block_sum(float v, float* red) {
   v = wave_sum(v);
-  __syncthreads();
+  if (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0.0f;
@@ -516,7 +653,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 template <int NT>
 __device__ __forceinline__ float block_max(float v, float* red) {
   v = wave_max(v);
-  __syncthreads();
+  if (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = red[0];
@@ -526,21 +663,39 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 }
 
 // LOSS: row loss and lse; GRAD: the gradient (with LOSS unset from the saved lse).
-template <typename T, bool LOSS, bool GRAD>
-__global__ __launch_bounds__(kDistillThreads) void k_distill(const DistillArgs a) {
-  constexpr int VEC = Elem<T>::kVec, NT = kDistillThreads;
+// NV > 0: the row stays in registers, NV 16-byte vectors per thread, so that loss and
+// gradient read it once; NV = 0 streams it, once per use.
+template <typename T, int NT, int NV, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
+  constexpr int VEC = Elem<T>::kVec;
+  constexpr uint32_t kStride = NT * VEC;  // offsets in a row stay below 2^31: a uniform base and 32 bits
   typedef typename VecOf<T>::type vec;
-  __shared__ int32_t at[kDistillMax];
-  __shared__ float prob[kDistillMax], own[kDistillMax];
-  __shared__ float red[NT / 64];
+  extern __shared__ int32_t entries[];  // 4 k words
+  int32_t *at = entries, *lead = entries + a.k;
+  float *prob = (float*)(entries + 2 * a.k), *own = (float*)(entries + 3 * a.k);
+  __shared__ float red[6][NT / 64];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
-  const int client = a.row_client[row];
-  const float weight = a.row_weights ? a.row_weights[row]
-                                     : 1.0f / (float)(a.offsets[client + 1] - a.offsets[client]);
   const T* s = (const T*)a.logits + row * a.ld;
   T* grad = (T*)a.grad + row * a.ld_grad;
   const float inv_tau = 1.0f / a.tau, scale = kLog2e * inv_tau;
+  const uint32_t first = tid * VEC;
+  const Row<T, VEC> at_row(s, a.vocab);
+  typedef uint32_t raw __attribute__((ext_vector_type(4)));
+  raw held[NV > 0 ? NV : 1];  // packed: unpacked to float32 the row would not fit
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    held[i] = __builtin_bit_cast(raw, at_row.load(first + i * kStride));
+  }
+  // vector by vector, and each use unpacks it anew
+  auto held_at = [&](int i) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "+v"(held[i]));
+    return __builtin_bit_cast(vec, held[i]);
+  };
+  const int client = a.row_client[row];
+  const float weight = a.row_weights ? a.row_weights[row]
+                                     : 1.0f / (float)(a.offsets[client + 1] - a.offsets[client]);
 
   // the teacher's row
   float high = -INFINITY;
@@ -550,17 +705,18 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(const DistillArgs a
     if ((uint32_t)j >= (uint32_t)a.vocab || t == -INFINITY) j = -1;
     at[i] = j;
     prob[i] = t;
+    lead[i] = i;
     if (j >= 0) high = t != t ? t : fmaxf(high, t);
   }
   const bool any = __syncthreads_or(high != -INFINITY);
-  if (!any || weight == 0.0f) {  // nothing to learn from: no loss, no gradient, logits not looked at
+  if (!any || weight == 0.0f) {  // nothing to learn from: no loss, no gradient, whatever the logits
     if (LOSS && tid == 0) {
       a.row_loss[row] = 0.0f;
       if (a.lse) a.lse[row] = 0.0f;
     }
     if (GRAD) {
       const vec zero = {};
-      for (int64_t c = (int64_t)tid * VEC; c < a.vocab; c += NT * VEC) store_vec(grad + c, zero, a.vocab - c);
+      for (uint32_t c = first; c < at_row.end; c += kStride) at_row.store(grad, c, zero);
     }
     return;
   }
@@ -568,40 +724,78 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(const DistillArgs a
   if (a.teacher_lse) {
     L = a.teacher_lse[row];
   } else {
-    high = block_max<NT>(high, red);
+    high = block_max<NT>(high, red[0]);
     float z = 0.0f;
     for (int i = tid; i < a.k; i += NT)
       if (at[i] >= 0) z += expf(prob[i] - high);
-    L = high + logf(block_sum<NT>(z, red));
+    L = high + logf(block_sum<NT>(z, red[1]));
+  }
+  if (GRAD) {  // the first of the entries that share an index
+    // waves take the earlier entries in turn, lanes the later ones
+    for (int i = tid & 63; i < a.k; i += 64) {
+      const int32_t mine = at[i];
+      int best = i;
+#pragma unroll 4
+      for (int h = tid >> 6; h < a.k; h += NT / 64) best = at[h] == mine ? min(best, h) : best;
+      if (best < i) atomicMin(&lead[i], best);
+    }
   }
 
-  // the student's softmax
-  float mx, lse;
+  // the student's softmax: q_j = exp2(s_j scale - r) / sum, or exp(s_j / tau - lse)
+  Softmax sm;
+  float lse;
   if (LOSS) {
-    float m = -INFINITY, z = 0.0f;
-    for (int64_t c = (int64_t)tid * VEC; c < a.vocab; c += NT * VEC) {
-      const vec v = load_vec(s + c, a.vocab - c);
-      float vm = -INFINITY;
+    auto unpack = [](const vec& v, float (&f)[VEC]) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) vm = fmaxf(vm, c + e < a.vocab ? (float)v[e] : -INFINITY);
-      if (vm > m) {
-        z *= exp2f((m - vm) * scale);
-        m = vm;
-      }
+      for (int e = 0; e < VEC; ++e) f[e] = (float)v[e];
+    };
+    float f[VEC];
+    if constexpr (NV > 0) {
+      float high = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float f = (float)v[e];
-        if (c + e < a.vocab && f != -INFINITY) z += exp2f((f - m) * scale);
+      for (int i = 0; i < NV; ++i) {
+        unpack(held_at(i), f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) high = fmaxf(high, f[e]);
       }
+      sm.raise(block_max<NT>(high, red[2]), scale);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        unpack(held_at(i), f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sm.sum += __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], scale, -sm.r));
+      }
+    } else {
+      uint32_t c = first;
+      for (; c + 3 * kStride < at_row.end; c += 4 * kStride) {
+        vec v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = at_row.load(c + u * kStride);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          unpack(v[u], f);
+          sm.add(f, scale);
+        }
+      }
+      for (; c < at_row.end; c += kStride) {
+        unpack(at_row.load(c), f);
+        sm.add(f, scale);
+      }
+      sm.raise(block_max<NT>(sm.m, red[2]), scale);
     }
-    mx = block_max<NT>(m, red);
-    z = block_sum<NT>(m > -INFINITY ? z * exp2f((m - mx) * scale) : z, red);
-    lse = mx == -INFINITY && z == 0.0f ? -INFINITY : mx * inv_tau + logf(z);
+    sm.sum = block_sum<NT>(sm.sum, red[3]);
+    lse = sm.lse(inv_tau, scale);
     if (tid == 0 && a.lse) a.lse[row] = lse;
-    if (!GRAD) mx = 0.0f;
   } else {
     lse = a.lse[row];
   }
+  const bool none = lse == -INFINITY;  // no student distribution: q = 0
+  const float unit = none ? 0.0f : LOSS ? 1.0f / sm.sum : 1.0f;
+  // q before the division by the sum
+  const float shift = none ? 0.0f : lse;
+  auto part = [&](float f) {
+    return __builtin_amdgcn_exp2f(LOSS ? __builtin_fmaf(f, scale, -sm.r) : (f * inv_tau - shift) * kLog2e);
+  };
 
   // teacher entries: probability, student logit, loss
   float loss = 0.0f, mass = 0.0f;
@@ -620,36 +814,44 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(const DistillArgs a
     mass += pr;
   }
   if (LOSS) {
-    loss = block_sum<NT>(loss, red);
+    loss = block_sum<NT>(loss, red[4]);
     if (tid == 0) a.row_loss[row] = weight * a.tau * a.tau * loss;
   }
   if (!GRAD) return;
-  mass = block_sum<NT>(mass, red);
+  mass = block_sum<NT>(mass, red[5]);
   float w = weight * a.tau;
   if (a.dloss) w *= a.dloss[client];
-  const float wm = w * mass;
-  const bool none = lse == -INFINITY;  // no student distribution: q = 0
-  const float shift = lse;
-  for (int64_t c = (int64_t)tid * VEC; c < a.vocab; c += NT * VEC) {
-    const vec v = load_vec(s + c, a.vocab - c);
+  const float wm = w * mass * unit;
+  auto emit = [&](const vec& v, uint32_t c) {
     vec o;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = (T)(none ? 0.0f : wm * expf((float)v[e] * inv_tau - shift));
-    store_vec(grad + c, o, a.vocab - c);
+    for (int e = 0; e < VEC; ++e) o[e] = (T)(none ? 0.0f : wm * part((float)v[e]));
+    at_row.store(grad, c, o);
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) emit(held_at(i), first + i * kStride);
+  } else {
+    // backwards: what the sum read last is in the caches still
+    int i = (int)((at_row.end + kStride - 1) / kStride) - 1;
+    for (; i >= 3; i -= 4) {
+      vec v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = at_row.load(first + (i - u) * kStride);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) emit(v[u], first + (i - u) * kStride);
+    }
+    for (; i >= 0; --i) emit(at_row.load(first + i * kStride), first + i * kStride);
   }
-  __syncthreads();
+  __syncthreads();  // the gradient's columns are written, `lead` is settled
   // the teacher's columns: the first entry of an index takes all of its entries, in order
   for (int i = tid; i < a.k; i += NT) {
     const int32_t j = at[i];
-    if (j < 0) continue;
-    bool first = true;
-    for (int h = 0; h < i; ++h) first &= at[h] != j;
-    if (!first) continue;
+    if (j < 0 || lead[i] != i) continue;
     float pr = prob[i];
     for (int h = i + 1; h < a.k; ++h)
-      if (at[h] == j) pr += prob[h];
-    const float q = none ? 0.0f : mass * expf(own[i] * inv_tau - shift);
-    grad[j] = (T)(w * (q - pr));
+      if (lead[h] == i) pr += prob[h];
+    grad[j] = (T)(none ? -w * pr : wm * part(own[i]) - w * pr);
   }
 }
 
@@ -667,21 +869,25 @@ __global__ __launch_bounds__(256) void k_distill_join(const float* row_loss, con
 // Host side.
 // ---------------------------------------------------------------------------
 
-template <typename T, int TPR, int NV>
+template <typename T, int TPR, int NV, int VEC = Elem<T>::kVec>
 void norm_launch(const NormArgs& p, bool backward, hipStream_t s) {
-  if (backward) hipLaunchKernelGGL((k_norm_backward<T, TPR, NV>), dim3(p.ntiles), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((k_norm<T, TPR, NV>), dim3(p.ntiles), dim3(256), 0, s, p);
+  const dim3 grid(p.ntiles), block(TPR > 256 ? TPR : 256);
+  if (backward) hipLaunchKernelGGL((k_norm_backward<T, TPR, NV, VEC>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((k_norm<T, TPR, NV, VEC>), grid, block, 0, s, p);
 }
 
 template <typename T>
 int norm_dispatch(const NormArgs& p, bool backward, hipStream_t s) {
   const int64_t vecs = (p.dim + Elem<T>::kVec - 1) / Elem<T>::kVec;
+  // the smallest shape that holds a row; a wave's 64 to 96 vectors as 8-byte ones (670
+  // bfloat16 elements: an eighth of the lanes idle instead of a third)
   if (vecs <= 64) norm_launch<T, 64, 1>(p, backward, s);
+  else if (sizeof(T) == 2 && vecs <= 96) norm_launch<T, 64, 3, 4>(p, backward, s);
   else if (vecs <= 128) norm_launch<T, 64, 2>(p, backward, s);
   else if (vecs <= 256) norm_launch<T, 256, 1>(p, backward, s);
   else if (vecs <= 512) norm_launch<T, 256, 2>(p, backward, s);
   else if (vecs <= 1024) norm_launch<T, 256, 4>(p, backward, s);
-  else if (vecs <= 2048) norm_launch<T, 256, 8>(p, backward, s);
+  else if (vecs <= 2048) norm_launch<T, 512, 4>(p, backward, s);
   else if (backward) hipLaunchKernelGGL((k_norm_backward_long<T>), dim3(p.ntiles), dim3(256), 0, s, p);
   else hipLaunchKernelGGL((k_norm_long<T>), dim3(p.ntiles), dim3(256), 0, s, p);
   return fc_internal_check_launch("k_norm");
@@ -696,12 +902,45 @@ int norm_dtype(int dtype, const NormArgs& p, bool backward, hipStream_t s) {
   return fc_internal_fail(-1, "bad dtype");
 }
 
+template <typename T, int NT, int NV>
+void distill_go(const DistillArgs& a, int64_t rows, bool loss, hipStream_t s) {
+  const dim3 grid((unsigned)rows), block(NT);
+  const size_t lds = 16 * (size_t)a.k;
+  if constexpr (NV > 0) {
+    hipLaunchKernelGGL((k_distill<T, NT, NV, true, true>), grid, block, lds, s, a);
+  } else {
+    if (loss && a.grad) hipLaunchKernelGGL((k_distill<T, NT, 0, true, true>), grid, block, lds, s, a);
+    else if (loss) hipLaunchKernelGGL((k_distill<T, NT, 0, true, false>), grid, block, lds, s, a);
+    else hipLaunchKernelGGL((k_distill<T, NT, 0, false, true>), grid, block, lds, s, a);
+  }
+}
+
 template <typename T>
 int distill_launch(const DistillArgs& a, int64_t rows, bool loss, hipStream_t s) {
-  const dim3 grid((unsigned)rows), block(kDistillThreads);
-  if (loss && a.grad) hipLaunchKernelGGL((k_distill<T, true, true>), grid, block, 0, s, a);
-  else if (loss) hipLaunchKernelGGL((k_distill<T, true, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((k_distill<T, false, true>), grid, block, 0, s, a);
+  const int64_t vecs = (a.vocab + Elem<T>::kVec - 1) / Elem<T>::kVec;
+  // One wave for a short row (100,000 rows of 3000 bfloat16: 375 us, 256 threads 498);
+  // loss and gradient together hold the row while it leaves registers for two blocks a
+  // CU, else stream it: what 512 blocks read comes back from the last-level cache (8197
+  // rows of 131072 bfloat16: 1019 us, held 1113).
+  if (!loss || !a.grad) {
+    if (vecs <= 512) distill_go<T, 64, 0>(a, rows, loss, s);
+    else if (vecs <= 4096) distill_go<T, 256, 0>(a, rows, loss, s);
+    else distill_go<T, 1024, 0>(a, rows, loss, s);
+  } else if (vecs < 64 * 4) {
+    distill_go<T, 64, 4>(a, rows, loss, s);
+  } else if (vecs < 64 * 8) {
+    distill_go<T, 64, 8>(a, rows, loss, s);
+  } else if (vecs < 256 * 5) {
+    distill_go<T, 256, 5>(a, rows, loss, s);
+  } else if (vecs < 256 * 10) {
+    distill_go<T, 256, 10>(a, rows, loss, s);
+  } else if (vecs < 1024 * 4) {
+    distill_go<T, 1024, 4>(a, rows, loss, s);
+  } else if (vecs < 1024 * 8 && sizeof(T) == 4) {  // 9375 rows of 32000: 477 us, streamed 572
+    distill_go<T, 1024, 8>(a, rows, loss, s);
+  } else {
+    distill_go<T, 1024, 0>(a, rows, loss, s);
+  }
   return fc_internal_check_launch("k_distill");
 }
 
@@ -712,6 +951,25 @@ int distill_dtype(int dtype, const DistillArgs& a, int64_t rows, bool loss, hipS
     case FC_FLOAT16: return distill_launch<f16>(a, rows, loss, s);
   }
   return fc_internal_fail(-1, "bad dtype");
+}
+
+template <typename T>
+int top_launch(const void* logits, int64_t stride, int64_t rows, int64_t vocab, int32_t k, float inv_tau, int32_t* index,
+               void* values, float* lse, hipStream_t s) {
+  // The bound is close while there are several times as many threads with elements as k,
+  // and a block is no larger than its row keeps busy.  100,000 rows of 10004 (bfloat16, k 16):
+  // 256 threads 297 us a 60,000, 1024 threads 903; 9155 rows of 65536: 251 against 204.
+  auto go = [&](auto threads, auto vec) {
+    constexpr int NT = decltype(threads)::value, VEC = decltype(vec)::value;
+    hipLaunchKernelGGL((k_top_logits<T, NT, VEC>), dim3((unsigned)rows), dim3(NT), 0, s, (const T*)logits, stride,
+                       (int32_t)vocab, k, inv_tau, index, (T*)values, lse);
+  };
+  typedef std::integral_constant<int, Elem<T>::kVec> wide;
+  if (vocab <= 4096 && k <= 32) go(std::integral_constant<int, 64>(), wide());
+  else if (vocab <= 2048) go(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+  else if (vocab <= 32768 && k <= 128) go(std::integral_constant<int, 256>(), wide());
+  else go(std::integral_constant<int, 1024>(), wide());
+  return fc_internal_check_launch("k_top_logits");
 }
 
 constexpr int64_t kMaxDim = 1 << 24;
@@ -782,7 +1040,7 @@ int fc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
     if (const int rc = norm_dtype(dtype, p, true, s)) return rc;
   }
   if (!want) return 0;
-  hipLaunchKernelGGL(k_norm_join, dim3((unsigned)nclients, (unsigned)((dim + 255) / 256), 2), dim3(256), 0, s,
+  hipLaunchKernelGGL(k_norm_join, dim3((unsigned)nclients, (unsigned)((dim + 63) / 64), 2), dim3(256), 0, s,
                      (const float*)partials, first_tile, (int32_t)dim, dweight, dweight_stride, dbias, dbias_stride,
                      accumulate);
   return fc_internal_check_launch("k_norm_join");
@@ -795,25 +1053,14 @@ int fc_top_logits(const void* logits, int64_t stride, int dtype, int64_t rows, i
   if (!(temperature > 0.0f) || std::isinf(temperature)) return fc_internal_fail(-1, "bad temperature");
   if (rows == 0) return 0;
   if (!logits || !index || !values || !lse) return fc_internal_fail(-1, "null pointer");
-  const float scale = kLog2e / temperature;
-  const dim3 grid((unsigned)rows), block(kTopThreads);
+  const float inv_tau = 1.0f / temperature;
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
-    case FC_FLOAT32:
-      hipLaunchKernelGGL((k_top_logits<float>), grid, block, 0, s, (const float*)logits, stride, (int32_t)vocab, k,
-                         scale, index, (float*)values, lse);
-      break;
-    case FC_BFLOAT16:
-      hipLaunchKernelGGL((k_top_logits<bf16>), grid, block, 0, s, (const bf16*)logits, stride, (int32_t)vocab, k,
-                         scale, index, (bf16*)values, lse);
-      break;
-    case FC_FLOAT16:
-      hipLaunchKernelGGL((k_top_logits<f16>), grid, block, 0, s, (const f16*)logits, stride, (int32_t)vocab, k, scale,
-                         index, (f16*)values, lse);
-      break;
-    default: return fc_internal_fail(-1, "bad dtype");
+    case FC_FLOAT32: return top_launch<float>(logits, stride, rows, vocab, k, inv_tau, index, values, lse, s);
+    case FC_BFLOAT16: return top_launch<bf16>(logits, stride, rows, vocab, k, inv_tau, index, values, lse, s);
+    case FC_FLOAT16: return top_launch<f16>(logits, stride, rows, vocab, k, inv_tau, index, values, lse, s);
   }
-  return fc_internal_check_launch("k_top_logits");
+  return fc_internal_fail(-1, "bad dtype");
 }
 
 int fc_distill(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t vocab, const int32_t* index,
