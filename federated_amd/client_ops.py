@@ -83,6 +83,7 @@ class ClientBatch:
     self.offsets, self.row_client, self._clients = views[:3]
     self._tiles = {rows: (views[3 + 2 * i], views[4 + 2 * i], parts[3 + 2 * i].shape[0])
                    for i, rows in enumerate(_TILES)}
+    self.tile_counts = tuple(self._tiles[rows][2] for rows in _TILE_COSTS)
 
   def _tile_table(self, rows):
     lib = _lib.load()
@@ -186,12 +187,19 @@ def _ld(t):
 
 
 def _call(device, name, *args):
-  stream = torch.cuda.current_stream(device).cuda_stream
-  if device.index == torch.cuda.current_device():
-    _lib.call(name, *args, stream)
+  """A C entry point on the current stream of `device`."""
+  index = device.index
+  # the raw handle: torch.cuda.current_stream(device) makes a Stream object, at 2 us a
+  # sixth of a small call
+  stream = torch._C._cuda_getCurrentRawStream(index)  # pylint: disable=protected-access
+  fn = getattr(_lib.load(), name)
+  if index == torch.cuda.current_device():
+    rc = fn(*args, stream)
   else:
     with torch.cuda.device(device):
-      _lib.call(name, *args, stream)
+      rc = fn(*args, stream)
+  if rc:
+    _lib.check(rc)
 
 
 # --- layer norm ------------------------------------------------------------------
@@ -314,14 +322,18 @@ def _workspace(blocks, rows, splits, device):
   return torch.empty(need, dtype=torch.uint8, device=device)
 
 
-def _dword_aligned(*tensors):
-  return all((t.data_ptr() | t.stride(0) * t.element_size() | t.stride(-2) * t.element_size()) % 4 == 0 for t in tensors)
+def _dword_aligned(size, a, b):
+  """Whether every row of both operands starts at a multiple of 4 bytes."""
+  return size == 4 or not (a.data_ptr() & 3 or b.data_ptr() & 3 or (a.stride(0) | b.stride(0) | b.stride(-2)) & 1)
 
 
 def _row_plan(batch, columns, contraction, a, weight):
-  tiles = tuple(batch._tiles[h][2] * -(-columns // max(128, h)) for h in _TILE_COSTS)  # pylint: disable=protected-access
-  steps = -(-contraction * a.element_size() // 128)
-  return _plan(tiles, steps, steps, a.element_size(), _dword_aligned(a, weight))
+  """_plan for an output of the activations' rows by `columns`."""
+  n32, n128, n256 = batch.tile_counts
+  narrow, wide = -(-columns // 128), -(-columns // 256)
+  size = a.element_size()
+  steps = -(-contraction * size // 128)
+  return _plan((n32 * narrow, n128 * narrow, n256 * wide), steps, steps, size, _dword_aligned(size, a, weight))
 
 
 def linear(x, weight, bias, batch, activation=None, residual=None, preactivation=False, out=None):
@@ -399,7 +411,7 @@ def linear_backward_weight(dz, x, batch, dweight=None, dbias=None, bias=True, ac
   tiles = tuple(batch.num_clients * -(-m // h) * -(-k // max(128, h)) for h in _TILE_COSTS)
   per = 128 // size
   rows, splits = _plan(tiles, -(-batch.num_rows // (per * batch.num_clients)), -(-batch.longest // per), size,
-                       _dword_aligned(dz, x))
+                       _dword_aligned(size, dz, x))
   ws = _workspace(batch.num_clients * -(-m // rows) * -(-k // max(128, rows)), rows, splits, batch.device)
   _call(batch.device, "fc_linear_backward_weight", _ptr(dz), dz.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
         _ptr(batch._clients), batch.num_clients, k, m, _ptr(dweight), dweight.stride(0), dweight.stride(1),  # pylint: disable=protected-access
