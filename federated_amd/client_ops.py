@@ -287,8 +287,8 @@ _CUS = 256
 
 
 @functools.lru_cache(maxsize=4096)
-def _plan(tiles, steps, longest, size, aligned):
-  """(tile rows, splits of the contraction) of a product, by the lowest estimate.
+def _estimate(tiles, steps, longest, size, aligned):
+  """(us, tile rows, splits of the contraction) of a product, by the lowest estimate.
 
   ``tiles``: output tiles for each of _TILE_COSTS' heights; ``steps`` / ``longest``: the
   mean and the largest number of k-steps of a tile.  Splitting pays where there are
@@ -304,15 +304,74 @@ def _plan(tiles, steps, longest, size, aligned):
     splits = 1
     while splits <= 16 and (splits == 1 or 2 * splits <= longest):
       blocks = max(1, count * splits)
-      per_cu = -(-blocks // _CUS) if blocks < 4 * _CUS else blocks / _CUS
-      rounds = max(1.0, blocks / (_CUS * resident))
-      t = max(per_cu * step * steps, rounds * _STEP_LATENCY * longest) / splits + rounds * ends
+      rounds, rest = divmod(blocks, _CUS * resident)
+      each = max(_STEP_LATENCY * longest, resident * step * steps) / splits + ends
+      if rounds >= 4:  # workgroups no longer start and end together
+        t = blocks / (_CUS * resident) * each
+      else:
+        t = rounds * each
+        if rest:
+          t += max(_STEP_LATENCY * longest, -(-rest // _CUS) * step * steps) / splits + ends
       if splits > 1:  # the parts' write and read, and the joining launch
         t += 4.0 + 2 * blocks * rows * max(128, rows) * 4 / 4e6
       if best is None or t < best[0]:
         best = (t, rows, splits)
       splits *= 2
-  return best[1:]
+  return best
+
+
+def _plan(tiles, steps, longest, size, aligned):
+  return _estimate(tiles, steps, longest, size, aligned)[1:]
+
+
+def _odd(t):
+  """Whether some row of a 16-bit operand starts at an odd element (of a 4-byte word)."""
+  return t.data_ptr() & 3 or (t.stride(0) | t.stride(-2)) & 1
+
+
+def _packed(t, rows):
+  """``t``'s rows ([rows, width], or [clients, out, in]) at a stride of whole vectors."""
+  width = t.shape[-1]
+  stride = (width + 7) // 8 * 8
+  if t.dim() == 2:
+    clients, per, client_stride = 1, rows, 0
+    out = torch.empty((rows, stride), dtype=t.dtype, device=t.device)
+  else:
+    clients, per, client_stride = (1 if t.stride(0) == 0 else t.shape[0]), t.shape[1], t.stride(0)
+    out = torch.empty((clients, per, stride), dtype=t.dtype, device=t.device)
+  _call(t.device, "fc_pack_rows", _ptr(t), client_stride, t.stride(-2), _DTYPES[t.dtype], clients, per, width, _ptr(out),
+        stride)
+  return out.expand(t.shape[0], per, stride) if t.dim() == 3 else out
+
+
+def _operands(a, b, rows, tiles, steps, longest):
+  """A product's operands as it reads them: (a, b, padded, tile rows, splits).
+
+  Rows of a 16-bit operand at odd elements go through registers, at about 2.2 times a
+  step's cost (two thirds of the load rate, and the wait is in the step); copied to
+  whole vectors first they do not.  Copying pays where a row is read by many tiles: 33
+  clients, 9001 rows in all, 1021 to 2050 (float16): 120 + 196 + 183 us as they are,
+  against 100 + 90 + 156 with the copies.
+  """
+  size = a.element_size()
+  odd = (_odd(a), _odd(b)) if size == 2 else (0, 0)
+  padded = 0
+  if (odd[0] or odd[1]) and rows:
+    copies = sum(4.0 + n * 4 / 4e6 for o, n in zip(odd, (rows * a.shape[1], _elements(b, rows))) if o)
+    if _estimate(tiles, steps, longest, 2, True)[0] + copies < 2.2 * _estimate(tiles, steps, longest, 2, False)[0]:
+      if odd[0]:
+        a, padded = _packed(a, rows), 1
+      if odd[1]:
+        b, padded = _packed(b, rows), padded | 2
+      odd = (0, 0)
+  height, splits = _plan(tiles, steps, longest, size, not (odd[0] or odd[1]))
+  return a, b, padded, height, splits
+
+
+def _elements(b, rows):
+  if b.dim() == 2:
+    return rows * b.shape[1]
+  return (1 if b.stride(0) == 0 else b.shape[0]) * b.shape[1] * b.shape[2]
 
 
 def _workspace(blocks, rows, splits, device):
@@ -322,18 +381,16 @@ def _workspace(blocks, rows, splits, device):
   return torch.empty(need, dtype=torch.uint8, device=device)
 
 
-def _dword_aligned(size, a, b):
-  """Whether every row of both operands starts at a multiple of 4 bytes."""
-  return size == 4 or not (a.data_ptr() & 3 or b.data_ptr() & 3 or (a.stride(0) | b.stride(0) | b.stride(-2)) & 1)
-
-
-def _row_plan(batch, columns, contraction, a, weight):
-  """_plan for an output of the activations' rows by `columns`."""
+def _row_product(batch, columns, a, weight):
+  """_operands for an output of the activations' rows by `columns`; and the row tiles."""
   n32, n128, n256 = batch.tile_counts
   narrow, wide = -(-columns // 128), -(-columns // 256)
-  size = a.element_size()
-  steps = -(-contraction * size // 128)
-  return _plan((n32 * narrow, n128 * narrow, n256 * wide), steps, steps, size, _dword_aligned(size, a, weight))
+  steps = -(-a.shape[1] * a.element_size() // 128)
+  a, weight, padded, rows, splits = _operands(a, weight, batch.num_rows, (n32 * narrow, n128 * narrow, n256 * wide),
+                                              steps, steps)
+  tiles, _, ntiles = batch._tiles[rows]  # pylint: disable=protected-access
+  ws = _workspace(ntiles * (wide if rows == 256 else narrow), rows, splits, batch.device)
+  return a, weight, (_ptr(tiles), ntiles, rows), (padded, splits, _ptr(ws), 0 if ws is None else ws.numel()), ws
 
 
 def linear(x, weight, bias, batch, activation=None, residual=None, preactivation=False, out=None):
@@ -353,13 +410,10 @@ def linear(x, weight, bias, batch, activation=None, residual=None, preactivation
     _activations("residual", residual, batch, m, x)
   out = _out("out", out, x, batch, m)
   z = _out("z", None, x, batch, m) if preactivation else None
-  rows, splits = _row_plan(batch, m, k, x, weight)
-  tiles, _, ntiles = batch._tiles[rows]  # pylint: disable=protected-access
-  ws = _workspace(ntiles * -(-m // max(128, rows)), rows, splits, batch.device)
-  _call(batch.device, "fc_linear", _ptr(x), x.stride(0), _DTYPES[x.dtype], _ptr(tiles), ntiles, rows,
-        batch.num_clients, k, m, _ptr(weight), weight.stride(0), weight.stride(1), _ptr(bias), _ld(bias), act,
-        _ptr(residual), _ld(residual), _ptr(z), _ld(z), _ptr(out), out.stride(0), splits, _ptr(ws),
-        0 if ws is None else ws.numel())
+  x, weight, tiles, last, _ws = _row_product(batch, m, x, weight)
+  _call(batch.device, "fc_linear", _ptr(x), x.stride(0), _DTYPES[x.dtype], *tiles, batch.num_clients, k, m,
+        _ptr(weight), weight.stride(0), weight.stride(1), _ptr(bias), _ld(bias), act, _ptr(residual), _ld(residual),
+        _ptr(z), _ld(z), _ptr(out), out.stride(0), *last)
   return (out, z) if preactivation else out
 
 
@@ -380,13 +434,10 @@ def linear_backward_input(dz, weight, batch, preactivation=None, activation=None
   if residual is not None:
     _activations("residual", residual, batch, k, dz)
   out = _out("out", out, dz, batch, k)
-  rows, splits = _row_plan(batch, k, m, dz, weight)
-  tiles, _, ntiles = batch._tiles[rows]  # pylint: disable=protected-access
-  ws = _workspace(ntiles * -(-k // max(128, rows)), rows, splits, batch.device)
-  _call(batch.device, "fc_linear_backward_input", _ptr(dz), dz.stride(0), _DTYPES[dz.dtype], _ptr(tiles), ntiles, rows,
+  dz, weight, tiles, last, _ws = _row_product(batch, k, dz, weight)
+  _call(batch.device, "fc_linear_backward_input", _ptr(dz), dz.stride(0), _DTYPES[dz.dtype], *tiles,
         batch.num_clients, k, m, _ptr(weight), weight.stride(0), weight.stride(1), act, _ptr(preactivation),
-        _ld(preactivation), _ptr(residual), _ld(residual), _ptr(out), out.stride(0), splits, _ptr(ws),
-        0 if ws is None else ws.numel())
+        _ld(preactivation), _ptr(residual), _ld(residual), _ptr(out), out.stride(0), *last)
   return out
 
 
@@ -407,15 +458,14 @@ def linear_backward_weight(dz, x, batch, dweight=None, dbias=None, bias=True, ac
   dweight = _grad_out("dweight", dweight, batch, (m, k))
   if bias:
     dbias = _grad_out("dbias", dbias, batch, (m,))
-  size = x.element_size()
   tiles = tuple(batch.num_clients * -(-m // h) * -(-k // max(128, h)) for h in _TILE_COSTS)
-  per = 128 // size
-  rows, splits = _plan(tiles, -(-batch.num_rows // (per * batch.num_clients)), -(-batch.longest // per), size,
-                       _dword_aligned(size, dz, x))
+  per = 128 // x.element_size()
+  dz, x, padded, rows, splits = _operands(dz, x, batch.num_rows, tiles,
+                                          -(-batch.num_rows // (per * batch.num_clients)), -(-batch.longest // per))
   ws = _workspace(batch.num_clients * -(-m // rows) * -(-k // max(128, rows)), rows, splits, batch.device)
   _call(batch.device, "fc_linear_backward_weight", _ptr(dz), dz.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
         _ptr(batch._clients), batch.num_clients, k, m, _ptr(dweight), dweight.stride(0), dweight.stride(1),  # pylint: disable=protected-access
-        _ptr(dbias), _ld(dbias), int(bool(accumulate)), rows, splits, _ptr(ws), 0 if ws is None else ws.numel())
+        _ptr(dbias), _ld(dbias), int(bool(accumulate)), rows, padded, splits, _ptr(ws), 0 if ws is None else ws.numel())
   return dweight, dbias
 
 

@@ -94,7 +94,7 @@ template <> __device__ __forceinline__ f32x4 mma<float>(VecOf<float>::type j, Ve
 // 16 bytes per lane from base + off straight to LDS (dword-aligned source): lane l's land
 // at lds + 16 l.  Untracked by the compiler: the caller waits for vmcnt(0).
 __device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
                : "memory");
 }
 
@@ -212,23 +212,65 @@ struct Stage {
   }
 
   // The same where k or the indices end inside the tile: part chunks go through
-  // registers, ks past the end are zero.  Rolled, with its own addresses: few steps take
-  // it, and the main loop keeps its registers.
-  static __device__ __forceinline__ void direct_edge(const T* base, int64_t ld, int nx, int64_t nk, char* lds) {
+  // registers, ks past the end are zero.  `back`: the rows begin before `base`.  Rolled,
+  // with its own addresses: few steps take it, and the main loop keeps its registers.
+  static __device__ __forceinline__ void direct_edge(const T* base, int64_t ld, int nx, int64_t nk, bool back,
+                                                     char* lds) {
     const uint32_t at = wave_base(lds);
     const int tid = hidden_thread();
-#pragma unroll 1
-    for (int s = 0; s < kChunks; ++s) {
+    // elements of chunk s that exist (0: zeros; negative: past the indices, any will do), and where it is
+    auto find = [&](int s, const T*& p, bool& room) -> int {
       int x, k;
       source(s, tid, x, k);
-      const int64_t valid = KC ? nk - k : k < nk ? nx - x : 0;
-      const bool whole = valid >= kVec || (!KC && k < nk && valid <= 0 && nx >= kVec);
+      const int valid = KC ? (int)min((int64_t)kVec, nk - k) : k < nk ? min(kVec, nx - x) : 0;
+      room = (KC ? k : x) > 0 || back;
       if (KC) x = min(x, nx - 1);
-      else if (x >= nx) x = 0;  // past the end: any valid index
-      const T* p = base + (KC ? x * ld + k : k * ld + x);
-      if (whole) load_lds16_at(p, at + s * NT * 16);
-      else *(vec*)(lds + (tid + s * NT) * 16) = load_vec(p, valid);
+      else if (x >= nx) x = 0;
+      p = base + (KC ? x * ld + k : k * ld + x);
+      if (!KC && k < nk && valid <= 0) return nx >= kVec ? kVec : 0;
+      return max(valid, 0);
+    };
+    const T* p;
+    bool room;
+#pragma unroll 1
+    for (int s = 0; s < kChunks; ++s) {
+      const int valid = find(s, p, room);
+      if (valid == kVec) load_lds16_at(p, at + s * NT * 16);
+      else if (valid == 0) *(vec*)(lds + (tid + s * NT) * 16) = vec{};
     }
+    constexpr int kAtOnce = NT == 512 && kChunks >= 2 ? 2 : kChunks;
+#pragma unroll 1
+    for (int s0 = 0; s0 < kChunks; s0 += kAtOnce) {
+      vec r[kAtOnce];
+      int valid[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        valid[u] = find(s0 + u, p, room);
+        if (valid[u] > 0 && valid[u] < kVec) r[u] = load_tail(p, valid[u], room);
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (valid[u] > 0 && valid[u] < kVec) *(vec*)(lds + (tid + (s0 + u) * NT) * 16) = r[u];
+    }
+    // vmcnt(0), here: a wait the compiler would else place behind, in every step's way
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+  }
+
+  // The last `valid` elements of a row, at p, and zeros: read as the vector that ends
+  // with them where the row has `room` for it, so that one load does.
+  static __device__ __forceinline__ vec load_tail(const T* p, int valid, bool room) {
+    if (!room) return load_vec(p, valid);
+    typedef uint64_t pair __attribute__((ext_vector_type(2)));
+    pair q = __builtin_bit_cast(pair, *(const typename VecOf<T>::loose*)(p + valid - kVec));
+    const int bits = (kVec - valid) * 8 * (int)sizeof(T);
+    if (bits >= 64) {
+      q.x = q.y >> (bits - 64);
+      q.y = 0;
+    } else {
+      q.x = q.x >> bits | q.y << (64 - bits);
+      q.y >>= bits;
+    }
+    return __builtin_bit_cast(vec, q);
   }
 
   // Column sums of an XC tile: thread t adds up the 4-byte column group t % kCols4 of
@@ -309,6 +351,7 @@ struct Args {
   int32_t accumulate;
   int32_t act;
   int32_t tiles_i, tiles_j;
+  int32_t padded;      // bit 0: a's rows, bit 1: b's can be read to a multiple of 8 elements
   int32_t splits;      // parts of the contraction, joined through `part`
   float* part;         // [tile][split][BM BN + BM]
 };
@@ -447,7 +490,8 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
     pa += first * step_a;
     pb += first * step_b;
   }
-  const bool edge_a = !kA_KC && ni < BM && ni % VEC, edge_b = !kB_KC && nj < BN && nj % VEC;
+  const bool edge_a = !kA_KC && ni < BM && ni % VEC && !(p.padded & 1);
+  const bool edge_b = !kB_KC && nj < BN && nj % VEC && !(p.padded & 2);
   uint32_t oa[SA::kOffsets], ob[SB::kOffsets];
   if (!REG) {
     SA::offsets(oa, p.lda, ni);
@@ -471,8 +515,8 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
       SA::direct(oa, a, p.lda, d);
       SB::direct(ob, b, p.ldb, d + SA::kBytes);
     } else if (t < steps) {
-      SA::direct_edge(a, p.lda, ni, left, d);
-      SB::direct_edge(b, p.ldb, nj, left, d + SA::kBytes);
+      SA::direct_edge(a, p.lda, ni, left, kA_KC ? t > 0 || blockIdx.y > 0 : i0 > 0, d);
+      SB::direct_edge(b, p.ldb, nj, left, kB_KC ? t > 0 || blockIdx.y > 0 : j0 > 0, d + SA::kBytes);
     }
   };
   auto put = [&](int t) {
@@ -506,12 +550,18 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  // this lane's columns on the way out, and their bias: there before it is needed
+  constexpr int kCols = BN / WN, kLanes = kCols / VEC;
+  const int jt = (lane % kLanes) * VEC, left = nj - wj - jt;
+  const int64_t jg = j0 + wj + jt;
+  typename VecOf<T>::type bias = {};
+  if (KIND == kForward && p.bias) bias = load_vec((const T*)p.bias + client * p.bias_client + jg, left);
   if (steps > 0) {
     load(0);
     put(0);
-    arrive();
     load(1);
     put(1);
+    arrive();
 #pragma unroll
     for (int m = 0; m < MF; ++m) fa[0][m] = SA::frag(lds, base_a, m, 0);
 #pragma unroll
@@ -530,9 +580,9 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
 
   // The accumulators leave through LDS, each wave through its own part, so that global
   // memory sees whole row segments of 16 bytes per lane.
-  constexpr int kRows = BM / WM, kCols = BN / WN, kRowB = kCols * 4, kPart = 2 * kStage / (WM * WN);
+  constexpr int kRows = BM / WM, kRowB = kCols * 4, kPart = 2 * kStage / (WM * WN);
   constexpr int kFit = kPart / kRowB >= kRows ? kRows : kPart / kRowB >= 64 ? 64 : kPart / kRowB >= 32 ? 32 : 16;
-  constexpr int kLanes = kCols / VEC, kPass = 64 / kLanes;  // lanes per row, rows per read
+  constexpr int kPass = 64 / kLanes;  // rows per read
   constexpr int kChunkMask = kCols / 4 < 16 ? kCols / 4 - 1 : 15;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   float* part = p.part + ((int64_t)tile * p.splits + blockIdx.y) * (BM * BN + BM);
@@ -559,10 +609,6 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
     }
   }
   char* mine = lds + wave * kPart;
-  const int jt = (lane % kLanes) * VEC, left = nj - wj - jt;  // this lane's columns
-  const int64_t jg = j0 + wj + jt;
-  typename VecOf<T>::type bias = {};
-  if (KIND == kForward && p.bias) bias = load_vec((const T*)p.bias + client * p.bias_client + jg, left);
 #pragma unroll
   for (int half = 0; half < kRows / kFit; ++half) {
 #pragma unroll
@@ -648,6 +694,20 @@ __global__ __launch_bounds__(256) void k_linear_join(const Args p) {
   }
 }
 
+// Rows copied to a stride of whole 16-byte vectors: [clients][rows][out_ld], zeros behind
+// `cols`.  A thread per vector.
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack_rows(const T* src, int64_t client, int64_t ld, int64_t rows, int32_t cols,
+                                                   T* dst, int32_t out_ld) {
+  constexpr int VEC = Elem<T>::kVec;
+  const int64_t per = out_ld / VEC, q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (q >= rows * per) return;
+  const int64_t r = q / per;
+  const int c = (int)(q - r * per) * VEC;
+  const T* from = src + blockIdx.y * client + r * ld + c;
+  *(typename VecOf<T>::type*)(dst + (blockIdx.y * rows + r) * out_ld + c) = load_vec(from, cols - c);
+}
+
 // Every address of the operand a multiple of 4 bytes: row stride, client stride, base.
 bool dword_aligned(const void* base, int64_t ld, int64_t client, size_t size) {
   return ((uintptr_t)base | (uintptr_t)(ld * (int64_t)size) | (uintptr_t)(client * (int64_t)size)) % 4 == 0;
@@ -711,11 +771,38 @@ int64_t fc_linear_workspace_bytes(int64_t blocks, int tile_rows, int splits) {
   return splits == 1 ? 0 : blocks * splits * (tile_rows * columns + tile_rows) * (int64_t)sizeof(float);
 }
 
+int fc_pack_rows(const void* src, int64_t client_stride, int64_t stride, int dtype, int32_t nclients, int64_t rows,
+                 int64_t cols, void* dst, int64_t dst_stride, void* stream) {
+  if (nclients <= 0 || nclients > 65535 || rows < 0 || cols <= 0 || dst_stride < cols || dst_stride > 0x7fffffff)
+    return fc_internal_fail(-1, "bad sizes");
+  if (rows == 0) return 0;
+  if (!src || !dst) return fc_internal_fail(-1, "null pointer");
+  const int64_t vec = dtype == FC_FLOAT32 ? 4 : 8;
+  if (dst_stride % vec || (uintptr_t)dst % 16) return fc_internal_fail(-1, "dst is not in whole 16-byte vectors");
+  const int64_t blocks = (rows * (dst_stride / vec) + 255) / 256;
+  if (blocks > 0x7fffffffLL) return fc_internal_fail(-1, "too many rows");
+  const dim3 grid((unsigned)blocks, (unsigned)nclients);
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case FC_FLOAT32:
+      hipLaunchKernelGGL((k_pack_rows<float>), grid, dim3(256), 0, s, (const float*)src, client_stride, stride, rows,
+                         (int32_t)cols, (float*)dst, (int32_t)dst_stride);
+      break;
+    case FC_BFLOAT16:
+    case FC_FLOAT16:  // a copy: 16 bits are 16 bits
+      hipLaunchKernelGGL((k_pack_rows<f16>), grid, dim3(256), 0, s, (const f16*)src, client_stride, stride, rows,
+                         (int32_t)cols, (f16*)dst, (int32_t)dst_stride);
+      break;
+    default: return fc_internal_fail(-1, "bad dtype");
+  }
+  return fc_internal_check_launch("k_pack_rows");
+}
+
 int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, int32_t ntiles, int tile_rows,
               int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
               int64_t weight_client_stride, int64_t weight_stride, const void* bias, int64_t bias_client_stride,
               int activation, const void* residual, int64_t residual_stride, void* preactivation,
-              int64_t preactivation_stride, void* y, int64_t y_stride, int splits, void* workspace, int64_t workspace_bytes, void* stream) {
+              int64_t preactivation_stride, void* y, int64_t y_stride, int padded, int splits, void* workspace, int64_t workspace_bytes, void* stream) {
   if (ntiles < 0 || nclients <= 0 || in_features <= 0 || out_features <= 0) return fc_internal_fail(-1, "bad sizes");
   if (activation < 0 || activation > 3) return fc_internal_fail(-1, "bad activation");
   if (ntiles == 0) return 0;
@@ -730,7 +817,7 @@ int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, 
   p.z = preactivation; p.ld_z = preactivation_stride;
   p.out = y; p.ld_out = y_stride;
   p.act = activation;
-  p.splits = splits; p.part = (float*)workspace;
+  p.padded = padded; p.splits = splits; p.part = (float*)workspace;
   return dispatch<kForward>(dtype, p, ntiles, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -738,7 +825,7 @@ int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const
                              int tile_rows, int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
                              int64_t weight_client_stride, int64_t weight_stride, int activation,
                              const void* preactivation, int64_t preactivation_stride, const void* residual,
-                             int64_t residual_stride, void* dx, int64_t dx_stride, int splits, void* workspace,
+                             int64_t residual_stride, void* dx, int64_t dx_stride, int padded, int splits, void* workspace,
                              int64_t workspace_bytes, void* stream) {
   if (ntiles < 0 || nclients <= 0 || in_features <= 0 || out_features <= 0) return fc_internal_fail(-1, "bad sizes");
   if (activation < 0 || activation > 3) return fc_internal_fail(-1, "bad activation");
@@ -754,14 +841,14 @@ int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const
   p.out = dx; p.ld_out = dx_stride;
   p.act = activation;
   if (activation && !preactivation) return fc_internal_fail(-1, "an activation needs its pre-activation");
-  p.splits = splits; p.part = (float*)workspace;
+  p.padded = padded; p.splits = splits; p.part = (float*)workspace;
   return dispatch<kInput>(dtype, p, ntiles, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 
 int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
                               const int32_t* clients, int32_t nclients, int64_t in_features, int64_t out_features,
                               float* dweight, int64_t dweight_client_stride, int64_t dweight_stride, float* dbias,
-                              int64_t dbias_client_stride, int accumulate, int tile_rows, int splits, void* workspace,
+                              int64_t dbias_client_stride, int accumulate, int tile_rows, int padded, int splits, void* workspace,
                               int64_t workspace_bytes, void* stream) {
   if (nclients <= 0 || nclients > 65535 || in_features <= 0 || out_features <= 0)
     return fc_internal_fail(-1, "bad sizes");
@@ -774,7 +861,7 @@ int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, 
   p.out = dweight; p.ld_out = dweight_stride; p.out_client = dweight_client_stride;
   p.db = dbias; p.db_client = dbias_client_stride;
   p.accumulate = accumulate;
-  p.splits = splits; p.part = (float*)workspace;
+  p.padded = padded; p.splits = splits; p.part = (float*)workspace;
   return dispatch<kWeight>(dtype, p, 0, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 

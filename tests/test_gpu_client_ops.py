@@ -277,15 +277,19 @@ def test_linear_long_contractions(gpu, dtype):
   check_linear(gpu, np.random.default_rng(3), [5000, 3], 24, 40, dtype, "relu")
 
 
-@pytest.mark.parametrize("rows,splits", [(32, 1), (32, 5), (128, 1), (128, 3), (256, 1), (256, 2), (128, 64)])
+@pytest.mark.parametrize("rows,splits", [(32, 1), (32, 5), (128, 1), (128, 3), (256, 1), (256, 2), (128, 64), (32, 2)])
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_linear_every_plan(gpu, monkeypatch, dtype, rows, splits):
   """Each tile height and split of the contraction, whatever the sizes would choose: odd
   sizes (16-bit rows at odd addresses), sizes at multiples of 4 bytes, whole tiles."""
   monkeypatch.setattr(ops, "_plan", lambda tiles, steps, longest, size, aligned: (
       128 if rows == 256 and (size == 4 or not aligned) else rows, splits))
+  # odd rows as they lie, or copied to whole vectors first
+  monkeypatch.setattr(ops, "_estimate", lambda tiles, steps, longest, size, aligned: (
+      1e9 if aligned == (splits == 1) else 1.0, rows, splits))
   rng = np.random.default_rng(rows + splits)
   check_linear(gpu, rng, [40, 0, 1, 300], 131, 77, dtype, "gelu")
+  check_linear(gpu, rng, [40, 0, 1, 300], 131, 77, dtype, "relu", shared=True, behind=3)
   check_linear(gpu, rng, [257, 3], 134, 260, dtype, None)
   check_linear(gpu, rng, [256, 128, 31], 256, 256, dtype, "silu", shared=True)
   check_linear(gpu, rng, [5], 4, 2, dtype, "relu")
