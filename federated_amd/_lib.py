@@ -81,11 +81,11 @@ SIGNATURES = {
     "fc_linear_workspace_bytes": (_I64, [_I64, _INT, _INT]),
     "fc_pack_rows": (_INT, [_P, _I64, _I64, _INT, _I32, _I64, _I64, _P, _I64, _P]),
     "fc_linear": (_INT, [_P, _I64, _INT, _P, _I32, _INT, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64, _INT, _P, _I64,
-                         _P, _I64, _P, _I64, _INT, _INT, _P, _I64, _P]),
+                         _P, _I64, _P, _I64, _INT, _P, _I64, _P]),
     "fc_linear_backward_input": (_INT, [_P, _I64, _INT, _P, _I32, _INT, _I32, _I64, _I64, _P, _I64, _I64, _INT, _P,
-                                        _I64, _P, _I64, _P, _I64, _INT, _INT, _P, _I64, _P]),
+                                        _I64, _P, _I64, _P, _I64, _INT, _P, _I64, _P]),
     "fc_linear_backward_weight": (_INT, [_P, _I64, _P, _I64, _INT, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64,
-                                         _INT, _INT, _INT, _INT, _P, _I64, _P]),
+                                         _INT, _INT, _INT, _P, _I64, _P]),
     "fc_top_logits": (_INT, [_P, _I64, _INT, _I64, _I64, _I32, _F32, _P, _P, _P, _P]),
     "fc_distill": (_INT, [_P, _I64, _INT, _I64, _I64, _P, _P, _I32, _P, _P, _I32, _F32, _P, _P, _P, _P, _P, _P, _P,
                           _I64, _P]),

@@ -277,12 +277,14 @@ def _weight(weight, batch, dtype, inner=None, outer=None):
 
 
 # How long a product takes with tiles of `rows` rows, from one card's measurements (us):
-# a CU's time for one 128-byte k-step of one tile (16-bit types: 1.03 us for two 128 x
-# 128 tiles side by side, 1.8 for one of 256 x 256, 1.2 for four of 32 x 128; float32
-# runs at a fourth of the rate), a tile's start and end, and how many tiles a CU holds.
-# A k-step that waits for memory takes about 0.7 however little it computes.
-_TILE_COSTS = {32: (0.3, 5.0, 4), 128: (0.52, 9.0, 2), 256: (1.8, 12.0, 1)}
-_STEP_LATENCY = 0.7
+# a CU's time for one 128-byte k-step of one tile in 16-bit types (1.03 us for two 128 x
+# 128 tiles side by side, 1.8 for one of 256 x 256, 1.2 for four of 32 x 128) and in
+# float32 (the matrix unit's time), a tile's start and end, and how many a CU holds.  A
+# k-step takes 0.9 however little it computes, from the wait for memory.
+_TILE_COSTS = {32: (0.3, 0.53, 5.0, 4), 128: (0.52, 2.08, 9.0, 2), 256: (1.8, 0.0, 12.0, 1)}
+_STEP_LATENCY = 0.9
+# a further launch (the parts' join, an operand's copy), on the host: what counts in small calls
+_LAUNCH = 8.0
 _CUS = 256
 
 
@@ -297,10 +299,10 @@ def _estimate(tiles, steps, longest, size, aligned):
   8192: 2.1 ms whole, 2.9 in four).
   """
   best = None
-  for (rows, (step, ends, resident)), count in zip(_TILE_COSTS.items(), tiles):
+  for (rows, (step16, step32, ends, resident)), count in zip(_TILE_COSTS.items(), tiles):
     if rows == 256 and (size == 4 or not aligned):
       continue  # the kernel's limits
-    step *= 4 if size == 4 else 1
+    step = step32 if size == 4 else step16
     splits = 1
     while splits <= 16 and (splits == 1 or 2 * splits <= longest):
       blocks = max(1, count * splits)
@@ -313,7 +315,7 @@ def _estimate(tiles, steps, longest, size, aligned):
         if rest:
           t += max(_STEP_LATENCY * longest, -(-rest // _CUS) * step * steps) / splits + ends
       if splits > 1:  # the parts' write and read, and the joining launch
-        t += 4.0 + 2 * blocks * rows * max(128, rows) * 4 / 4e6
+        t += _LAUNCH + 2 * blocks * rows * max(128, rows) * 4 / 4e6
       if best is None or t < best[0]:
         best = (t, rows, splits)
       splits *= 2
@@ -345,7 +347,7 @@ def _packed(t, rows):
 
 
 def _operands(a, b, rows, tiles, steps, longest):
-  """A product's operands as it reads them: (a, b, padded, tile rows, splits).
+  """A product's operands as it reads them: (a, b, tile rows, splits).
 
   Rows of a 16-bit operand at odd elements go through registers, at about 2.2 times a
   step's cost (two thirds of the load rate, and the wait is in the step); copied to
@@ -355,17 +357,16 @@ def _operands(a, b, rows, tiles, steps, longest):
   """
   size = a.element_size()
   odd = (_odd(a), _odd(b)) if size == 2 else (0, 0)
-  padded = 0
   if (odd[0] or odd[1]) and rows:
-    copies = sum(4.0 + n * 4 / 4e6 for o, n in zip(odd, (rows * a.shape[1], _elements(b, rows))) if o)
+    copies = sum(_LAUNCH + n * 4 / 4e6 for o, n in zip(odd, (rows * a.shape[1], _elements(b, rows))) if o)
     if _estimate(tiles, steps, longest, 2, True)[0] + copies < 2.2 * _estimate(tiles, steps, longest, 2, False)[0]:
       if odd[0]:
-        a, padded = _packed(a, rows), 1
+        a = _packed(a, rows)
       if odd[1]:
-        b, padded = _packed(b, rows), padded | 2
+        b = _packed(b, rows)
       odd = (0, 0)
   height, splits = _plan(tiles, steps, longest, size, not (odd[0] or odd[1]))
-  return a, b, padded, height, splits
+  return a, b, height, splits
 
 
 def _elements(b, rows):
@@ -386,11 +387,11 @@ def _row_product(batch, columns, a, weight):
   n32, n128, n256 = batch.tile_counts
   narrow, wide = -(-columns // 128), -(-columns // 256)
   steps = -(-a.shape[1] * a.element_size() // 128)
-  a, weight, padded, rows, splits = _operands(a, weight, batch.num_rows, (n32 * narrow, n128 * narrow, n256 * wide),
+  a, weight, rows, splits = _operands(a, weight, batch.num_rows, (n32 * narrow, n128 * narrow, n256 * wide),
                                               steps, steps)
   tiles, _, ntiles = batch._tiles[rows]  # pylint: disable=protected-access
   ws = _workspace(ntiles * (wide if rows == 256 else narrow), rows, splits, batch.device)
-  return a, weight, (_ptr(tiles), ntiles, rows), (padded, splits, _ptr(ws), 0 if ws is None else ws.numel()), ws
+  return a, weight, (_ptr(tiles), ntiles, rows), (splits, _ptr(ws), 0 if ws is None else ws.numel()), ws
 
 
 def linear(x, weight, bias, batch, activation=None, residual=None, preactivation=False, out=None):
@@ -460,12 +461,12 @@ def linear_backward_weight(dz, x, batch, dweight=None, dbias=None, bias=True, ac
     dbias = _grad_out("dbias", dbias, batch, (m,))
   tiles = tuple(batch.num_clients * -(-m // h) * -(-k // max(128, h)) for h in _TILE_COSTS)
   per = 128 // x.element_size()
-  dz, x, padded, rows, splits = _operands(dz, x, batch.num_rows, tiles,
+  dz, x, rows, splits = _operands(dz, x, batch.num_rows, tiles,
                                           -(-batch.num_rows // (per * batch.num_clients)), -(-batch.longest // per))
   ws = _workspace(batch.num_clients * -(-m // rows) * -(-k // max(128, rows)), rows, splits, batch.device)
   _call(batch.device, "fc_linear_backward_weight", _ptr(dz), dz.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
         _ptr(batch._clients), batch.num_clients, k, m, _ptr(dweight), dweight.stride(0), dweight.stride(1),  # pylint: disable=protected-access
-        _ptr(dbias), _ld(dbias), int(bool(accumulate)), rows, padded, splits, _ptr(ws), 0 if ws is None else ws.numel())
+        _ptr(dbias), _ld(dbias), int(bool(accumulate)), rows, splits, _ptr(ws), 0 if ws is None else ws.numel())
   return dweight, dbias
 
 

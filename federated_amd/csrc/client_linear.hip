@@ -351,7 +351,6 @@ struct Args {
   int32_t accumulate;
   int32_t act;
   int32_t tiles_i, tiles_j;
-  int32_t padded;      // bit 0: a's rows, bit 1: b's can be read to a multiple of 8 elements
   int32_t splits;      // parts of the contraction, joined through `part`
   float* part;         // [tile][split][BM BN + BM]
 };
@@ -490,15 +489,16 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
     pa += first * step_a;
     pb += first * step_b;
   }
-  const bool edge_a = !kA_KC && ni < BM && ni % VEC && !(p.padded & 1);
-  const bool edge_b = !kB_KC && nj < BN && nj % VEC && !(p.padded & 2);
+  // An XC tile whose indices end inside a vector reads on into the next row: into columns
+  // that are not stored.  The last step, with no next row, goes by the edges.
+  const bool edge = (!kA_KC && ni < BM && ni % VEC) || (!kB_KC && nj < BN && nj % VEC);
   uint32_t oa[SA::kOffsets], ob[SB::kOffsets];
   if (!REG) {
     SA::offsets(oa, p.lda, ni);
     SB::offsets(ob, p.ldb, nj);
   }
   const int steps = (int)((nk + kK - 1) / kK);
-  const int full = edge_a || edge_b ? 0 : (int)(nk / kK);  // steps whose loads are all direct
+  const int full = edge ? min((int)(nk / kK), steps - 1) : (int)(nk / kK);  // steps whose loads are all direct
   typename SA::vec ra[REG ? SA::kChunks : 1];
   typename SB::vec rb[REG ? SB::kChunks : 1];
 
@@ -802,7 +802,7 @@ int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, 
               int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
               int64_t weight_client_stride, int64_t weight_stride, const void* bias, int64_t bias_client_stride,
               int activation, const void* residual, int64_t residual_stride, void* preactivation,
-              int64_t preactivation_stride, void* y, int64_t y_stride, int padded, int splits, void* workspace, int64_t workspace_bytes, void* stream) {
+              int64_t preactivation_stride, void* y, int64_t y_stride, int splits, void* workspace, int64_t workspace_bytes, void* stream) {
   if (ntiles < 0 || nclients <= 0 || in_features <= 0 || out_features <= 0) return fc_internal_fail(-1, "bad sizes");
   if (activation < 0 || activation > 3) return fc_internal_fail(-1, "bad activation");
   if (ntiles == 0) return 0;
@@ -817,7 +817,7 @@ int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, 
   p.z = preactivation; p.ld_z = preactivation_stride;
   p.out = y; p.ld_out = y_stride;
   p.act = activation;
-  p.padded = padded; p.splits = splits; p.part = (float*)workspace;
+  p.splits = splits; p.part = (float*)workspace;
   return dispatch<kForward>(dtype, p, ntiles, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -825,7 +825,7 @@ int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const
                              int tile_rows, int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
                              int64_t weight_client_stride, int64_t weight_stride, int activation,
                              const void* preactivation, int64_t preactivation_stride, const void* residual,
-                             int64_t residual_stride, void* dx, int64_t dx_stride, int padded, int splits, void* workspace,
+                             int64_t residual_stride, void* dx, int64_t dx_stride, int splits, void* workspace,
                              int64_t workspace_bytes, void* stream) {
   if (ntiles < 0 || nclients <= 0 || in_features <= 0 || out_features <= 0) return fc_internal_fail(-1, "bad sizes");
   if (activation < 0 || activation > 3) return fc_internal_fail(-1, "bad activation");
@@ -841,14 +841,14 @@ int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const
   p.out = dx; p.ld_out = dx_stride;
   p.act = activation;
   if (activation && !preactivation) return fc_internal_fail(-1, "an activation needs its pre-activation");
-  p.padded = padded; p.splits = splits; p.part = (float*)workspace;
+  p.splits = splits; p.part = (float*)workspace;
   return dispatch<kInput>(dtype, p, ntiles, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 
 int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
                               const int32_t* clients, int32_t nclients, int64_t in_features, int64_t out_features,
                               float* dweight, int64_t dweight_client_stride, int64_t dweight_stride, float* dbias,
-                              int64_t dbias_client_stride, int accumulate, int tile_rows, int padded, int splits, void* workspace,
+                              int64_t dbias_client_stride, int accumulate, int tile_rows, int splits, void* workspace,
                               int64_t workspace_bytes, void* stream) {
   if (nclients <= 0 || nclients > 65535 || in_features <= 0 || out_features <= 0)
     return fc_internal_fail(-1, "bad sizes");
@@ -861,7 +861,7 @@ int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, 
   p.out = dweight; p.ld_out = dweight_stride; p.out_client = dweight_client_stride;
   p.db = dbias; p.db_client = dbias_client_stride;
   p.accumulate = accumulate;
-  p.padded = padded; p.splits = splits; p.part = (float*)workspace;
+  p.splits = splits; p.part = (float*)workspace;
   return dispatch<kWeight>(dtype, p, 0, tile_rows, workspace_bytes, (hipStream_t)stream);
 }
 

@@ -479,8 +479,7 @@ int fc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
 
 /* Rows copied to a stride of whole 16-byte vectors, [nclients][rows][dst_stride], zeros
  * behind cols: what 16-bit operands with rows at odd elements are worth where they are
- * read often.  A product's `padded` says whose rows can be read to a multiple of 8
- * elements, the last row's too: bit 0 its first operand's, bit 1 its second's. */
+ * read often. */
 int fc_pack_rows(const void* src, int64_t client_stride, int64_t stride, int dtype, int32_t nclients, int64_t rows,
                  int64_t cols, void* dst, int64_t dst_stride, void* stream);
 
@@ -494,7 +493,7 @@ int fc_linear(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, 
               int32_t nclients, int64_t in_features, int64_t out_features, const void* weight,
               int64_t weight_client_stride, int64_t weight_stride, const void* bias, int64_t bias_client_stride,
               int activation, const void* residual, int64_t residual_stride, void* preactivation,
-              int64_t preactivation_stride, void* y, int64_t y_stride, int padded, int splits, void* workspace,
+              int64_t preactivation_stride, void* y, int64_t y_stride, int splits, void* workspace,
               int64_t workspace_bytes, void* stream);
 
 /* dx = (dz weight_c) * act'(preactivation) + residual. */
@@ -502,7 +501,7 @@ int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const
                              int tile_rows, int32_t nclients, int64_t in_features, int64_t out_features,
                              const void* weight, int64_t weight_client_stride, int64_t weight_stride, int activation,
                              const void* preactivation, int64_t preactivation_stride, const void* residual,
-                             int64_t residual_stride, void* dx, int64_t dx_stride, int padded, int splits, void* workspace,
+                             int64_t residual_stride, void* dx, int64_t dx_stride, int splits, void* workspace,
                              int64_t workspace_bytes, void* stream);
 
 /* dweight_c = sum of dz_r x_r^T, dbias_c (nullable) = sum of dz_r over the client's
@@ -511,7 +510,7 @@ int fc_linear_backward_input(const void* dz, int64_t dz_stride, int dtype, const
 int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
                               const int32_t* clients, int32_t nclients, int64_t in_features, int64_t out_features,
                               float* dweight, int64_t dweight_client_stride, int64_t dweight_stride, float* dbias,
-                              int64_t dbias_client_stride, int accumulate, int tile_rows, int padded, int splits, void* workspace,
+                              int64_t dbias_client_stride, int accumulate, int tile_rows, int splits, void* workspace,
                               int64_t workspace_bytes, void* stream);
 
 /* The k largest logits of every row, falling, ties to the lowest index, NaN below every

@@ -97,7 +97,7 @@ def test_linear_refusals():
 
   def forward(dtype=1, ntiles=1, rows=128, clients=1, k=8, m=8, act=0, splits=1, ws=NULL, nbytes=0, x=b, stride=8):
     return lib.fc_linear(x, stride, dtype, b, ntiles, rows, clients, k, m, b, 64, 8, NULL, 0, act, NULL, 0, NULL, 0, b,
-                         8, 0, splits, ws, nbytes, None)
+                         8, splits, ws, nbytes, None)
 
   refused(forward(k=0), b"sizes")
   refused(forward(clients=0), b"sizes")
@@ -115,7 +115,7 @@ def test_linear_refusals():
   assert forward(ntiles=0) == 0
 
   def backward_input(act=0, pre=NULL, dz=b):
-    return lib.fc_linear_backward_input(dz, 8, 1, b, 1, 128, 1, 8, 8, b, 64, 8, act, pre, 8, NULL, 0, b, 8, 0, 1, NULL, 0,
+    return lib.fc_linear_backward_input(dz, 8, 1, b, 1, 128, 1, 8, 8, b, 64, 8, act, pre, 8, NULL, 0, b, 8, 1, NULL, 0,
                                         None)
 
   refused(backward_input(act=1), b"pre-activation")
@@ -123,7 +123,7 @@ def test_linear_refusals():
   refused(backward_input(dz=NULL), b"null")
 
   def weight(clients=1, m=8, dw=b, splits=1):
-    return lib.fc_linear_backward_weight(b, 8, b, 8, 1, b, clients, 8, m, dw, 64, 8, NULL, 0, 0, 128, 0, splits, NULL, 0,
+    return lib.fc_linear_backward_weight(b, 8, b, 8, 1, b, clients, 8, m, dw, 64, 8, NULL, 0, 0, 128, splits, NULL, 0,
                                          None)
 
   refused(weight(clients=0), b"sizes")
