@@ -17,13 +17,17 @@ Activations and weights are float32, bfloat16 or float16, of one type per call;
 sums, statistics and gradients of weights are held in float32.  All calls are
 asynchronous on the current stream of the tensors' device, allocate what they return
 (unless given ``out``) and keep nothing.  Rows behind the batch's last are not read;
-in a given output they are left as they were, in an allocated one they are zero.
+in a given output they are left as they were, in an allocated one they are zero.  A
+given output shares no memory with the call's other tensors (rows side by side in one
+buffer are apart), but may be ``residual`` itself.  A batch whose calls were captured
+into a graph has to live as long as the graph.
 
 Forward and backward are separate calls with explicit gradients: a broadcast weight
 still gets one gradient per client, which is what the codec encodes.
 """
 import ctypes
 import functools
+import operator
 
 import numpy as np
 import torch
@@ -34,6 +38,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
 _TILES = (16, 32, 128, 256)
 MAX_TOP = 1024  # FC_MAX_TOP
+MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-15, 1e15  # FC_MIN_TEMPERATURE, FC_MAX_TEMPERATURE
 
 
 class ClientBatch:
@@ -79,11 +84,17 @@ class ClientBatch:
     for p, s in zip(parts, starts):
       host[s:s + p.size] = p.reshape(-1)
     dev = torch.from_numpy(host).to(self.device)
+    self._buffer, self._streams = dev, {torch.cuda.current_stream(self.device).cuda_stream}
     views = [dev[s:s + p.size] for p, s in zip(parts, starts)]
     self.offsets, self.row_client, self._clients = views[:3]
     self._tiles = {rows: (views[3 + 2 * i], views[4 + 2 * i], parts[3 + 2 * i].shape[0])
                    for i, rows in enumerate(_TILES)}
     self.tile_counts = tuple(self._tiles[rows][2] for rows in _TILE_COSTS)
+
+  def _used_on(self, stream):
+    """The tables are read on another stream than they were made on (a raw handle, the current one)."""
+    self._buffer.record_stream(torch.cuda.current_stream(self.device))
+    self._streams.add(stream)
 
   def _tile_table(self, rows):
     lib = _lib.load()
@@ -146,19 +157,51 @@ def _params(name, t, batch, shape, dtype):
   return t
 
 
-def _grad_out(name, t, batch, shape):
+def _grad_out(name, t, batch, shape, **others):
   if t is None:
     return torch.empty((batch.num_clients,) + shape, dtype=torch.float32, device=batch.device)
-  return _distinct(name, _params(name, t, batch, shape, torch.float32))
+  _distinct(name, _params(name, t, batch, shape, torch.float32))
+  _apart(name, t, **others)
+  return t
 
 
-def _out(name, out, like, batch, width):
+def _out(name, out, like, batch, width, itself=None, **others):
   if out is not None:
-    return _distinct(name, _activations(name, out, batch, width, like))
+    _distinct(name, _activations(name, out, batch, width, like))
+    _apart(name, out, itself, **others)
+    return out
   out = torch.empty((like.shape[0], width), dtype=like.dtype, device=like.device)
   if like.shape[0] > batch.num_rows:
     out[batch.num_rows:].zero_()
   return out
+
+
+def _extent(t):
+  """(first byte, bytes of an outermost entry, bytes between those, entries)."""
+  size = t.element_size()
+  inner = 1
+  for n, stride in zip(t.shape[1:], t.stride()[1:]):
+    inner += (n - 1) * stride
+  return t.data_ptr(), inner * size, t.stride(0) * size, t.shape[0]
+
+
+def _apart(name, out, itself=None, **others):
+  """A given output that must not share memory with the call's other tensors.
+
+  Rows side by side in a wider buffer are apart; the one in ``itself`` may be ``out``.
+  """
+  if itself is not None and itself.data_ptr() == out.data_ptr() and itself.stride() == out.stride():
+    itself = None
+  start, inner, outer, n = _extent(out)
+  for other, t in list(others.items()) + [("an input", itself)]:
+    if t is None or not n or not t.shape[0]:
+      continue
+    start2, inner2, outer2, n2 = _extent(t)
+    if start + (n - 1) * outer + inner <= start2 or start2 + (n2 - 1) * outer2 + inner2 <= start:
+      continue
+    if outer == outer2 > 0 and (start2 - start) % outer >= inner and (start - start2) % outer >= inner2:
+      continue
+    raise ValueError("%s shares memory with %s" % (name, other))
 
 
 def _vector(name, t, rows, device):
@@ -186,12 +229,16 @@ def _ld(t):
   return 0 if t is None else t.stride(0)
 
 
-def _call(device, name, *args):
-  """A C entry point on the current stream of `device`."""
+def _call(where, name, *args):
+  """A C entry point on the current stream of `where`: a batch, or a device."""
+  batch = where if isinstance(where, ClientBatch) else None
+  device = batch.device if batch else where
   index = device.index
   # the raw handle: torch.cuda.current_stream(device) makes a Stream object, at 2 us a
   # sixth of a small call
   stream = torch._C._cuda_getCurrentRawStream(index)  # pylint: disable=protected-access
+  if batch and stream not in batch._streams:  # pylint: disable=protected-access
+    batch._used_on(stream)  # pylint: disable=protected-access
   fn = getattr(_lib.load(), name)
   if index == torch.cuda.current_device():
     rc = fn(*args, stream)
@@ -216,10 +263,12 @@ def layer_norm(x, weight, bias, batch, eps=1e-5, out=None):
   for name, t in (("weight", weight), ("bias", bias)):
     if t is not None:
       _params(name, t, batch, (dim,), x.dtype)
-  out = _out("out", out, x, batch, dim)
+  if not 0.0 <= float(eps) < float("inf"):
+    raise ValueError("eps must not be negative, got %r" % (eps,))
+  out = _out("out", out, x, batch, dim, x=x, weight=weight, bias=bias)
   mean, rstd = _stats(x.shape[0], batch), _stats(x.shape[0], batch)
   tiles, _, ntiles = batch._tiles[16]  # pylint: disable=protected-access
-  _call(batch.device, "fc_layer_norm", _ptr(x), x.stride(0), _DTYPES[x.dtype], _ptr(tiles), ntiles, dim,
+  _call(batch, "fc_layer_norm", _ptr(x), x.stride(0), _DTYPES[x.dtype], _ptr(tiles), ntiles, dim,
         _ptr(weight), _ld(weight), _ptr(bias), _ld(bias), float(eps), _ptr(out), out.stride(0), _ptr(mean),
         _ptr(rstd))
   return out, mean, rstd
@@ -244,12 +293,13 @@ def layer_norm_backward(dy, x, mean, rstd, weight, batch, residual=None, dweight
     _activations("residual", residual, batch, dim, x)
   if accumulate and (dweight is None or dbias is None):
     raise ValueError("accumulate needs dweight and dbias to add to")
-  dweight = _grad_out("dweight", dweight, batch, (dim,))
-  dbias = _grad_out("dbias", dbias, batch, (dim,))
-  out = _out("out", out, x, batch, dim)
+  inputs = dict(dy=dy, x=x, mean=mean, rstd=rstd, weight=weight)
+  dbias = _grad_out("dbias", dbias, batch, (dim,), residual=residual, **inputs)
+  dweight = _grad_out("dweight", dweight, batch, (dim,), dbias=dbias, residual=residual, **inputs)
+  out = _out("out", out, x, batch, dim, residual, dweight=dweight, dbias=dbias, **inputs)
   tiles, first, ntiles = batch._tiles[32]  # pylint: disable=protected-access
   part = torch.empty(ntiles * 2 * dim, dtype=torch.float32, device=batch.device)
-  _call(batch.device, "fc_layer_norm_backward", _ptr(dy), dy.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
+  _call(batch, "fc_layer_norm_backward", _ptr(dy), dy.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
         _ptr(mean), _ptr(rstd), _ptr(tiles), ntiles, _ptr(first), batch.num_clients, dim, _ptr(weight), _ld(weight),
         _ptr(residual), _ld(residual), _ptr(out), out.stride(0), _ptr(dweight), dweight.stride(0), _ptr(dbias),
         dbias.stride(0), int(bool(accumulate)), _ptr(part))
@@ -327,8 +377,11 @@ def _plan(tiles, steps, longest, size, aligned):
 
 
 def _odd(t):
-  """Whether some row of a 16-bit operand starts at an odd element (of a 4-byte word)."""
-  return t.data_ptr() & 3 or (t.stride(0) | t.stride(-2)) & 1
+  """Whether some row of a 16-bit operand starts at an odd element (of a 4-byte word).
+
+  Or the rows are too far apart for 32-bit offsets inside a tile.
+  """
+  return t.data_ptr() & 3 or (t.stride(0) | t.stride(-2)) & 1 or t.stride(-2) >= 1 << 22
 
 
 def _packed(t, rows):
@@ -358,7 +411,7 @@ def _operands(a, b, rows, tiles, steps, longest):
   size = a.element_size()
   odd = (_odd(a), _odd(b)) if size == 2 else (0, 0)
   if (odd[0] or odd[1]) and rows:
-    copies = sum(_LAUNCH + n * 4 / 4e6 for o, n in zip(odd, (rows * a.shape[1], _elements(b, rows))) if o)
+    copies = sum(2 * _LAUNCH + n * 4 / 4e6 for o, n in zip(odd, (rows * a.shape[1], _elements(b, rows))) if o)
     if _estimate(tiles, steps, longest, 2, True)[0] + copies < 2.2 * _estimate(tiles, steps, longest, 2, False)[0]:
       if odd[0]:
         a = _packed(a, rows)
@@ -387,8 +440,7 @@ def _row_product(batch, columns, a, weight):
   n32, n128, n256 = batch.tile_counts
   narrow, wide = -(-columns // 128), -(-columns // 256)
   steps = -(-a.shape[1] * a.element_size() // 128)
-  a, weight, rows, splits = _operands(a, weight, batch.num_rows, (n32 * narrow, n128 * narrow, n256 * wide),
-                                              steps, steps)
+  a, weight, rows, splits = _operands(a, weight, batch.num_rows, (n32 * narrow, n128 * narrow, n256 * wide), steps, steps)
   tiles, _, ntiles = batch._tiles[rows]  # pylint: disable=protected-access
   ws = _workspace(ntiles * (wide if rows == 256 else narrow), rows, splits, batch.device)
   return a, weight, (_ptr(tiles), ntiles, rows), (splits, _ptr(ws), 0 if ws is None else ws.numel()), ws
@@ -409,10 +461,10 @@ def linear(x, weight, bias, batch, activation=None, residual=None, preactivation
     _params("bias", bias, batch, (m,), x.dtype)
   if residual is not None:
     _activations("residual", residual, batch, m, x)
-  out = _out("out", out, x, batch, m)
+  out = _out("out", out, x, batch, m, residual, x=x, weight=weight, bias=bias)
   z = _out("z", None, x, batch, m) if preactivation else None
   x, weight, tiles, last, _ws = _row_product(batch, m, x, weight)
-  _call(batch.device, "fc_linear", _ptr(x), x.stride(0), _DTYPES[x.dtype], *tiles, batch.num_clients, k, m,
+  _call(batch, "fc_linear", _ptr(x), x.stride(0), _DTYPES[x.dtype], *tiles, batch.num_clients, k, m,
         _ptr(weight), weight.stride(0), weight.stride(1), _ptr(bias), _ld(bias), act, _ptr(residual), _ld(residual),
         _ptr(z), _ld(z), _ptr(out), out.stride(0), *last)
   return (out, z) if preactivation else out
@@ -434,9 +486,9 @@ def linear_backward_input(dz, weight, batch, preactivation=None, activation=None
     _activations("preactivation", preactivation, batch, k, dz)
   if residual is not None:
     _activations("residual", residual, batch, k, dz)
-  out = _out("out", out, dz, batch, k)
+  out = _out("out", out, dz, batch, k, residual, dz=dz, weight=weight, preactivation=preactivation)
   dz, weight, tiles, last, _ws = _row_product(batch, k, dz, weight)
-  _call(batch.device, "fc_linear_backward_input", _ptr(dz), dz.stride(0), _DTYPES[dz.dtype], *tiles,
+  _call(batch, "fc_linear_backward_input", _ptr(dz), dz.stride(0), _DTYPES[dz.dtype], *tiles,
         batch.num_clients, k, m, _ptr(weight), weight.stride(0), weight.stride(1), act, _ptr(preactivation),
         _ld(preactivation), _ptr(residual), _ld(residual), _ptr(out), out.stride(0), *last)
   return out
@@ -456,15 +508,15 @@ def linear_backward_weight(dz, x, batch, dweight=None, dbias=None, bias=True, ac
     raise ValueError("dbias given with bias=False")
   if accumulate and (dweight is None or (bias and dbias is None)):
     raise ValueError("accumulate needs dweight and dbias to add to")
-  dweight = _grad_out("dweight", dweight, batch, (m, k))
   if bias:
-    dbias = _grad_out("dbias", dbias, batch, (m,))
+    dbias = _grad_out("dbias", dbias, batch, (m,), dz=dz, x=x)
+  dweight = _grad_out("dweight", dweight, batch, (m, k), dz=dz, x=x, dbias=dbias)
   tiles = tuple(batch.num_clients * -(-m // h) * -(-k // max(128, h)) for h in _TILE_COSTS)
   per = 128 // x.element_size()
-  dz, x, rows, splits = _operands(dz, x, batch.num_rows, tiles,
-                                          -(-batch.num_rows // (per * batch.num_clients)), -(-batch.longest // per))
+  dz, x, rows, splits = _operands(dz, x, batch.num_rows, tiles, -(-batch.num_rows // (per * batch.num_clients)),
+                                  -(-batch.longest // per))
   ws = _workspace(batch.num_clients * -(-m // rows) * -(-k // max(128, rows)), rows, splits, batch.device)
-  _call(batch.device, "fc_linear_backward_weight", _ptr(dz), dz.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
+  _call(batch, "fc_linear_backward_weight", _ptr(dz), dz.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
         _ptr(batch._clients), batch.num_clients, k, m, _ptr(dweight), dweight.stride(0), dweight.stride(1),  # pylint: disable=protected-access
         _ptr(dbias), _ld(dbias), int(bool(accumulate)), rows, splits, _ptr(ws), 0 if ws is None else ws.numel())
   return dweight, dbias
@@ -486,7 +538,7 @@ def top_logits(logits, k, temperature=1.0):
     raise ValueError("logits must be float32, bfloat16 or float16, got %s" % logits.dtype)
   _rows_ok("logits", logits)
   rows, vocab = logits.shape
-  k = int(k)
+  k = operator.index(k)
   if not 1 <= k <= min(vocab, MAX_TOP):
     raise ValueError("k must be in [1, %d], got %d" % (min(vocab, MAX_TOP), k))
   _temperature(temperature)
@@ -499,8 +551,8 @@ def top_logits(logits, k, temperature=1.0):
 
 
 def _temperature(t):
-  if not 0.0 < float(t) < float("inf"):
-    raise ValueError("temperature must be positive and finite, got %r" % (t,))
+  if not MIN_TEMPERATURE <= float(t) <= MAX_TEMPERATURE:
+    raise ValueError("temperature must be in [%g, %g], got %r" % (MIN_TEMPERATURE, MAX_TEMPERATURE, t))
 
 
 def _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights):
@@ -527,7 +579,7 @@ def _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weigh
 def _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, lse, grad, want_loss, dloss):
   loss = torch.empty(batch.num_clients, dtype=torch.float32, device=batch.device) if want_loss else None
   row_loss = torch.empty(batch.num_rows, dtype=torch.float32, device=batch.device) if want_loss else None
-  _call(batch.device, "fc_distill", _ptr(logits), logits.stride(0), _DTYPES[logits.dtype], batch.num_rows,
+  _call(batch, "fc_distill", _ptr(logits), logits.stride(0), _DTYPES[logits.dtype], batch.num_rows,
         logits.shape[1], _ptr(indices), _ptr(values), indices.shape[1], _ptr(batch.row_client), _ptr(batch.offsets),
         batch.num_clients, float(temperature), _ptr(teacher_lse), _ptr(row_weights), _ptr(dloss), _ptr(row_loss),
         _ptr(lse), _ptr(loss), _ptr(grad), _ld(grad))
@@ -565,7 +617,7 @@ def distillation_backward(logits, lse, indices, values, batch, temperature=1.0, 
   _vector("lse", lse, batch.num_rows, batch.device)
   if dloss is not None:
     _vector("dloss", dloss, batch.num_clients, batch.device)
-  out = _out("out", out, logits, batch, logits.shape[1])
+  out = _out("out", out, logits, batch, logits.shape[1], logits, indices=indices, values=values, lse=lse)
   _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, lse, out, False, dloss)
   return out
 
@@ -577,6 +629,6 @@ def distillation_with_gradient(logits, indices, values, batch, temperature=1.0, 
   ``out`` may be ``logits`` itself.
   """
   indices, values = _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights)
-  out = _out("out", out, logits, batch, logits.shape[1])
+  out = _out("out", out, logits, batch, logits.shape[1], logits, indices=indices, values=values)
   loss = _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, None, out, True, None)
   return loss, out

@@ -10,6 +10,7 @@
 // ("KC": a row of 16-byte chunks along k) or along their own index ("XC").
 #include "client_common.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -490,15 +491,17 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
     pb += first * step_b;
   }
   // An XC tile whose indices end inside a vector reads on into the next row: into columns
-  // that are not stored.  The last step, with no next row, goes by the edges.
-  const bool edge = (!kA_KC && ni < BM && ni % VEC) || (!kB_KC && nj < BN && nj % VEC);
+  // that are not stored.  The last step, with no next row, goes by the edges, and so does
+  // every step where the vector would go past that row too.
+  const bool edge_a = !kA_KC && ni < BM && ni % VEC, edge_b = !kB_KC && nj < BN && nj % VEC, edge = edge_a || edge_b;
   uint32_t oa[SA::kOffsets], ob[SB::kOffsets];
   if (!REG) {
     SA::offsets(oa, p.lda, ni);
     SB::offsets(ob, p.ldb, nj);
   }
   const int steps = (int)((nk + kK - 1) / kK);
-  const int full = edge ? min((int)(nk / kK), steps - 1) : (int)(nk / kK);  // steps whose loads are all direct
+  int full = (int)(nk / kK);  // steps whose loads are all direct
+  if (edge) full = (edge_a && p.lda < VEC) || (edge_b && p.ldb < VEC) ? 0 : min(full, steps - 1);
   typename SA::vec ra[REG ? SA::kChunks : 1];
   typename SB::vec rb[REG ? SB::kChunks : 1];
 
@@ -697,16 +700,20 @@ __global__ __launch_bounds__(256) void k_linear_join(const Args p) {
 // Rows copied to a stride of whole 16-byte vectors: [clients][rows][out_ld], zeros behind
 // `cols`.  A thread per vector.
 template <typename T>
-__global__ __launch_bounds__(256) void k_pack_rows(const T* src, int64_t client, int64_t ld, int64_t rows, int32_t cols,
-                                                   T* dst, int32_t out_ld) {
+__global__ __launch_bounds__(256) void k_pack_rows(const T* src, int64_t client, int64_t ld, int32_t blocks, int64_t rows,
+                                                   int32_t cols, T* dst, int32_t out_ld) {
   constexpr int VEC = Elem<T>::kVec;
-  const int64_t per = out_ld / VEC, q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t which = blockIdx.x / blocks, per = out_ld / VEC;
+  const int64_t q = (blockIdx.x - which * blocks) * 256 + threadIdx.x;
   if (q >= rows * per) return;
   const int64_t r = q / per;
   const int c = (int)(q - r * per) * VEC;
-  const T* from = src + blockIdx.y * client + r * ld + c;
-  *(typename VecOf<T>::type*)(dst + (blockIdx.y * rows + r) * out_ld + c) = load_vec(from, cols - c);
+  const T* from = src + which * client + r * ld + c;
+  *(typename VecOf<T>::type*)(dst + (which * rows + r) * out_ld + c) = load_vec(from, cols - c);
 }
+
+constexpr int64_t kMaxBlocks = (1LL << 32) / 256 - 1;  // a launch has fewer than 2^32 threads
+constexpr int64_t kMaxSide = 1LL << 31;
 
 // Every address of the operand a multiple of 4 bytes: row stride, client stride, base.
 bool dword_aligned(const void* base, int64_t ld, int64_t client, size_t size) {
@@ -715,13 +722,15 @@ bool dword_aligned(const void* base, int64_t ld, int64_t client, size_t size) {
 
 template <typename T, int KIND, int BM, int BN, int WM, int WN>
 int launch(Args p, int32_t ntiles, int64_t workspace_bytes, hipStream_t s) {
+  constexpr int NT = WM * WN * 64;
+  if (p.ni >= kMaxSide || p.nj >= kMaxSide || p.nk >= kMaxSide) return fc_internal_fail(-1, "bad sizes");
   p.tiles_j = (int32_t)((p.nj + BN - 1) / BN);
   p.tiles_i = KIND == kWeight ? (int32_t)((p.ni + BM - 1) / BM) : ntiles;
   const int64_t blocks = (int64_t)p.tiles_i * p.tiles_j * (KIND == kWeight ? p.nclients : 1);
-  if (blocks > 0x7fffffffLL) return fc_internal_fail(-1, "too many tiles");
+  if (blocks > kMaxBlocks / std::max(1, NT / 256)) return fc_internal_fail(-1, "too many tiles");
   if (p.splits > 1 && (!p.part || workspace_bytes < blocks * p.splits * (BM * BN + BM) * (int64_t)sizeof(float)))
     return fc_internal_fail(-1, "workspace too small");
-  const dim3 grid((unsigned)blocks, (unsigned)p.splits), block(WM * WN * 64);
+  const dim3 grid((unsigned)blocks, (unsigned)p.splits), block(NT);
   const bool direct = dword_aligned(p.a, p.lda, 0, sizeof(T)) && dword_aligned(p.b, p.ldb, p.b_client, sizeof(T)) &&
                       p.lda < (1 << 22) && p.ldb < (1 << 22);  // offsets inside a tile in 32 bits
   if (direct) {
@@ -773,25 +782,26 @@ int64_t fc_linear_workspace_bytes(int64_t blocks, int tile_rows, int splits) {
 
 int fc_pack_rows(const void* src, int64_t client_stride, int64_t stride, int dtype, int32_t nclients, int64_t rows,
                  int64_t cols, void* dst, int64_t dst_stride, void* stream) {
-  if (nclients <= 0 || nclients > 65535 || rows < 0 || cols <= 0 || dst_stride < cols || dst_stride > 0x7fffffff)
+  if (nclients <= 0 || rows < 0 || cols <= 0 || dst_stride < cols || dst_stride > 0x7fffffff)
     return fc_internal_fail(-1, "bad sizes");
   if (rows == 0) return 0;
   if (!src || !dst) return fc_internal_fail(-1, "null pointer");
   const int64_t vec = dtype == FC_FLOAT32 ? 4 : 8;
   if (dst_stride % vec || (uintptr_t)dst % 16) return fc_internal_fail(-1, "dst is not in whole 16-byte vectors");
+  if (rows >= kMaxSide) return fc_internal_fail(-1, "bad sizes");
   const int64_t blocks = (rows * (dst_stride / vec) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return fc_internal_fail(-1, "too many rows");
-  const dim3 grid((unsigned)blocks, (unsigned)nclients);
+  if (blocks > kMaxBlocks / nclients) return fc_internal_fail(-1, "too many rows");
+  const dim3 grid((unsigned)(blocks * nclients));
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case FC_FLOAT32:
-      hipLaunchKernelGGL((k_pack_rows<float>), grid, dim3(256), 0, s, (const float*)src, client_stride, stride, rows,
-                         (int32_t)cols, (float*)dst, (int32_t)dst_stride);
+      hipLaunchKernelGGL((k_pack_rows<float>), grid, dim3(256), 0, s, (const float*)src, client_stride, stride,
+                         (int32_t)blocks, rows, (int32_t)cols, (float*)dst, (int32_t)dst_stride);
       break;
     case FC_BFLOAT16:
     case FC_FLOAT16:  // a copy: 16 bits are 16 bits
-      hipLaunchKernelGGL((k_pack_rows<f16>), grid, dim3(256), 0, s, (const f16*)src, client_stride, stride, rows,
-                         (int32_t)cols, (f16*)dst, (int32_t)dst_stride);
+      hipLaunchKernelGGL((k_pack_rows<f16>), grid, dim3(256), 0, s, (const f16*)src, client_stride, stride,
+                         (int32_t)blocks, rows, (int32_t)cols, (f16*)dst, (int32_t)dst_stride);
       break;
     default: return fc_internal_fail(-1, "bad dtype");
   }
@@ -850,8 +860,7 @@ int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, 
                               float* dweight, int64_t dweight_client_stride, int64_t dweight_stride, float* dbias,
                               int64_t dbias_client_stride, int accumulate, int tile_rows, int splits, void* workspace,
                               int64_t workspace_bytes, void* stream) {
-  if (nclients <= 0 || nclients > 65535 || in_features <= 0 || out_features <= 0)
-    return fc_internal_fail(-1, "bad sizes");
+  if (nclients <= 0 || in_features <= 0 || out_features <= 0) return fc_internal_fail(-1, "bad sizes");
   if (!clients || !dweight) return fc_internal_fail(-1, "null pointer");
   Args p = {};
   p.a = dz; p.lda = dz_stride;

@@ -5,7 +5,6 @@
 #include "client_common.h"
 
 #include <algorithm>
-#include <cmath>
 #include <type_traits>
 
 namespace {
@@ -13,7 +12,6 @@ namespace {
 using namespace fc;
 
 constexpr float kLog2e = 1.44269504f;
-constexpr float kLn2 = 0.69314718f;
 
 // ---------------------------------------------------------------------------
 // Layer norm
@@ -319,11 +317,11 @@ __global__ __launch_bounds__(256) void k_norm_backward_long(const NormArgs p) {
 // dg_c, db_c: the client's tiles' partial rows.  A block adds up 64 columns, its four waves
 // every fourth tile each, joined in wave order.
 __global__ __launch_bounds__(256) void k_norm_join(const float* part, const int32_t* first_tile, int32_t dim,
-                                                   float* dw, int64_t ld_dw, float* db, int64_t ld_db,
+                                                   int32_t blocks, float* dw, int64_t ld_dw, float* db, int64_t ld_db,
                                                    int accumulate) {
   __shared__ float sums[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.y * 64 + lane, client = blockIdx.x, which = blockIdx.z;
+  const int client = blockIdx.x / blocks, c = (blockIdx.x - client * blocks) * 64 + lane, which = blockIdx.y;
   float* o = which ? db : dw;
   if (!o) return;
   const int hi = first_tile[client + 1];
@@ -400,18 +398,16 @@ struct Row {
   }
 };
 
-// A running maximum m of f and sum of exp2(f scale - r), r = m scale (0 while nothing but
-// -inf and NaN came by).  r is rounded once and then exact: each term is one multiply-add
-// and one exp2.  A NaN makes the sum NaN, and so does +inf.
+// A running maximum m of f and sum of exp2((f - c) scale), c = m (0 while nothing but -inf
+// and NaN came by).  The difference comes before the scale: a row of nothing but a type's
+// lowest values is a uniform one.  A NaN makes the sum NaN, and so does +inf.
 struct Softmax {
-  float m = -INFINITY, r = 0.0f, sum = 0.0f;
+  float m = -INFINITY, c = 0.0f, sum = 0.0f;
 
   __device__ __forceinline__ void raise(float to, float scale) {
     if (to > m) {
-      const float next = to * scale;
-      sum *= m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(r - next);
-      m = to;
-      r = next;
+      sum *= m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((c - to) * scale);
+      m = c = to;
     }
   }
 
@@ -422,16 +418,15 @@ struct Softmax {
     for (int e = 1; e < N; ++e) high = fmaxf(high, f[e]);
     raise(high, scale);
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], scale, -r));
+    for (int e = 0; e < N; ++e) sum += __builtin_amdgcn_exp2f((f[e] - c) * scale);
   }
 
   // log sum exp(f / tau), scale = log2(e) / tau
-  __device__ __forceinline__ float lse(float inv_tau, float scale) const {
+  __device__ __forceinline__ float lse(float inv_tau) const {
     if (m == -INFINITY) return sum == 0.0f ? -INFINITY : sum;
-    return m * inv_tau + (__builtin_fmaf(-m, scale, r) * kLn2 + logf(sum));
+    return m * inv_tau + logf(sum);
   }
 };
-
 
 // Orders as the float does; -0 = +0; NaN lowest.
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -526,7 +521,7 @@ __global__ __launch_bounds__(NT) void k_top_logits(const T* logits, int64_t ld, 
     sm.sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; ++w) sm.sum += red[1][w];
-    lse[row] = sm.lse(inv_tau, scale);
+    lse[row] = sm.lse(inv_tau);
   }
   const int chunks = (int)((at_row.end + kStride - 1) / kStride);  // per thread
   if (best >= t0) active[atomicAdd(&nactive, 1u)] = tid;
@@ -701,7 +696,7 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
   float high = -INFINITY;
   for (int i = tid; i < a.k; i += NT) {
     int32_t j = a.index[row * a.k + i];
-    const float t = a.values[row * a.k + i] * inv_tau;
+    const float t = a.values[row * a.k + i];
     if ((uint32_t)j >= (uint32_t)a.vocab || t == -INFINITY) j = -1;
     at[i] = j;
     prob[i] = t;
@@ -720,15 +715,16 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
     }
     return;
   }
-  float L;
+  // log p = (t - base) / tau - L
+  float base = 0.0f, L;
   if (a.teacher_lse) {
     L = a.teacher_lse[row];
   } else {
-    high = block_max<NT>(high, red[0]);
+    base = block_max<NT>(high, red[0]);
     float z = 0.0f;
     for (int i = tid; i < a.k; i += NT)
-      if (at[i] >= 0) z += expf(prob[i] - high);
-    L = high + logf(block_sum<NT>(z, red[1]));
+      if (at[i] >= 0) z += expf((prob[i] - base) * inv_tau);
+    L = logf(block_sum<NT>(z, red[1]));
   }
   if (GRAD) {  // the first of the entries that share an index
     // waves take the earlier entries in turn, lanes the later ones
@@ -741,10 +737,13 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
     }
   }
 
-  // the student's softmax: q_j = exp2(s_j scale - r) / sum, or exp(s_j / tau - lse)
+  // The student's softmax: q_j = exp2((s_j - c) scale) / sum.  A saved lse is c = lse tau and
+  // a sum of 1, and costs q an error of |lse| 2^-24: beyond kFar the row is summed again.
+  constexpr float kFar = 1024.0f;
   Softmax sm;
-  float lse;
-  if (LOSS) {
+  float lse = LOSS ? 0.0f : a.lse[row];
+  const bool scan = LOSS || !(fabsf(lse) <= kFar);
+  if (scan) {
     auto unpack = [](const vec& v, float (&f)[VEC]) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[e] = (float)v[e];
@@ -763,7 +762,7 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
       for (int i = 0; i < NV; ++i) {
         unpack(held_at(i), f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sm.sum += __builtin_amdgcn_exp2f(__builtin_fmaf(f[e], scale, -sm.r));
+        for (int e = 0; e < VEC; ++e) sm.sum += __builtin_amdgcn_exp2f((f[e] - sm.c) * scale);
       }
     } else {
       uint32_t c = first;
@@ -784,30 +783,28 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
       sm.raise(block_max<NT>(sm.m, red[2]), scale);
     }
     sm.sum = block_sum<NT>(sm.sum, red[3]);
-    lse = sm.lse(inv_tau, scale);
-    if (tid == 0 && a.lse) a.lse[row] = lse;
+    if (LOSS && tid == 0 && a.lse) a.lse[row] = sm.lse(inv_tau);
   } else {
-    lse = a.lse[row];
+    sm.c = lse * a.tau;
+    sm.sum = 1.0f;
   }
-  const bool none = lse == -INFINITY;  // no student distribution: q = 0
-  const float unit = none ? 0.0f : LOSS ? 1.0f / sm.sum : 1.0f;
+  const bool none = sm.sum == 0.0f;  // all -inf, no student distribution: q = 0
+  const float unit = none ? 0.0f : 1.0f / sm.sum;
   // q before the division by the sum
-  const float shift = none ? 0.0f : lse;
-  auto part = [&](float f) {
-    return __builtin_amdgcn_exp2f(LOSS ? __builtin_fmaf(f, scale, -sm.r) : (f * inv_tau - shift) * kLog2e);
-  };
+  auto part = [&](float f) { return __builtin_amdgcn_exp2f((f - sm.c) * scale); };
 
   // teacher entries: probability, student logit, loss
   float loss = 0.0f, mass = 0.0f;
+  const float log_sum = logf(sm.sum);
   for (int i = tid; i < a.k; i += NT) {
     const int32_t j = at[i];
     float pr = 0.0f, st = 0.0f;
     if (j >= 0) {
-      const float logp = prob[i] - L;
+      const float logp = (prob[i] - base) * inv_tau - L;
       pr = expf(logp);
       st = (float)s[j];
-      const float logq = st == -INFINITY ? -INFINITY : st * inv_tau - lse;
-      if (pr != 0.0f) loss += pr * (logp - logq);
+      const float logq = st == -INFINITY ? -INFINITY : (st - sm.c) * inv_tau - log_sum;
+      if (LOSS && pr != 0.0f) loss += pr * (logp - logq);
     }
     prob[i] = pr;
     own[i] = st;
@@ -973,6 +970,9 @@ int top_launch(const void* logits, int64_t stride, int64_t rows, int64_t vocab, 
 }
 
 constexpr int64_t kMaxDim = 1 << 24;
+constexpr int64_t kMaxBlocks = (1LL << 32) / 256 - 1;  // a launch has fewer than 2^32 threads
+
+bool bad_temperature(float t) { return !(t >= FC_MIN_TEMPERATURE && t <= FC_MAX_TEMPERATURE); }
 
 }  // namespace
 
@@ -1003,6 +1003,7 @@ int fc_layer_norm(const void* x, int64_t x_stride, int dtype, const int32_t* til
                   const void* weight, int64_t weight_stride, const void* bias, int64_t bias_stride, float eps,
                   void* y, int64_t y_stride, float* mean, float* rstd, void* stream) {
   if (ntiles < 0 || dim <= 0 || dim > kMaxDim) return fc_internal_fail(-1, "bad sizes");
+  if (!(eps >= 0.0f)) return fc_internal_fail(-1, "bad eps");
   if (ntiles == 0) return 0;
   if (!x || !tiles || !y || !mean || !rstd) return fc_internal_fail(-1, "null pointer");
   NormArgs p = {};
@@ -1024,6 +1025,8 @@ int fc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
   if (ntiles < 0 || nclients <= 0 || dim <= 0 || dim > kMaxDim) return fc_internal_fail(-1, "bad sizes");
   const bool want = dweight || dbias;
   if (want && !first_tile) return fc_internal_fail(-1, "null pointer");
+  const int64_t columns = (dim + 63) / 64;  // blocks per client that join the gradients
+  if (want && nclients * columns > kMaxBlocks) return fc_internal_fail(-1, "bad sizes");
   hipStream_t s = (hipStream_t)stream;
   if (ntiles > 0) {
     if (!x || !dy || !tiles || !dx || !mean || !rstd || (want && !partials)) return fc_internal_fail(-1, "null pointer");
@@ -1040,8 +1043,8 @@ int fc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
     if (const int rc = norm_dtype(dtype, p, true, s)) return rc;
   }
   if (!want) return 0;
-  hipLaunchKernelGGL(k_norm_join, dim3((unsigned)nclients, (unsigned)((dim + 63) / 64), 2), dim3(256), 0, s,
-                     (const float*)partials, first_tile, (int32_t)dim, dweight, dweight_stride, dbias, dbias_stride,
+  hipLaunchKernelGGL(k_norm_join, dim3((unsigned)(nclients * columns), 2), dim3(256), 0, s, (const float*)partials,
+                     first_tile, (int32_t)dim, (int32_t)columns, dweight, dweight_stride, dbias, dbias_stride,
                      accumulate);
   return fc_internal_check_launch("k_norm_join");
 }
@@ -1050,7 +1053,7 @@ int fc_top_logits(const void* logits, int64_t stride, int dtype, int64_t rows, i
                   float temperature, int32_t* index, void* values, float* lse, void* stream) {
   if (rows < 0 || rows > 0x7fffffffLL || vocab <= 0 || vocab > 0x7fffffffLL - 65536) return fc_internal_fail(-1, "bad sizes");
   if (k <= 0 || k > vocab || k > FC_MAX_TOP) return fc_internal_fail(-1, "bad k");
-  if (!(temperature > 0.0f) || std::isinf(temperature)) return fc_internal_fail(-1, "bad temperature");
+  if (bad_temperature(temperature)) return fc_internal_fail(-1, "bad temperature");
   if (rows == 0) return 0;
   if (!logits || !index || !values || !lse) return fc_internal_fail(-1, "null pointer");
   const float inv_tau = 1.0f / temperature;
@@ -1070,7 +1073,7 @@ int fc_distill(const void* logits, int64_t stride, int dtype, int64_t rows, int6
   if (rows < 0 || rows > 0x7fffffffLL || nclients <= 0 || vocab <= 0 || vocab > 0x7fffffffLL - 65536)
     return fc_internal_fail(-1, "bad sizes");
   if (k <= 0 || k > kDistillMax) return fc_internal_fail(-1, "bad k");
-  if (!(temperature > 0.0f) || std::isinf(temperature)) return fc_internal_fail(-1, "bad temperature");
+  if (bad_temperature(temperature)) return fc_internal_fail(-1, "bad temperature");
   if (!offsets || (!loss && !grad) || (!loss && rows && !lse) || (loss && rows && !row_loss))
     return fc_internal_fail(-1, "null pointer");
   if (loss && dloss) return fc_internal_fail(-1, "dloss goes with the gradient alone");

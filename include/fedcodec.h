@@ -433,7 +433,8 @@ int fc_quantize_floor(const float* const* xs, int32_t nclients, int64_t P, float
  * with a client stride (0: one weight for all clients), gradients of weights
  * float32 with a client stride (views of the clients' float32[P] rows).  Strides
  * count elements; a pointer needs its type's own alignment only.  Rows no tile
- * names are neither read nor written.
+ * names are neither read nor written.  An output shares no memory with an input but
+ * where this says so, or where it is the residual or the pre-activation itself.
  * ------------------------------------------------------------------------- */
 
 /* Types of activations and weights. */
@@ -449,6 +450,10 @@ int fc_quantize_floor(const float* const* xs, int32_t nclients, int64_t P, float
 
 #define FC_MAX_TOP 1024 /* top logits of a row */
 
+/* Temperatures: T, 1 / T and T^2 are float32 numbers well inside its range. */
+#define FC_MIN_TEMPERATURE 1e-15f
+#define FC_MAX_TEMPERATURE 1e15f
+
 /* HOST: the row-tile table of a batch whose client c has counts[c] rows, in client
  * order: per tile int32 {client, first row, rows, 0} with at most tile_rows rows, and
  * first_tile[nclients + 1] (both nullable: the count alone).  Returns the number of
@@ -456,7 +461,8 @@ int fc_quantize_floor(const float* const* xs, int32_t nclients, int64_t P, float
 int64_t fc_client_tiles(const int64_t* counts, int32_t nclients, int32_t tile_rows, int32_t* tiles,
                         int32_t* first_tile);
 
-/* y = (x - mean) rstd weight_c + bias_c; weight, bias nullable.  tiles of 16 rows. */
+/* y = (x - mean) rstd weight_c + bias_c; weight, bias nullable; eps >= 0.  tiles of at
+ * most 16 rows keep the chip busy. */
 int fc_layer_norm(const void* x, int64_t x_stride, int dtype, const int32_t* tiles, int32_t ntiles, int64_t dim,
                   const void* weight, int64_t weight_stride, const void* bias, int64_t bias_stride, float eps,
                   void* y, int64_t y_stride, float* mean, float* rstd, void* stream);

@@ -156,3 +156,41 @@ def test_pack_rows_refusals():
   refused(pack(src=NULL), b"null")
   refused(pack(dtype=5), b"dtype")
   assert pack(rows=0) == 0
+
+
+def test_limits_of_scalars_and_sizes():
+  lib, b = _lib.load(), _buf()
+  for t in (1e-16, 1e16, 1e-40):
+    refused(lib.fc_top_logits(b, 8, 0, 1, 8, 2, t, b, b, b, None), b"temperature")
+  for eps in (-1e-5, float("nan")):
+    refused(lib.fc_layer_norm(b, 4, 0, b, 1, 4, b, 4, b, 4, eps, b, 4, b, b, None), b"eps")
+  # the gradients' join: clients x columns in one launch of fewer than 2^32 threads
+  refused(lib.fc_layer_norm_backward(b, 4, b, 4, 0, b, b, b, 0, b, 1 << 20, 4096, b, 4, NULL, 0, b, 4, b, 4, b, 4, 0, b,
+                                     None), b"sizes")
+  refused(lib.fc_linear(b, 8, 1, b, 1, 128, 1, 1 << 31, 8, b, 64, 8, NULL, 0, 0, NULL, 0, NULL, 0, b, 8, 1, NULL, 0,
+                        None), b"sizes")
+  refused(lib.fc_linear_backward_weight(b, 8, b, 8, 1, b, 1 << 24, 8, 8, b, 64, 8, NULL, 0, 0, 128, 1, NULL, 0, None),
+          b"too many tiles")
+  refused(lib.fc_pack_rows(b, 8, 8, 1, 1 << 30, 1 << 20, 8, b - b % 16, 8, None), b"too many rows")
+
+
+def test_memory_that_two_tensors_share():
+  import torch
+  from federated_amd import client_ops as ops
+  buf = torch.zeros(10, 100)
+  left, right, mid = buf[:, :50], buf[:, 50:], buf[:, 40:60]
+  ops._apart("out", left, x=right)
+  ops._apart("out", right, x=left, y=None)
+  ops._apart("out", buf[:5], x=buf[5:])
+  ops._apart("out", left, itself=left, x=right)
+  ops._apart("out", buf[3:4, 20:30], x=left[:3], y=left[4:])
+  ops._apart("out", buf[:0], x=buf)
+  ops._apart("out", torch.zeros(1, 8).as_strided((1, 8), (0, 1)), x=buf)
+  whole = buf[:, :99].unflatten(1, (9, 11))
+  ops._apart("dweight", whole, dbias=buf[:, 99:])
+  for out, x in [(left, mid), (mid, left), (right, mid), (buf, right), (left, left), (left[:1], buf), (whole, buf[:, 98:]),
+                 (left, buf.view(-1)[:50].expand(10, 50))]:
+    with pytest.raises(ValueError):
+      ops._apart("out", out, x=x)
+  with pytest.raises(ValueError):
+    ops._apart("out", left, itself=mid)

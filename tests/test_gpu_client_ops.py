@@ -805,3 +805,266 @@ def test_operator_refusals(gpu):
     with pytest.raises(ValueError):
       call()
       pytest.fail("call %d was not refused" % i)
+
+
+# --- limits: launch shapes, lowest values, wide strides, many clients, shared memory --------
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("vocab", [1021, 1029, 2043, 4093, 5115, 10237, 16381, 20477, 32765, 65531, 65541])
+def test_distillation_every_launch_shape(gpu, dtype, vocab):
+  rng = np.random.default_rng(vocab)
+  logits = rand(rng, (3, vocab), dtype, 2.0)
+  index, values = teacher_rows(rng, 3, vocab, 5)
+  check_distill(logits, index, values, [2, 1], tau=1.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("vocab,k", [(4096, 32), (4097, 32), (2048, 33), (2049, 33), (513, 200), (32768, 128), (32769, 128),
+                                     (32768, 129), (32771, 5), (70001, 1024)])
+def test_top_logits_every_launch_shape(gpu, dtype, vocab, k):
+  check_top(rand(np.random.default_rng(vocab + k), (3, vocab), dtype, 2.0), k, 1.3)
+
+
+@pytest.mark.parametrize("tau", [0.5, 1.0, 3.0])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("vocab", [96, 3001, 70001])
+def test_rows_of_the_lowest_value(gpu, dtype, tau, vocab):
+  """A mask of the type's lowest value over a whole row leaves a uniform softmax, over most
+  of it one over the rest; a teacher whose values are all the lowest is uniform too.  A
+  gradient is w tau (q - p): q by an exponential, a sum of vocab / 64 + 24 terms and a
+  division, p by an exponential of a logarithm of 4."""
+  low = torch.finfo(dtype).min
+  logits = torch.full((3, vocab), low, dtype=dtype, device=gpu)
+  logits[1, 7:11] = 0.0
+  batch = ops.ClientBatch([2, 1])
+  index = torch.tensor([[1, 8, 60, 95]] * 3, dtype=torch.int32, device=gpu)
+  values = torch.zeros(3, 4, device=gpu)
+  values[2] = torch.finfo(torch.float32).min
+  q = torch.full((3, vocab), 1.0 / vocab, dtype=torch.float64)
+  q[1] = 0.0
+  q[1, 7:11] = 0.25
+  grad = q.clone()
+  grad[:, index[0].long().cpu()] -= 0.25
+  w = torch.tensor([0.5, 0.5, 1.0], dtype=torch.float64)[:, None]
+  grad = grad * w * tau
+  tol = ((vocab / 64 + 24) * U32 * (q + 0.25) + 16 * U32) * tau + unit(dtype) * grad.abs() + tiny(dtype)
+  loss, got = ops.distillation_with_gradient(logits, index, values, batch, temperature=tau)
+  check(got, grad, tol, "gradient")
+  loss2, lse = ops.distillation(logits, index, values, batch, temperature=tau)
+  check(ops.distillation_backward(logits, lse, index, values, batch, temperature=tau), grad, tol, "gradient alone")
+  assert torch.equal(loss, loss2)
+  row = math.log(vocab / 4)  # of rows 0 and 2: p log(p / q)
+  e = (vocab / 64 + 64) * U32 * tau * tau * (row + 2)
+  check(loss[1:], torch.tensor([tau * tau * row]), e, "loss")
+  top, _, top_lse = ops.top_logits(logits, 4, tau)
+  assert top[0].tolist() == [0, 1, 2, 3] and top[1].tolist() == [7, 8, 9, 10]
+  assert abs(float(top_lse[1]) - math.log(4)) < 8 * U32
+
+
+@pytest.mark.parametrize("vocab", [301, 40001])
+def test_distillation_far_from_zero(gpu, vocab):
+  """Logits around 3000: a saved lse holds q to 3000 u only, the softmax itself to the
+  roundings of the differences (below 16) and of the sum (vocab / 64 + 24 terms)."""
+  rng = np.random.default_rng(9)
+  batch = ops.ClientBatch([2, 1])
+  logits = rand(rng, (3, vocab), torch.float32) + 3000.0
+  index, values = teacher_rows(rng, 3, vocab, 4, pad=0)
+  weights = torch.tensor([0.5, 0.5, 1.0], dtype=torch.float64)
+  q, p = torch.softmax(logits.double().cpu(), 1), torch.softmax(values.double().cpu(), 1)
+  want = weights[:, None] * q.scatter_add(1, index.long().cpu(), -p)
+  tol = (2 * 16 + vocab / 64 + 24 + 16) * 2 * U32 * (q + want.abs() + p.sum(1, keepdim=True) * (want < 0))
+  _, lse = ops.distillation(logits, index, values, batch)
+  check(ops.distillation_with_gradient(logits, index, values, batch)[1], want, tol, "gradient")
+  check(ops.distillation_backward(logits, lse, index, values, batch), want, tol, "gradient alone")
+
+
+def far_rows(rows, width, stride, dtype, rng, scale=1.0):
+  """[rows, width] at a row stride such that the last row lies past 2^31 elements."""
+  assert (rows - 1) * stride > 2**31
+  t = torch.empty((rows - 1) * stride + width, dtype=dtype, device="cuda").as_strided((rows, width), (stride, 1))
+  t.copy_(rand(rng, (rows, width), dtype, scale))
+  return t
+
+
+@pytest.mark.parametrize("odd", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_offsets_past_32_bits(gpu, dtype, odd):
+  rng = np.random.default_rng(odd)
+  stride, u = 2**30 + 2 + odd, unit(dtype)
+  x = far_rows(4, 300, stride, dtype, rng)
+  check_top(x, 5)
+  index, values = teacher_rows(rng, 4, 300, 5)
+  batch = ops.ClientBatch([1, 3])
+  loss, grad, el, eg = distill_reference(x, index, values, [1, 3], 1.0)
+  far = torch.empty_strided((4, 300), (stride, 1), dtype=dtype, device=gpu)
+  got, lse = ops.distillation(x, index, values, batch)
+  check(got, loss, el, "loss")
+  eg = eg + u * (grad.abs() + eg) + tiny(dtype)
+  check(ops.distillation_with_gradient(x, index, values, batch, out=far)[1], grad, eg, "gradient")
+  check(ops.distillation_backward(x, lse, index, values, batch, out=far), grad, eg, "gradient alone")
+  del far
+  y, mean, rstd = ops.layer_norm(x, None, None, batch)
+  ref = norm_reference(x, None, None, [1, 3], 1e-5)
+  check(y, ref["y"], norm_tolerances(ref, x, None, 300, dtype)["y"], "norm")
+  dx, _, _ = ops.layer_norm_backward(x, x, mean, rstd, None, batch)
+  near = ops.layer_norm_backward(x.contiguous(), x.contiguous(), mean, rstd, None, batch)[0]
+  assert torch.equal(dx, near)
+  # clients' weights that far apart, activations too, and gradients written there
+  many = ops.ClientBatch([1, 0, 2, 1])
+  flat = far_rows(4, 70 * 300, stride, dtype, rng, 1 / math.sqrt(300))
+  w = flat.unflatten(1, (70, 300))
+  wide = torch.empty(3 * stride + 70, dtype=dtype, device=gpu).as_strided((4, 70), (stride, 1))
+  ops.linear(x, w, None, many, out=wide)
+  want, e = linear_reference(x, w, [1, 0, 2, 1])
+  check(wide, want, e + u * (want.abs() + e) + tiny(dtype), "linear")
+  back = ops.linear_backward_input(wide, w, many)
+  want, e = linear_reference(wide, w.double().cpu().transpose(1, 2), [1, 0, 2, 1])
+  check(back, want, e + u * (want.abs() + e) + tiny(dtype), "input gradient")
+  del flat, w
+  rows = torch.empty(3 * stride + 70 * 301, device=gpu).as_strided((4, 70 * 301), (stride, 1))
+  dw, db = ops.linear_backward_weight(wide, x, many, dweight=rows[:, :70 * 300].unflatten(1, (70, 300)),
+                                      dbias=rows[:, 70 * 300:])
+  for c, (lo, hi) in enumerate(spans([1, 0, 2, 1])):
+    d, xx = wide[lo:hi].double().cpu(), x[lo:hi].double().cpu()
+    check(dw[c], d.t() @ xx, 2 * max(1, hi - lo) * U32 * (d.abs().t() @ xx.abs()), "dw")
+    check(db[c], d.sum(0), 2 * max(1, hi - lo) * U32 * d.abs().sum(0), "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("k,m", [(1, 3), (3, 1), (7, 5), (40, 33)])
+def test_linear_rows_that_overlap(gpu, dtype, k, m):
+  """One row of activations for all (stride 0), and windows one element apart."""
+  rng = np.random.default_rng(k)
+  counts = [200, 0, 70]
+  batch = ops.ClientBatch(counts)
+  w = rand(rng, (3, m, k), dtype, 1 / math.sqrt(k))
+  for x, dz in [(rand(rng, (1, k), dtype).expand(270, k), rand(rng, (1, m), dtype).expand(270, m)),
+                (rand(rng, (269 + k,), dtype).as_strided((270, k), (1, 1)),
+                 rand(rng, (269 + m,), dtype).as_strided((270, m), (1, 1)))]:
+    want, e = linear_reference(x, w, counts)
+    check(ops.linear(x, w, None, batch), want, e + unit(dtype) * (want.abs() + e) + tiny(dtype), "y")
+    dw, db = ops.linear_backward_weight(dz, x, batch)
+    for c, (lo, hi) in enumerate(spans(counts)):
+      d, xx = dz[lo:hi].double().cpu(), x[lo:hi].double().cpu()
+      check(dw[c], d.t() @ xx, 2 * max(1, hi - lo) * U32 * (d.abs().t() @ xx.abs()), "dw")
+      check(db[c], d.sum(0), 2 * max(1, hi - lo) * U32 * d.abs().sum(0), "db")
+
+
+@pytest.mark.parametrize("rows,splits", [(32, 5), (128, 3), (256, 2)])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_odd_widths_with_rows_behind(gpu, monkeypatch, dtype, rows, splits):
+  plan = (1.0, 128 if rows == 256 and dtype == torch.float32 else rows, splits)
+  monkeypatch.setattr(ops, "_estimate", lambda *a: plan if a[4] else (9.0, min(plan[1], 128), splits))
+  check_linear(gpu, np.random.default_rng(rows), [70, 0, 129], 257, 131, dtype, "gelu", behind=5)
+  check_linear(gpu, np.random.default_rng(splits), [70, 0, 129], 130, 262, dtype, None, shared=True, behind=300)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_many_clients(gpu, dtype):
+  """More clients than a grid's second axis holds; every other one without rows."""
+  rng = np.random.default_rng(3)
+  n, k, m, u = 70001, 5, 3, unit(dtype)
+  counts = np.arange(n) % 2
+  rows = int(counts.sum())
+  batch = ops.ClientBatch(counts)
+  x, dz = rand(rng, (rows, k), dtype), rand(rng, (rows, m), dtype)
+  flat = rand(rng, (n, m * k), dtype)
+  w = flat.unflatten(1, (m, k))
+  mine = w[1::2].double()
+  y = ops.linear(x, w, None, batch)
+  want = (mine * x.double()[:, None]).sum(2)
+  e = 2 * k * U32 * (mine * x.double()[:, None]).abs().sum(2)
+  check(y, want, (e + u * (want.abs() + e) + tiny(dtype)).cpu(), "y")
+  dx = ops.linear_backward_input(dz, w, batch)
+  want = (mine * dz.double()[:, :, None]).sum(1)
+  e = 2 * m * U32 * (mine * dz.double()[:, :, None]).abs().sum(1)
+  check(dx, want, (e + u * (want.abs() + e) + tiny(dtype)).cpu(), "dx")
+  dw, db = ops.linear_backward_weight(dz, x, batch)
+  outer = dz.double()[:, :, None] * x.double()[:, None]
+  check(dw[1::2], outer, (2 * U32 * outer.abs()).cpu(), "dw")
+  assert (dw[::2] == 0).all() and (db[::2] == 0).all() and torch.equal(db[1::2], dz.float())
+  _, mean, rstd = ops.layer_norm(x, None, None, batch)
+  _, gw, gb = ops.layer_norm_backward(dx, x, mean, rstd, None, batch)
+  assert (gw[::2] == 0).all() and torch.equal(gb[1::2], dx.float())
+  index = torch.zeros(rows, 1, dtype=torch.int32, device=gpu)
+  loss, _ = ops.distillation_with_gradient(x, index, torch.zeros(rows, 1, device=gpu), batch)
+  want = torch.logsumexp(x.double(), 1) - x.double()[:, 0]
+  check(loss[1::2], want, 64 * U32 * (1 + x.double().abs().amax(1)).cpu(), "loss")
+  assert (loss[::2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_outputs_beside_and_over_their_inputs(gpu, dtype):
+  """Columns of one buffer as inputs and outputs, an output over the residual; an output
+  over anything else is refused before it is written."""
+  rng = np.random.default_rng(5)
+  counts = [30, 3]
+  batch = ops.ClientBatch(counts)
+  buf = rand(rng, (33, 160), dtype)
+  x, out, res = buf[:, :64], buf[:, 64:128], buf[:, 128:]
+  w = rand(rng, (2, 64, 64), dtype, 0.1)
+  want = ops.linear(x.clone(), w, None, batch)
+  assert torch.equal(ops.linear(x, w, None, batch, out=out), want)
+  down = rand(rng, (2, 32, 64), dtype, 0.1)
+  want = ops.linear(x.clone(), down, None, batch, residual=res.clone())
+  assert torch.equal(ops.linear(x, down, None, batch, residual=res, out=res), want)
+  y, mean, rstd = ops.layer_norm(x, None, None, batch)
+  want = ops.layer_norm_backward(y, x, mean, rstd, None, batch, residual=out.clone())[0]
+  assert torch.equal(ops.layer_norm_backward(y, x, mean, rstd, None, batch, residual=out, out=out)[0], want)
+  before, w0 = buf.clone(), w.clone()
+  index, values = torch.zeros(33, 2, dtype=torch.int32, device=gpu), torch.zeros(33, 2, device=gpu)
+  grads = torch.zeros(2, 64 * 65, device=gpu)
+  calls = [
+      lambda: ops.linear(x, w, None, batch, out=x),
+      lambda: ops.linear(x, w, None, batch, out=buf[:, 32:96]),
+      lambda: ops.linear(x, w, None, batch, residual=buf[:, 65:129], out=out),
+      lambda: ops.linear(x, w, None, batch, out=w.view(-1)[:33 * 64].view(33, 64)),
+      lambda: ops.linear_backward_input(x, w, batch, out=x),
+      lambda: ops.layer_norm(x, None, None, batch, out=x),
+      lambda: ops.layer_norm_backward(y, x, mean, rstd, None, batch, out=y),
+      lambda: ops.layer_norm_backward(y, x, mean, rstd, None, batch, out=x),
+      lambda: ops.layer_norm_backward(y, x, mean, rstd, None, batch, dweight=grads[:, :64], dbias=grads[:, 1:65]),
+      lambda: ops.linear_backward_weight(x, x, batch, dweight=grads[:, :4096].unflatten(1, (64, 64)),
+                                         dbias=grads[:, 4095:4159]),
+      lambda: ops.distillation_with_gradient(x, index, values, batch, out=buf[:, 1:65]),
+      lambda: ops.layer_norm(x, None, None, batch, eps=-1e-5),
+      lambda: ops.top_logits(x, 2, temperature=1e-16),
+      lambda: ops.top_logits(x, 2, temperature=1e16),
+  ]
+  for i, call in enumerate(calls):
+    with pytest.raises(ValueError):
+      call()
+      pytest.fail("call %d was not refused" % i)
+  assert torch.equal(buf, before) and torch.equal(w, w0)
+
+
+def test_two_streams_at_once_and_a_batch_that_ends(gpu):
+  """The same weights on two streams at a time, with a batch each that is dropped while its
+  kernels may still run."""
+  rng = np.random.default_rng(6)
+  counts = [700, 0, 300]
+  x, dz = rand(rng, (1000, 520), torch.bfloat16), rand(rng, (1000, 515), torch.bfloat16)
+  w = rand(rng, (3, 515, 520), torch.bfloat16, 0.05)
+
+  def run():
+    batch = ops.ClientBatch(counts)
+    y = ops.linear(x, w, None, batch, activation="gelu")
+    return [y, ops.linear_backward_input(dz, w, batch), *ops.linear_backward_weight(dz, x, batch)]
+
+  want = run()
+  torch.cuda.synchronize()
+  streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+  batches, outs = [ops.ClientBatch(counts) for _ in streams], []
+  for s, batch in zip(streams, batches):
+    with torch.cuda.stream(s):
+      y = ops.linear(x, w, None, batch, activation="gelu")
+      outs.append([y, ops.linear_backward_input(dz, w, batch), *ops.linear_backward_weight(dz, x, batch)])
+  del batches, batch
+  filler = [torch.full((1 << 16,), 7, dtype=torch.int32, device=gpu) for _ in range(64)]
+  for s in streams:
+    s.synchronize()
+  for out in outs:
+    for a, b in zip(out, want):
+      assert torch.equal(a, b)
+  del filler
