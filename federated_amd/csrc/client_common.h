@@ -46,14 +46,60 @@ __device__ __forceinline__ typename VecOf<T, N>::type load_vec(const T* p, int64
   return v;
 }
 
+// A part vector leaves in pieces of 8, 4 and 2 bytes: three stores instead of up to seven.
 template <typename T, int N = Elem<T>::kVec>
 __device__ __forceinline__ void store_vec(T* p, typename VecOf<T, N>::type v, int64_t valid) {
   if (valid >= N) {
     *(typename VecOf<T, N>::loose*)p = v;
+  } else if (valid > 0) {
+    const int left = (int)valid;
+    if constexpr (N >= 8)
+      if (left & 4) {
+        *(typename VecOf<T, 4>::loose*)p = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+        v = __builtin_shufflevector(v, v, 4, 5, 6, 7, 4, 5, 6, 7);
+        p += 4;
+      }
+    if constexpr (N >= 4)
+      if (left & 2) {
+        *(typename VecOf<T, 2>::loose*)p = __builtin_shufflevector(v, v, 0, 1);
+        v[0] = v[2];
+        p += 2;
+      }
+    if (left & 1) *p = v[0];
+  }
+}
+
+// Columns [c, c + N) of a row of `dim` >= N: read as the last N where they go past its end,
+// with no branch, and put right by settle() where they are used (a wait for the load).
+template <typename T, int N>
+__device__ __forceinline__ typename VecOf<T, N>::type load_columns(const T* row, int c, int dim) {
+  return *(const typename VecOf<T, N>::loose*)(row + min(c, dim - N));
+}
+
+// Those columns, zeros behind the row's end.
+template <typename T, int N>
+__device__ __forceinline__ typename VecOf<T, N>::type settle(typename VecOf<T, N>::type v, int c, int dim) {
+  const int over = c - (dim - N);
+  if (over <= 0) return v;
+  const int bits = min(over, N) * 8 * (int)sizeof(T);
+  if constexpr (N == 1) {
+    return v;  // its one column past the end: not asked for
+  } else if constexpr (N * sizeof(T) == 8) {
+    const uint64_t q = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(typename VecOf<T, N>::type, bits >= 64 ? 0 : q >> bits);
   } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (e < valid) p[e] = v[e];
+    typedef uint64_t pair __attribute__((ext_vector_type(2)));
+    pair q = __builtin_bit_cast(pair, v);
+    if (bits >= 128) {
+      q.x = q.y = 0;
+    } else if (bits >= 64) {
+      q.x = q.y >> (bits - 64);
+      q.y = 0;
+    } else {
+      q.x = q.x >> bits | q.y << (64 - bits);
+      q.y >>= bits;
+    }
+    return __builtin_bit_cast(typename VecOf<T, N>::type, q);
   }
 }
 

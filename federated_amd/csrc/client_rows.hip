@@ -55,28 +55,31 @@ struct NormArgs {
 };
 
 // TPR threads per row, NV vectors of VEC elements per thread: the row stays in registers, the next
-// row's are on their way while this one is summed, and the client's weights stay too.
+// row's are on their way while this one is summed, and the client's weights stay too.  Bound
+// by memory: one read and one write (backward: two and one).  A row's last vector is read
+// where it ends, so that no lane goes element by element (2500 bfloat16 elements, backward:
+// 564 us with such a tail, 321 without).
 template <typename T, int TPR, int NV, int VEC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm(const NormArgs p) {
   constexpr int G = TPR > 256 ? 1 : 256 / TPR;
   typedef typename VecOf<T, VEC>::type vec;
-  __shared__ float slots[2][2 * 8];
+  __shared__ float slots[2][2 * (TPR > 64 ? TPR / 64 : 1)];
   const RowTile t = p.tiles[blockIdx.x];
   const int lane = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const float inv = 1.0f / (float)p.dim;
   vec gw[NV], gb[NV], next[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + lane) * VEC, left = p.dim - c;
+    const int c = (i * TPR + lane) * VEC;
     gw[i] = gb[i] = vec{};
     if (p.weight) {
-      gw[i] = load_vec<T, VEC>((const T*)p.weight + t.client * p.ld_w + c, left);
+      gw[i] = settle<T, VEC>(load_columns<T, VEC>((const T*)p.weight + t.client * p.ld_w, c, p.dim), c, p.dim);
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) gw[i][e] = (T)1.0f;
     }
-    if (p.bias) gb[i] = load_vec<T, VEC>((const T*)p.bias + t.client * p.ld_b + c, left);
-    next[i] = load_vec<T, VEC>((const T*)p.x + (t.begin + min(g, t.rows - 1)) * p.ld_x + c, left);
+    if (p.bias) gb[i] = settle<T, VEC>(load_columns<T, VEC>((const T*)p.bias + t.client * p.ld_b, c, p.dim), c, p.dim);
+    next[i] = load_columns<T, VEC>((const T*)p.x + (t.begin + min(g, t.rows - 1)) * p.ld_x, c, p.dim);
   }
   // every group walks the same number of rows: barriers are uniform
   for (int r = 0; r < t.rows; r += G) {
@@ -85,14 +88,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm(const NormArgs p
     vec v[NV];
     float f[1] = {0.0f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = next[i];
+    for (int i = 0; i < NV; ++i) v[i] = settle<T, VEC>(next[i], (i * TPR + lane) * VEC, p.dim);
     if (r + G < t.rows) {
       const T* x = (const T*)p.x + (t.begin + min(r + G + g, t.rows - 1)) * p.ld_x;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + lane) * VEC;
-        next[i] = load_vec<T, VEC>(x + c, p.dim - c);
-      }
+      for (int i = 0; i < NV; ++i) next[i] = load_columns<T, VEC>(x, (i * TPR + lane) * VEC, p.dim);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -132,7 +132,7 @@ template <typename T, int TPR, int NV, int VEC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(const NormArgs p) {
   constexpr int G = TPR > 256 ? 1 : 256 / TPR;
   typedef typename VecOf<T, VEC>::type vec;
-  __shared__ float slots[2][2 * 8];
+  __shared__ float slots[2][2 * (TPR > 64 ? TPR / 64 : 1)];
   __shared__ float join[G > 1 ? TPR * VEC * NV : 1];
   const RowTile t = p.tiles[blockIdx.x];
   const int lane = threadIdx.x % TPR, g = threadIdx.x / TPR;
@@ -140,24 +140,22 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(const N
   float dg[NV][VEC] = {}, db[NV][VEC] = {};
   vec gw[NV], nx[NV], nd[NV];
   float nmu, ns;
-  // Row r of this group; a group past the tile's rows reads zeros, and adds none.
   auto fetch = [&](int r) {
     const int64_t row = t.begin + min(r + g, t.rows - 1);
-    const bool live = r + g < t.rows;
     nmu = p.mean[row];
     ns = p.rstd[row];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC, left = live ? p.dim - c : 0;
-      nx[i] = load_vec<T, VEC>((const T*)p.x + row * p.ld_x + c, left);
-      nd[i] = load_vec<T, VEC>((const T*)p.dy + row * p.ld_dy + c, left);
+      const int c = (i * TPR + lane) * VEC;
+      nx[i] = load_columns<T, VEC>((const T*)p.x + row * p.ld_x, c, p.dim);
+      nd[i] = load_columns<T, VEC>((const T*)p.dy + row * p.ld_dy, c, p.dim);
     }
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + lane) * VEC;
     if (p.weight) {
-      gw[i] = load_vec<T, VEC>((const T*)p.weight + t.client * p.ld_w + c, p.dim - c);
+      gw[i] = settle<T, VEC>(load_columns<T, VEC>((const T*)p.weight + t.client * p.ld_w, c, p.dim), c, p.dim);
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) gw[i][e] = (T)(c + e < p.dim ? 1.0f : 0.0f);
@@ -172,8 +170,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(const N
     vec vx[NV], vd[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      vx[i] = nx[i];
-      vd[i] = nd[i];
+      const int c = (i * TPR + lane) * VEC;
+      // a group past the tile's rows adds zeros
+      vx[i] = live ? settle<T, VEC>(nx[i], c, p.dim) : vec{};
+      vd[i] = live ? settle<T, VEC>(nd[i], c, p.dim) : vec{};
     }
     if (r + G < t.rows) fetch(r + G);
     float f[2] = {0.0f, 0.0f};
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(const N
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
       vec res = {};
-      if (p.residual) res = load_vec<T, VEC>((const T*)p.residual + row * p.ld_res + c, p.dim - c);
+      if (p.residual) res = settle<T, VEC>(load_columns<T, VEC>((const T*)p.residual + row * p.ld_res, c, p.dim), c, p.dim);
       vec o;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -238,79 +238,128 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(const N
   }
 }
 
-// Rows longer than the registers of a block hold: the row is read once per sum.
-template <typename T>
-__global__ __launch_bounds__(256) void k_norm_long(const NormArgs p) {
-  __shared__ float slots[2][2 * 4];
+// Rows longer than the registers of a block hold (the row is read once per sum), and rows
+// shorter than a vector (N 1).
+template <typename T, int NT, int N>
+__global__ __launch_bounds__(NT) void k_norm_long(const NormArgs p) {
+  typedef typename VecOf<T, N>::type vec;
+  __shared__ float slots[2][2 * NT / 64];
   const RowTile t = p.tiles[blockIdx.x];
+  const int first = threadIdx.x * N;
   const float inv = 1.0f / (float)p.dim;
   const T* w = (const T*)p.weight + t.client * p.ld_w;
   const T* b = (const T*)p.bias + t.client * p.ld_b;
+  auto read = [&](const T* row, int c) { return settle<T, N>(load_columns<T, N>(row, c, p.dim), c, p.dim); };
   for (int r = 0; r < t.rows; ++r) {
     const int64_t row = t.begin + r;
     const T* x = (const T*)p.x + row * p.ld_x;
     float f[1] = {0.0f};
-    for (int c = threadIdx.x; c < p.dim; c += 256) f[0] += (float)x[c];
-    group_sum<256>(f, slots[0]);
+#pragma unroll 4
+    for (int c = first; c < p.dim; c += NT * N) {
+      const vec v = read(x, c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[0] += (float)v[e];
+    }
+    group_sum<NT>(f, slots[0]);
     const float mu = f[0] * inv;
     f[0] = 0.0f;
-    for (int c = threadIdx.x; c < p.dim; c += 256) {
-      const float d = (float)x[c] - mu;
-      f[0] += d * d;
+#pragma unroll 4
+    for (int c = first; c < p.dim; c += NT * N) {
+      const vec v = read(x, c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float d = (float)v[e] - mu;
+        f[0] += c + e < p.dim ? d * d : 0.0f;
+      }
     }
-    group_sum<256>(f, slots[1]);
+    group_sum<NT>(f, slots[1]);
     const float s = 1.0f / sqrtf(f[0] * inv + p.eps);
     if (threadIdx.x == 0) {
       p.mean[row] = mu;
       p.rstd[row] = s;
     }
     T* o = (T*)p.out + row * p.ld_out;
-    for (int c = threadIdx.x; c < p.dim; c += 256) {
-      float y = ((float)x[c] - mu) * s;
-      if (p.weight) y *= (float)w[c];
-      if (p.bias) y += (float)b[c];
-      o[c] = (T)y;
+#pragma unroll 2
+    for (int c = first; c < p.dim; c += NT * N) {
+      vec v = read(x, c), gw = {}, gb = {};
+      if (p.weight) gw = read(w, c);
+      if (p.bias) gb = read(b, c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        float y = ((float)v[e] - mu) * s;
+        if (p.weight) y *= (float)gw[e];
+        v[e] = (T)(y + (float)gb[e]);
+      }
+      store_vec<T, N>(o + c, v, p.dim - c);
     }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_norm_backward_long(const NormArgs p) {
-  __shared__ float slots[2][2 * 4];
+template <typename T, int NT, int N>
+__global__ __launch_bounds__(NT) void k_norm_backward_long(const NormArgs p) {
+  typedef typename VecOf<T, N>::type vec;
+  __shared__ float slots[2][2 * NT / 64];
   const RowTile t = p.tiles[blockIdx.x];
+  const int first = threadIdx.x * N;
   const float inv = 1.0f / (float)p.dim;
   const T* w = (const T*)p.weight + t.client * p.ld_w;
+  auto read = [&](const T* row, int c) { return settle<T, N>(load_columns<T, N>(row, c, p.dim), c, p.dim); };
   for (int r = 0; r < t.rows; ++r) {
     const int64_t row = t.begin + r;
     const T* x = (const T*)p.x + row * p.ld_x;
     const T* dy = (const T*)p.dy + row * p.ld_dy;
     const float mu = p.mean[row], s = p.rstd[row];
     float f[2] = {0.0f, 0.0f};
-    for (int c = threadIdx.x; c < p.dim; c += 256) {
-      const float a = (float)dy[c] * (p.weight ? (float)w[c] : 1.0f);
-      f[0] += a;
-      f[1] += a * ((float)x[c] - mu) * s;
+#pragma unroll 2
+    for (int c = first; c < p.dim; c += NT * N) {
+      const vec vx = read(x, c), vd = read(dy, c);
+      vec gw = {};
+      if (p.weight) gw = read(w, c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float a = p.weight ? (float)vd[e] * (float)gw[e] : (float)vd[e];
+        f[0] += a;
+        f[1] += c + e < p.dim ? a * ((float)vx[e] - mu) * s : 0.0f;
+      }
     }
-    group_sum<256>(f, slots[r & 1]);
+    group_sum<NT>(f, slots[r & 1]);
     const float m0 = f[0] * inv, m1 = f[1] * inv;
-    for (int c = threadIdx.x; c < p.dim; c += 256) {
-      const float a = (float)dy[c] * (p.weight ? (float)w[c] : 1.0f);
-      float v = s * (a - m0 - ((float)x[c] - mu) * s * m1);
-      if (p.residual) v += (float)((const T*)p.residual)[row * p.ld_res + c];
-      ((T*)p.out)[row * p.ld_out + c] = (T)v;
+#pragma unroll 2
+    for (int c = first; c < p.dim; c += NT * N) {
+      const vec vx = read(x, c), vd = read(dy, c);
+      vec gw = {}, res = {};
+      if (p.weight) gw = read(w, c);
+      if (p.residual) res = read((const T*)p.residual + row * p.ld_res, c);
+      vec o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float a = p.weight ? (float)vd[e] * (float)gw[e] : (float)vd[e];
+        o[e] = (T)(s * (a - m0 - ((float)vx[e] - mu) * s * m1) + (float)res[e]);
+      }
+      store_vec<T, N>((T*)p.out + row * p.ld_out + c, o, p.dim - c);
     }
   }
   if (!p.part) return;
-  for (int c = threadIdx.x; c < p.dim; c += 256) {
-    float dg = 0.0f, db = 0.0f;
+  for (int c = first; c < p.dim; c += NT * N) {
+    float dg[N] = {}, db[N] = {};
+#pragma unroll 2
     for (int r = 0; r < t.rows; ++r) {
       const int64_t row = t.begin + r;
-      const float d = (float)((const T*)p.dy)[row * p.ld_dy + c];
-      dg += d * ((float)((const T*)p.x)[row * p.ld_x + c] - p.mean[row]) * p.rstd[row];
-      db += d;
+      const float mu = p.mean[row], s = p.rstd[row];
+      const vec vx = read((const T*)p.x + row * p.ld_x, c), vd = read((const T*)p.dy + row * p.ld_dy, c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        dg[e] += (float)vd[e] * ((float)vx[e] - mu) * s;
+        db[e] += (float)vd[e];
+      }
     }
-    p.part[((int64_t)blockIdx.x * 2) * p.dim + c] = dg;
-    p.part[((int64_t)blockIdx.x * 2 + 1) * p.dim + c] = db;
+    float* o = p.part + (int64_t)blockIdx.x * 2 * p.dim + c;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c + e < p.dim) {
+        o[e] = dg[e];
+        o[p.dim + e] = db[e];
+      }
   }
 }
 
@@ -866,27 +915,46 @@ __global__ __launch_bounds__(256) void k_distill_join(const float* row_loss, con
 // Host side.
 // ---------------------------------------------------------------------------
 
-template <typename T, int TPR, int NV, int VEC = Elem<T>::kVec>
+template <typename T, int TPR, int NV, int VEC>
+void norm_forward(const NormArgs& p, hipStream_t s) {
+  hipLaunchKernelGGL((k_norm<T, TPR, NV, VEC>), dim3(p.ntiles), dim3(TPR > 256 ? TPR : 256), 0, s, p);
+}
+
+template <typename T, int TPR, int NV, int VEC>
 void norm_launch(const NormArgs& p, bool backward, hipStream_t s) {
-  const dim3 grid(p.ntiles), block(TPR > 256 ? TPR : 256);
-  if (backward) hipLaunchKernelGGL((k_norm_backward<T, TPR, NV, VEC>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((k_norm<T, TPR, NV, VEC>), grid, block, 0, s, p);
+  if (!backward) norm_forward<T, TPR, NV, VEC>(p, s);
+  else hipLaunchKernelGGL((k_norm_backward<T, TPR, NV, VEC>), dim3(p.ntiles), dim3(TPR > 256 ? TPR : 256), 0, s, p);
+}
+
+template <typename T, int NT, int N>
+void norm_long(const NormArgs& p, bool backward, hipStream_t s) {
+  if (backward) hipLaunchKernelGGL((k_norm_backward_long<T, NT, N>), dim3(p.ntiles), dim3(NT), 0, s, p);
+  else hipLaunchKernelGGL((k_norm_long<T, NT, N>), dim3(p.ntiles), dim3(NT), 0, s, p);
 }
 
 template <typename T>
 int norm_dispatch(const NormArgs& p, bool backward, hipStream_t s) {
-  const int64_t vecs = (p.dim + Elem<T>::kVec - 1) / Elem<T>::kVec;
-  // the smallest shape that holds a row; a wave's 64 to 96 vectors as 8-byte ones (670
-  // bfloat16 elements: an eighth of the lanes idle instead of a third)
-  if (vecs <= 64) norm_launch<T, 64, 1>(p, backward, s);
-  else if (sizeof(T) == 2 && vecs <= 96) norm_launch<T, 64, 3, 4>(p, backward, s);
-  else if (vecs <= 128) norm_launch<T, 64, 2>(p, backward, s);
-  else if (vecs <= 256) norm_launch<T, 256, 1>(p, backward, s);
-  else if (vecs <= 512) norm_launch<T, 256, 2>(p, backward, s);
-  else if (vecs <= 1024) norm_launch<T, 256, 4>(p, backward, s);
-  else if (vecs <= 2048) norm_launch<T, 512, 4>(p, backward, s);
-  else if (backward) hipLaunchKernelGGL((k_norm_backward_long<T>), dim3(p.ntiles), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((k_norm_long<T>), dim3(p.ntiles), dim3(256), 0, s, p);
+  // Threads per row, vectors per thread, elements per vector.  8-byte vectors where a 16-bit
+  // row fills 16-byte ones no better: more waves for the same registers, which is what
+  // keeps the loads coming (backward, bfloat16, rows of 2500: 3.9 TB/s in 256 x 3 x 4, 3.3 in
+  // 256 x 2 x 8; 8000: 4.1 in 1024 x 2 x 4, 3.7 in 512 x 2 x 8).  float32 takes more threads:
+  // 1500 in 512 x 1 x 4 4.4 / 4.3 TB/s (forward / backward), in 256 x 2 x 4 4.3 / 3.8.
+  const bool wide = sizeof(T) == 4;
+  const int quads = (p.dim + 3) / 4;
+  if (p.dim < 4) norm_long<T, 64, 1>(p, backward, s);
+  else if (quads <= 64) norm_launch<T, 64, 1, 4>(p, backward, s);
+  else if (quads <= 64 * 2) norm_launch<T, 64, 2, 4>(p, backward, s);
+  else if (quads <= 64 * 3) norm_launch<T, 64, 3, 4>(p, backward, s);
+  else if (quads <= 64 * 4) norm_launch<T, 64, 4, 4>(p, backward, s);
+  else if (quads <= 256 * 2) norm_launch<T, wide ? 512 : 256, wide ? 1 : 2, 4>(p, backward, s);
+  else if (quads <= 256 * 3 && !wide) norm_launch<T, 256, 3, 4>(p, backward, s);
+  else if (quads <= 512 * 2) norm_launch<T, 512, 2, 4>(p, backward, s);
+  else if (quads <= 512 * 3 && !wide) norm_launch<T, 512, 3, 4>(p, backward, s);
+  else if (quads <= 1024 * 2) norm_launch<T, 1024, 2, 4>(p, backward, s);
+  // Wider rows: forward in registers still (16000: 4.8 TB/s, streamed 2.7); backward, with
+  // its two accumulators per column, spills there (float32: 1.1 TB/s, streamed 1.8).
+  else if (quads <= 1024 * 4 && !backward) norm_forward<T, wide ? 1024 : 512, 4, Elem<T>::kVec>(p, s);
+  else norm_long<T, 1024, Elem<T>::kVec>(p, backward, s);
   return fc_internal_check_launch("k_norm");
 }
 

@@ -1068,3 +1068,36 @@ def test_two_streams_at_once_and_a_batch_that_ends(gpu):
     for a, b in zip(out, want):
       assert torch.equal(a, b)
   del filler
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("dim", [2, 3, 4, 255, 258, 510, 515, 766, 771, 1022, 1030, 1537, 2046, 2051, 2500, 4095, 4101,
+                                 6001, 7999, 8195, 12003, 16381, 16390])
+def test_layer_norm_every_launch_shape(gpu, dtype, dim):
+  """Widths on both sides of every shape's limit, none of them whole vectors; tiles that end
+  inside a block's row groups; parameters at odd elements; NaN behind the batch and its rows."""
+  rng = np.random.default_rng(dim)
+  counts = [3, 0, 37]
+  batch = ops.ClientBatch(counts)
+  buf = torch.full((42, dim + 3), math.nan, dtype=dtype, device=gpu)
+  buf[:40, 1:1 + dim] = rand(rng, (40, dim), dtype) + 0.5
+  x = buf[:, 1:1 + dim]
+  dy, res = rand(rng, (40, dim), dtype), rand(rng, (40, dim), dtype)
+  w, b = flat_params(rng, 3, [(dim,), (dim,)], dtype, 1.0)
+  out = torch.full((42, dim + 3), 9.0, dtype=dtype, device=gpu)
+  y, mean, rstd = ops.layer_norm(x, w, b, batch, out=out[:, 1:1 + dim])
+  ref = norm_reference(x[:40], w, b, counts, 1e-5, dy, res)
+  tol = norm_tolerances(ref, x[:40], b, dim, dtype, counts, dy, res)
+  check(y[:40], ref["y"], tol["y"], "y")
+  check(mean[:40], ref["mean"], tol["mean"], "mean")
+  check(rstd[:40], ref["rstd"], tol["rstd"], "rstd")
+  rows = torch.full((3, 2 * dim + 3), 3.0, device=gpu)
+  dx = torch.full((42, dim + 3), 9.0, dtype=dtype, device=gpu)
+  _, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, w, batch, residual=res, dweight=rows[:, 1:1 + dim],
+                                      dbias=rows[:, 2 + dim:2 + 2 * dim], out=dx[:, 1:1 + dim])
+  check(dx[:40, 1:1 + dim], ref["dx"], tol["dx"], "dx")
+  check(dw, ref["dw"], tol["dw"], "dw")
+  check(db, ref["db"], tol["db"], "db")
+  for t in (out, dx):
+    assert (t[:, 0] == 9.0).all() and (t[:, 1 + dim:] == 9.0).all() and (t[40:] == 9.0).all()
+  assert (rows[:, 0] == 3.0).all() and (rows[:, 1 + dim] == 3.0).all() and (rows[:, -1] == 3.0).all()
