@@ -157,18 +157,18 @@ def _params(name, t, batch, shape, dtype):
   return t
 
 
-def _grad_out(name, t, batch, shape, **others):
+def _grad_out(name, t, batch, shape, *others):
   if t is None:
     return torch.empty((batch.num_clients,) + shape, dtype=torch.float32, device=batch.device)
   _distinct(name, _params(name, t, batch, shape, torch.float32))
-  _apart(name, t, **others)
+  _apart(name, t, None, *others)
   return t
 
 
-def _out(name, out, like, batch, width, itself=None, **others):
+def _out(name, out, like, batch, width, itself=None, *others):
   if out is not None:
     _distinct(name, _activations(name, out, batch, width, like))
-    _apart(name, out, itself, **others)
+    _apart(name, out, itself, *others)
     return out
   out = torch.empty((like.shape[0], width), dtype=like.dtype, device=like.device)
   if like.shape[0] > batch.num_rows:
@@ -185,23 +185,26 @@ def _extent(t):
   return t.data_ptr(), inner * size, t.stride(0) * size, t.shape[0]
 
 
-def _apart(name, out, itself=None, **others):
+def _apart(name, out, itself, *others):
   """A given output that must not share memory with the call's other tensors.
 
-  Rows side by side in a wider buffer are apart; the one in ``itself`` may be ``out``.
+  Rows side by side in a wider buffer are apart; ``itself`` may be ``out``.
   """
   if itself is not None and itself.data_ptr() == out.data_ptr() and itself.stride() == out.stride():
     itself = None
   start, inner, outer, n = _extent(out)
-  for other, t in list(others.items()) + [("an input", itself)]:
-    if t is None or not n or not t.shape[0]:
+  end = start + (n - 1) * outer + inner
+  storage = out.untyped_storage().data_ptr()
+  for t in (itself,) + others:
+    # the two cheap tests end nearly all pairs
+    if t is None or t.data_ptr() >= end or t.untyped_storage().data_ptr() != storage or not n or not t.shape[0]:
       continue
     start2, inner2, outer2, n2 = _extent(t)
-    if start + (n - 1) * outer + inner <= start2 or start2 + (n2 - 1) * outer2 + inner2 <= start:
+    if start2 + (n2 - 1) * outer2 + inner2 <= start:
       continue
     if outer == outer2 > 0 and (start2 - start) % outer >= inner and (start - start2) % outer >= inner2:
       continue
-    raise ValueError("%s shares memory with %s" % (name, other))
+    raise ValueError("%s shares memory with another tensor of the call (%s)" % (name, list(t.shape)))
 
 
 def _vector(name, t, rows, device):
@@ -265,7 +268,7 @@ def layer_norm(x, weight, bias, batch, eps=1e-5, out=None):
       _params(name, t, batch, (dim,), x.dtype)
   if not 0.0 <= float(eps) < float("inf"):
     raise ValueError("eps must not be negative, got %r" % (eps,))
-  out = _out("out", out, x, batch, dim, x=x, weight=weight, bias=bias)
+  out = _out("out", out, x, batch, dim, None, x, weight, bias)
   mean, rstd = _stats(x.shape[0], batch), _stats(x.shape[0], batch)
   tiles, _, ntiles = batch._tiles[16]  # pylint: disable=protected-access
   _call(batch, "fc_layer_norm", _ptr(x), x.stride(0), _DTYPES[x.dtype], _ptr(tiles), ntiles, dim,
@@ -293,10 +296,9 @@ def layer_norm_backward(dy, x, mean, rstd, weight, batch, residual=None, dweight
     _activations("residual", residual, batch, dim, x)
   if accumulate and (dweight is None or dbias is None):
     raise ValueError("accumulate needs dweight and dbias to add to")
-  inputs = dict(dy=dy, x=x, mean=mean, rstd=rstd, weight=weight)
-  dbias = _grad_out("dbias", dbias, batch, (dim,), residual=residual, **inputs)
-  dweight = _grad_out("dweight", dweight, batch, (dim,), dbias=dbias, residual=residual, **inputs)
-  out = _out("out", out, x, batch, dim, residual, dweight=dweight, dbias=dbias, **inputs)
+  dbias = _grad_out("dbias", dbias, batch, (dim,), dy, x, mean, rstd, weight, residual)
+  dweight = _grad_out("dweight", dweight, batch, (dim,), dbias, dy, x, mean, rstd, weight, residual)
+  out = _out("out", out, x, batch, dim, residual, dweight, dbias, dy, x, mean, rstd, weight)
   tiles, first, ntiles = batch._tiles[32]  # pylint: disable=protected-access
   part = torch.empty(ntiles * 2 * dim, dtype=torch.float32, device=batch.device)
   _call(batch, "fc_layer_norm_backward", _ptr(dy), dy.stride(0), _ptr(x), x.stride(0), _DTYPES[x.dtype],
@@ -461,7 +463,7 @@ def linear(x, weight, bias, batch, activation=None, residual=None, preactivation
     _params("bias", bias, batch, (m,), x.dtype)
   if residual is not None:
     _activations("residual", residual, batch, m, x)
-  out = _out("out", out, x, batch, m, residual, x=x, weight=weight, bias=bias)
+  out = _out("out", out, x, batch, m, residual, x, weight, bias)
   z = _out("z", None, x, batch, m) if preactivation else None
   x, weight, tiles, last, _ws = _row_product(batch, m, x, weight)
   _call(batch, "fc_linear", _ptr(x), x.stride(0), _DTYPES[x.dtype], *tiles, batch.num_clients, k, m,
@@ -486,7 +488,7 @@ def linear_backward_input(dz, weight, batch, preactivation=None, activation=None
     _activations("preactivation", preactivation, batch, k, dz)
   if residual is not None:
     _activations("residual", residual, batch, k, dz)
-  out = _out("out", out, dz, batch, k, residual, dz=dz, weight=weight, preactivation=preactivation)
+  out = _out("out", out, dz, batch, k, residual, dz, weight, preactivation)
   dz, weight, tiles, last, _ws = _row_product(batch, k, dz, weight)
   _call(batch, "fc_linear_backward_input", _ptr(dz), dz.stride(0), _DTYPES[dz.dtype], *tiles,
         batch.num_clients, k, m, _ptr(weight), weight.stride(0), weight.stride(1), act, _ptr(preactivation),
@@ -509,8 +511,8 @@ def linear_backward_weight(dz, x, batch, dweight=None, dbias=None, bias=True, ac
   if accumulate and (dweight is None or (bias and dbias is None)):
     raise ValueError("accumulate needs dweight and dbias to add to")
   if bias:
-    dbias = _grad_out("dbias", dbias, batch, (m,), dz=dz, x=x)
-  dweight = _grad_out("dweight", dweight, batch, (m, k), dz=dz, x=x, dbias=dbias)
+    dbias = _grad_out("dbias", dbias, batch, (m,), dz, x)
+  dweight = _grad_out("dweight", dweight, batch, (m, k), dz, x, dbias)
   tiles = tuple(batch.num_clients * -(-m // h) * -(-k // max(128, h)) for h in _TILE_COSTS)
   per = 128 // x.element_size()
   dz, x, rows, splits = _operands(dz, x, batch.num_rows, tiles, -(-batch.num_rows // (per * batch.num_clients)),
@@ -617,7 +619,7 @@ def distillation_backward(logits, lse, indices, values, batch, temperature=1.0, 
   _vector("lse", lse, batch.num_rows, batch.device)
   if dloss is not None:
     _vector("dloss", dloss, batch.num_clients, batch.device)
-  out = _out("out", out, logits, batch, logits.shape[1], logits, indices=indices, values=values, lse=lse)
+  out = _out("out", out, logits, batch, logits.shape[1], logits, indices, values, lse)
   _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, lse, out, False, dloss)
   return out
 
@@ -629,6 +631,6 @@ def distillation_with_gradient(logits, indices, values, batch, temperature=1.0, 
   ``out`` may be ``logits`` itself.
   """
   indices, values = _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights)
-  out = _out("out", out, logits, batch, logits.shape[1], logits, indices=indices, values=values)
+  out = _out("out", out, logits, batch, logits.shape[1], logits, indices, values)
   loss = _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, None, out, True, None)
   return loss, out

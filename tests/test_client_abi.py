@@ -179,18 +179,18 @@ def test_memory_that_two_tensors_share():
   from federated_amd import client_ops as ops
   buf = torch.zeros(10, 100)
   left, right, mid = buf[:, :50], buf[:, 50:], buf[:, 40:60]
-  ops._apart("out", left, x=right)
-  ops._apart("out", right, x=left, y=None)
-  ops._apart("out", buf[:5], x=buf[5:])
-  ops._apart("out", left, itself=left, x=right)
-  ops._apart("out", buf[3:4, 20:30], x=left[:3], y=left[4:])
-  ops._apart("out", buf[:0], x=buf)
-  ops._apart("out", torch.zeros(1, 8).as_strided((1, 8), (0, 1)), x=buf)
+  ops._apart("out", left, None, right)
+  ops._apart("out", right, None, left, None)
+  ops._apart("out", buf[:5], None, buf[5:])
+  ops._apart("out", left, left, right)
+  ops._apart("out", buf[3:4, 20:30], None, left[:3], left[4:])
+  ops._apart("out", buf[:0], None, buf)
+  ops._apart("out", torch.zeros(1, 8).as_strided((1, 8), (0, 1)), None, buf)
   whole = buf[:, :99].unflatten(1, (9, 11))
-  ops._apart("dweight", whole, dbias=buf[:, 99:])
+  ops._apart("dweight", whole, None, buf[:, 99:])
   for out, x in [(left, mid), (mid, left), (right, mid), (buf, right), (left, left), (left[:1], buf), (whole, buf[:, 98:]),
                  (left, buf.view(-1)[:50].expand(10, 50))]:
     with pytest.raises(ValueError):
-      ops._apart("out", out, x=x)
+      ops._apart("out", out, None, x)
   with pytest.raises(ValueError):
-    ops._apart("out", left, itself=mid)
+    ops._apart("out", left, mid)
