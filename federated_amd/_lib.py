@@ -86,6 +86,8 @@ SIGNATURES = {
                                         _I64, _P, _I64, _P, _I64, _INT, _P, _I64, _P]),
     "fc_linear_backward_weight": (_INT, [_P, _I64, _P, _I64, _INT, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64,
                                          _INT, _INT, _INT, _P, _I64, _P]),
+    "fc_linear_backward_weight_few": (_INT, [_P, _I64, _P, _I64, _INT, _P, _I32, _I64, _I64, _I64, _P, _I64, _I64, _P,
+                                             _I64, _INT, _P]),
     "fc_top_logits": (_INT, [_P, _I64, _INT, _I64, _I64, _I32, _F32, _P, _P, _P, _P]),
     "fc_distill": (_INT, [_P, _I64, _INT, _I64, _I64, _P, _P, _I32, _P, _P, _I32, _F32, _P, _P, _P, _P, _P, _P, _P,
                           _I64, _P]),

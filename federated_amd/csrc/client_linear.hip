@@ -328,6 +328,9 @@ struct Stage {
 
 enum Kind { kForward = 0, kInput = 1, kWeight = 2 };
 
+constexpr int64_t kMaxBlocks = (1LL << 32) / 256 - 1;  // a launch has fewer than 2^32 threads
+constexpr int64_t kMaxSide = 1LL << 31;
+
 struct Args {
   const void* a;       // rows operand: x (forward), dz (input, weight)
   const void* b;       // W (forward, input), x (weight)
@@ -697,6 +700,85 @@ __global__ __launch_bounds__(256) void k_linear_join(const Args p) {
   }
 }
 
+// The weight gradient of clients with few rows: what bounds it is the write of M x K
+// float32, and a matrix tile's start and end (loads, LDS, way out) take longer than its
+// 64 KB of writes do.  So each thread keeps R rows of its four columns of x in registers,
+// reads the rows' dz of an output row from LDS (the same for a whole wave) and writes one
+// 16-byte vector per output row, 4 R multiply-adds each.  More rows than R are added in
+// turns.  TPR threads side by side on a row, I output rows per block.  Neighbours in memory
+// are made on one XCD: rows begin anywhere in a 128-byte line, and a line that two L2s
+// write in parts costs twice (6 x 3062 x 6547, one row: 140 us without, 107 with).
+template <typename T, int R, int TPR, int I>
+__global__ __launch_bounds__(256) void k_weight_few(const Args p) {
+  constexpr int G = 256 / TPR, kPad = R + 4;
+  __shared__ __attribute__((aligned(16))) float dz[I * kPad];
+  const int tile = xcd_order(blockIdx.x, gridDim.x);
+  const int per = p.tiles_i * p.tiles_j, client = tile / per, b = tile - client * per;
+  const int ti = b / p.tiles_j, tj = b - ti * p.tiles_j, tid = threadIdx.x;
+  const RowTile rt = p.tiles[client];
+  const int64_t i0 = (int64_t)ti * I, j = ((int64_t)tj * TPR + tid % TPR) * 4;
+  const int ni = (int)min((int64_t)I, p.ni - i0), left = (int)min((int64_t)4, p.nj - j);
+  for (int r0 = 0; r0 == 0 || r0 < rt.rows; r0 += R) {
+    const int rows = min(R, rt.rows - r0);
+    const bool add = p.accumulate || r0 > 0;
+    const T* a = (const T*)p.a + (int64_t)(rt.begin + r0) * p.lda + i0;
+    const T* x = (const T*)p.b + (int64_t)(rt.begin + r0) * p.ldb + j;
+    float xr[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const auto v = load_vec<T, 4>(x + r * p.ldb, r < rows ? left : 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) xr[r][e] = (float)v[e];
+    }
+    for (int q = tid; q < I * R; q += 256) {
+      const int r = q / I, i = q % I;
+      dz[i * kPad + r] = r < rows && i < ni ? (float)a[r * p.lda + i] : 0.0f;
+    }
+    __syncthreads();
+    if (p.db && tj == 0 && tid < ni) {
+      float* o = p.db + client * p.db_client + i0 + tid;
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum += dz[tid * kPad + r];
+      *o = add ? *o + sum : sum;
+    }
+    if (left > 0) {
+      for (int i = tid / TPR; i < ni; i += G) {
+        float* o = (float*)p.out + client * p.out_client + (i0 + i) * p.ld_out + j;
+        VecOf<float>::type v = {}, old = {};
+        if (add) old = load_vec(o, left);
+#pragma unroll
+        for (int r = 0; r < R; r += 4) {
+          const f32x4 d = *(const f32x4*)&dz[i * kPad + r];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(d[u], xr[r + u][e], v[e]);
+        }
+        store_vec(o, v + old, left);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int R, int TPR, int I>
+int few_launch(Args p, hipStream_t s) {
+  p.tiles_i = (int32_t)((p.ni + I - 1) / I);
+  p.tiles_j = (int32_t)((p.nj + 4 * TPR - 1) / (4 * TPR));
+  const int64_t blocks = (int64_t)p.tiles_i * p.tiles_j * p.nclients;
+  if (blocks > kMaxBlocks) return fc_internal_fail(-1, "too many tiles");
+  hipLaunchKernelGGL((k_weight_few<T, R, TPR, I>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+  return fc_internal_check_launch("k_weight_few");
+}
+
+template <typename T>
+int few_pick(const Args& p, int longest, hipStream_t s) {
+  // narrow rows: 16 threads each, so that a wave writes four
+  if (p.nj <= 64) return longest <= 8 ? few_launch<T, 8, 16, 256>(p, s) : few_launch<T, 16, 16, 256>(p, s);
+  return longest <= 8 ? few_launch<T, 8, 64, 64>(p, s) : few_launch<T, 16, 64, 128>(p, s);
+}
+
 // Rows copied to a stride of whole 16-byte vectors: [clients][rows][out_ld], zeros behind
 // `cols`.  A thread per vector.
 template <typename T>
@@ -711,9 +793,6 @@ __global__ __launch_bounds__(256) void k_pack_rows(const T* src, int64_t client,
   const T* from = src + which * client + r * ld + c;
   *(typename VecOf<T>::type*)(dst + (which * rows + r) * out_ld + c) = load_vec(from, cols - c);
 }
-
-constexpr int64_t kMaxBlocks = (1LL << 32) / 256 - 1;  // a launch has fewer than 2^32 threads
-constexpr int64_t kMaxSide = 1LL << 31;
 
 // Every address of the operand a multiple of 4 bytes: row stride, client stride, base.
 bool dword_aligned(const void* base, int64_t ld, int64_t client, size_t size) {
@@ -872,6 +951,32 @@ int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, 
   p.accumulate = accumulate;
   p.splits = splits; p.part = (float*)workspace;
   return dispatch<kWeight>(dtype, p, 0, tile_rows, workspace_bytes, (hipStream_t)stream);
+}
+
+int fc_linear_backward_weight_few(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
+                                  const int32_t* clients, int32_t nclients, int64_t longest, int64_t in_features,
+                                  int64_t out_features, float* dweight, int64_t dweight_client_stride,
+                                  int64_t dweight_stride, float* dbias, int64_t dbias_client_stride, int accumulate,
+                                  void* stream) {
+  if (nclients <= 0 || longest < 0 || in_features <= 0 || out_features <= 0 || in_features >= kMaxSide ||
+      out_features >= kMaxSide)
+    return fc_internal_fail(-1, "bad sizes");
+  if (!clients || !dweight || (longest > 0 && (!dz || !x))) return fc_internal_fail(-1, "null pointer");
+  Args p = {};
+  p.a = dz; p.lda = dz_stride;
+  p.b = x; p.ldb = x_stride;
+  p.tiles = (const RowTile*)clients; p.nclients = nclients;
+  p.ni = out_features; p.nj = in_features;
+  p.out = dweight; p.ld_out = dweight_stride; p.out_client = dweight_client_stride;
+  p.db = dbias; p.db_client = dbias_client_stride;
+  p.accumulate = accumulate;
+  const int rows = (int)std::min<int64_t>(longest, 1 << 30);
+  switch (dtype) {
+    case FC_FLOAT32: return few_pick<float>(p, rows, (hipStream_t)stream);
+    case FC_BFLOAT16: return few_pick<bf16>(p, rows, (hipStream_t)stream);
+    case FC_FLOAT16: return few_pick<f16>(p, rows, (hipStream_t)stream);
+  }
+  return fc_internal_fail(-1, "bad dtype");
 }
 
 }  // extern "C"

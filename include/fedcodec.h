@@ -519,6 +519,14 @@ int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, 
                               int64_t dbias_client_stride, int accumulate, int tile_rows, int splits, void* workspace,
                               int64_t workspace_bytes, void* stream);
 
+/* The same for clients of few rows, where the write of dweight is what takes time: any
+ * number of rows is right, up to 8 or 16 fast.  longest: the largest client's. */
+int fc_linear_backward_weight_few(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
+                                  const int32_t* clients, int32_t nclients, int64_t longest, int64_t in_features,
+                                  int64_t out_features, float* dweight, int64_t dweight_client_stride,
+                                  int64_t dweight_stride, float* dbias, int64_t dbias_client_stride, int accumulate,
+                                  void* stream);
+
 /* The k largest logits of every row, falling, ties to the lowest index, NaN below every
  * number; lse = log sum exp(logits / temperature) of the whole row. */
 int fc_top_logits(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t vocab, int32_t k,

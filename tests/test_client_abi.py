@@ -194,3 +194,17 @@ def test_memory_that_two_tensors_share():
       ops._apart("out", out, None, x)
   with pytest.raises(ValueError):
     ops._apart("out", left, mid)
+
+
+def test_weight_gradient_of_few_rows_refusals():
+  lib, b = _lib.load(), _buf()
+
+  def few(dz=b, dw=b, clients=1, longest=1, k=8, m=8, dtype=1):
+    return lib.fc_linear_backward_weight_few(dz, 8, b, 8, dtype, b, clients, longest, k, m, dw, 64, 8, NULL, 0, 0, None)
+
+  for kw in (dict(clients=0), dict(longest=-1), dict(k=0), dict(m=0), dict(k=1 << 31), dict(m=1 << 31)):
+    refused(few(**kw), b"sizes")
+  refused(few(dz=NULL), b"null")
+  refused(few(dw=NULL), b"null")
+  refused(few(dtype=3), b"dtype")
+  refused(few(clients=1 << 30, k=1 << 12), b"too many tiles")

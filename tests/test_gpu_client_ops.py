@@ -1101,3 +1101,34 @@ def test_layer_norm_every_launch_shape(gpu, dtype, dim):
   for t in (out, dx):
     assert (t[:, 0] == 9.0).all() and (t[:, 1 + dim:] == 9.0).all() and (t[40:] == 9.0).all()
   assert (rows[:, 0] == 3.0).all() and (rows[:, 1 + dim] == 3.0).all() and (rows[:, -1] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("k,m", [(1, 1), (3, 70), (17, 300), (64, 256), (65, 257), (131, 77), (256, 64), (515, 130)])
+@pytest.mark.parametrize("counts", [[1], [8, 0, 3], [16, 1, 0, 9], [7, 40, 0, 33]], ids=str)
+def test_weight_gradient_of_few_rows(gpu, monkeypatch, dtype, k, m, counts):
+  """The kernel for few rows at every shape, also where it takes a client's rows in turns;
+  rows behind the batch NaN, accumulation, no bias, overlapping client rows left alone."""
+  monkeypatch.setattr(ops, "_few_rows", lambda *a: True)
+  rng = np.random.default_rng(k + m)
+  n = sum(counts)
+  batch = ops.ClientBatch(counts)
+  wide = rand(rng, (n + 2, k + m + 1), dtype)
+  wide[n:] = math.nan
+  x, dz = wide[:, :k], wide[:, k + 1:]
+  rows = torch.full((len(counts), m * k + m + 2), 3.0, device=gpu)
+  dw, db = ops.linear_backward_weight(dz, x, batch, dweight=rows[:, 1:1 + m * k].unflatten(1, (m, k)),
+                                      dbias=rows[:, 1 + m * k:1 + m * k + m])
+  for c, (lo, hi) in enumerate(spans(counts)):
+    d, xx = dz[lo:hi].double().cpu(), x[lo:hi].double().cpu()
+    check(dw[c], d.t() @ xx, 2 * max(1, hi - lo) * U32 * (d.abs().t() @ xx.abs()), "dw of client %d" % c)
+    check(db[c], d.sum(0), 2 * max(1, hi - lo) * U32 * d.abs().sum(0), "db of client %d" % c)
+  assert (rows[:, 0] == 3.0).all() and (rows[:, -1] == 3.0).all()
+  alone, none = ops.linear_backward_weight(dz, x, batch, bias=False)
+  assert none is None and torch.equal(alone, dw)
+  two = rows.clone()
+  ops.linear_backward_weight(dz, x, batch, dweight=two[:, 1:1 + m * k].unflatten(1, (m, k)),
+                             dbias=two[:, 1 + m * k:1 + m * k + m], accumulate=True)
+  for c, (lo, hi) in enumerate(spans(counts)):
+    tol = 2 * (hi - lo + 2) * U32 * (dz[lo:hi].double().abs().t() @ x[lo:hi].double().abs()).cpu() * 2
+    check(two[c, 1:1 + m * k].view(m, k), 2 * dw[c].double(), tol + U32 * dw[c].double().abs().cpu() * 2, "twice")
