@@ -434,11 +434,15 @@ struct Row {
     return v;
   }
 
-  // to another row of the same length, element 0 at `to`
+  // to another row of the same length, element 0 at `to`; PASSING: not to be kept in the
+  // caches
+  template <bool PASSING>
   __device__ __forceinline__ void store(T* to, uint32_t c, vec v) const {
+    typedef typename VecOf<T, N>::loose loose;
     T* p = to + (int64_t)c - head;
     if (whole(c)) {
-      *(typename VecOf<T, N>::loose*)p = v;
+      if (PASSING) __builtin_nontemporal_store((loose)v, (loose*)p);
+      else *(loose*)p = v;
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e)
@@ -727,8 +731,10 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
   const Row<T, VEC> at_row(s, a.vocab);
   typedef uint32_t raw __attribute__((ext_vector_type(4)));
   raw held[NV > 0 ? NV : 1];  // packed: unpacked to float32 the row would not fit
+  auto past = [&](int i) { return i * kStride >= at_row.end; };  // no thread's vector i lies in the row
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    if (past(i)) continue;
     held[i] = __builtin_bit_cast(raw, at_row.load(first + i * kStride));
   }
   // vector by vector, and each use unpacks it anew
@@ -760,7 +766,7 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
     }
     if (GRAD) {
       const vec zero = {};
-      for (uint32_t c = first; c < at_row.end; c += kStride) at_row.store(grad, c, zero);
+      for (uint32_t c = first; c < at_row.end; c += kStride) at_row.template store<false>(grad, c, zero);
     }
     return;
   }
@@ -802,6 +808,7 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
       float high = -INFINITY;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        if (past(i)) continue;
         unpack(held_at(i), f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) high = fmaxf(high, f[e]);
@@ -809,6 +816,7 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
       sm.raise(block_max<NT>(high, red[2]), scale);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        if (past(i)) continue;
         unpack(held_at(i), f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) sm.sum += __builtin_amdgcn_exp2f((f[e] - sm.c) * scale);
@@ -868,15 +876,21 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
   float w = weight * a.tau;
   if (a.dloss) w *= a.dloss[client];
   const float wm = w * mass * unit;
+  // a streamed row's gradient leaves the caches to the logits that are read again (8197 rows
+  // of 131072 bfloat16: 961 us, kept 1006); of a row read once it costs up to a tenth
+  constexpr bool kPassing = LOSS && NV == 0;
   auto emit = [&](const vec& v, uint32_t c) {
     vec o;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[e] = (T)(none ? 0.0f : wm * part((float)v[e]));
-    at_row.store(grad, c, o);
+    at_row.template store<kPassing>(grad, c, o);
   };
   if constexpr (NV > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) emit(held_at(i), first + i * kStride);
+    for (int i = 0; i < NV; ++i) {
+      if (past(i)) continue;
+      emit(held_at(i), first + i * kStride);
+    }
   } else {
     // backwards: what the sum read last is in the caches still
     int i = (int)((at_row.end + kStride - 1) / kStride) - 1;
@@ -1001,7 +1015,7 @@ int distill_launch(const DistillArgs& a, int64_t rows, bool loss, hipStream_t s)
     distill_go<T, 256, 10>(a, rows, loss, s);
   } else if (vecs < 1024 * 4) {
     distill_go<T, 1024, 4>(a, rows, loss, s);
-  } else if (vecs < 1024 * 8 && sizeof(T) == 4) {  // 9375 rows of 32000: 477 us, streamed 572
+  } else if (vecs < 1024 * 8 && vecs >= 1024 * 7 && sizeof(T) == 4) {  // 9375 rows of 32000: 465 us, streamed 497
     distill_go<T, 1024, 8>(a, rows, loss, s);
   } else {
     distill_go<T, 1024, 0>(a, rows, loss, s);
