@@ -368,7 +368,7 @@ def _estimate(tiles, steps, longest, size, aligned):
         if rest:
           t += max(_STEP_LATENCY * longest, -(-rest // _CUS) * step * steps) / splits + ends
       if splits > 1:  # the parts' write and read, and the joining launch
-        t += _LAUNCH + 2 * blocks * rows * max(128, rows) * 4 / 4e6
+        t += _LAUNCH + 3 * blocks * rows * max(128, rows) * 4 / 4e6
       if best is None or t < best[0]:
         best = (t, rows, splits)
       splits *= 2
