@@ -206,6 +206,21 @@ struct Stage {
     }
   }
 
+  // direct() of the chunks whose k lies in [0, nk): the others' LDS stays as it is.
+  static __device__ __forceinline__ void direct_some(const uint32_t (&o)[kOffsets], const T* base, int64_t ld,
+                                                     int64_t nk, const char* lds) {
+    const uint32_t at = wave_base(lds);
+#pragma unroll
+    for (int s = 0; s < kChunks; ++s) {
+      int x, k;
+      source(s, threadIdx.x, x, k);
+      if (k < nk) {
+        if (kOffsets == 1) load_lds16(base + s * kChunkRows * ld, o[0], at + s * NT * 16);
+        else load_lds16(base, o[s], at + s * NT * 16);
+      }
+    }
+  }
+
   // LDS address of this wave's first instruction in the buffer `lds`.
   static __device__ __forceinline__ uint32_t wave_base(const char* lds) {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds +
@@ -357,6 +372,7 @@ struct Args {
   int32_t tiles_i, tiles_j;
   int32_t splits;      // parts of the contraction, joined through `part`
   float* part;         // [tile][split][BM BN + BM]
+  int32_t walk;        // column tiles a k_linear_short block walks
 };
 
 // Workgroups go round the 8 XCDs; tiles are dealt to them kRun at a time, so that what
@@ -665,6 +681,127 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
   }
 }
 
+// A contraction of at most two 128-byte steps and many columns (an output head's forward:
+// 96 to 10004), bound by its outputs' write: a block that makes one tile spends most of its
+// time on its start and end (20480 rows, 64 clients, bfloat16: 287 to 318 us).  So a block
+// keeps its 128 rows of A in LDS and walks along `walk` column tiles, the next one's B
+// loading while this one's outputs leave: 204 us, 2.0 TB/s.  What is left is the chain of
+// one tile (LDS reads, products, way out) in two blocks a CU; the writes alone, in such
+// tiles at rows of 20008 bytes, take 110.  In float32 the products are the chain, and it
+// gains nothing (64 to 10004: 214 us in tiles, 239 walking).
+template <typename T, int KIND, int STEPS>
+__global__ __launch_bounds__(256, 2) void k_linear_short(const Args p) {
+  constexpr bool kB_KC = KIND == kForward;
+  constexpr int kTile = 128, NT = 256, MF = 4, NF = 4;
+  typedef Stage<T, kTile, true, NT> SA;
+  typedef Stage<T, kTile, kB_KC, NT> SB;
+  constexpr int kK = SA::kK, VEC = SA::kVec, kStep = SA::kBytes;
+  constexpr int kCols = 64, kFit = 16, kRowB = kCols * 4, kLanes = kCols / VEC, kPass = 64 / kLanes;
+  // A's steps, B's steps, the waves' parts of the way out
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STEPS * kStep + 4 * kFit * kRowB];
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
+  const int chunks = (p.tiles_j + p.walk - 1) / p.walk, block = xcd_order(blockIdx.x, gridDim.x);
+  const int ti = block / chunks, first = (block - ti * chunks) * p.walk, last = min(first + p.walk, p.tiles_j);
+  const RowTile rt = p.tiles[ti];
+  const int ni = rt.rows;
+  const int64_t i0 = rt.begin;
+  const T* pb = (const T*)p.b + rt.client * p.b_client;
+
+  // Both steps of an operand's tile.  Chunks past the contraction's end are zero from the
+  // start; only part chunks go through registers.
+  auto stage = [&](auto s_type, auto kc, const T* base, int64_t ld, int nx, bool before, char* d) {
+    typedef typename decltype(s_type)::type S;
+    constexpr bool KC = decltype(kc)::value;
+    uint32_t o[S::kOffsets];
+    S::offsets(o, ld, nx);
+    const bool columns = !KC && nx < kTile && nx % VEC;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const T* b = base + s * (KC ? kK : kK * ld);
+      const int64_t left = p.nk - s * kK;
+      if (columns && (s == STEPS - 1 || ld < VEC)) S::direct_edge(b, ld, nx, left, before, d + s * kStep);
+      else if (KC && left < kK && left % VEC) S::direct_edge(b, ld, nx, left, s > 0, d + s * kStep);
+      else if (left < kK) S::direct_some(o, b, ld, left, d + s * kStep);
+      else S::direct(o, b, ld, d + s * kStep);
+    }
+  };
+  auto stage_b = [&](int tj) {
+    const int64_t j0 = (int64_t)tj * kTile;
+    stage(std::common_type<SB>(), std::integral_constant<bool, kB_KC>(), pb + (kB_KC ? j0 * p.ldb : j0), p.ldb,
+          (int)min((int64_t)kTile, p.nj - j0), tj > 0, lds + STEPS * kStep);
+  };
+  if (p.nk % kK) {
+    for (int q = tid; q < 2 * STEPS * kStep / 16; q += NT) *(typename SA::vec*)(lds + q * 16) = typename SA::vec{};
+    __syncthreads();
+  }
+  stage(std::common_type<SA>(), std::true_type(), (const T*)p.a + i0 * p.lda, p.lda, ni, false, lds);
+  stage_b(first);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+  const uint32_t base_a = SA::lane_base(wi), base_b = SB::lane_base(wj);
+  char* mine = lds + 2 * STEPS * kStep + wave * kFit * kRowB;
+  const int jt = (lane % kLanes) * VEC;
+#pragma unroll 1
+  for (int tj = first; tj < last; ++tj) {
+    const int64_t j0 = (int64_t)tj * kTile, jg = j0 + wj + jt;
+    const int left = (int)min((int64_t)kTile, p.nj - j0) - wj - jt;
+    typename VecOf<T>::type bias = {};
+    if (KIND == kForward && p.bias) bias = load_vec((const T*)p.bias + rt.client * p.bias_client + jg, left);
+    f32x4 acc[MF][NF] = {};
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        typename SA::vec fa[MF];
+        typename SB::vec fb[NF];
+#pragma unroll
+        for (int m = 0; m < MF; ++m) fa[m] = SA::frag(lds + s * kStep, base_a, m, h);
+#pragma unroll
+        for (int n = 0; n < NF; ++n) fb[n] = SB::frag(lds + (STEPS + s) * kStep, base_b, n, h);
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+#pragma unroll
+          for (int n = 0; n < NF; ++n) acc[m][n] = mma<T>(fb[n], fa[m], acc[m][n]);
+      }
+    // B is read
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (tj + 1 < last) stage_b(tj + 1);
+    // out through the wave's own part of LDS, 16 rows at a time
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+#pragma unroll
+      for (int n = 0; n < NF; ++n) {
+        const int r = lane & 15, c = n * 4 + (lane >> 4);
+        *(f32x4*)(mine + r * kRowB + ((c ^ r) << 4)) = acc[m][n];
+      }
+      __builtin_amdgcn_wave_barrier();
+      // the next B has landed, before these outputs are in its queue
+      if (m == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < kFit / kPass; ++u) {
+        const int r = lane / kLanes + u * kPass, i = wi + m * 16 + r;
+        const int64_t row = i0 + i;
+        if (i >= ni || left <= 0) continue;
+        typename VecOf<T>::type pre = {}, extra = {};
+        if (KIND == kInput && p.pre) pre = load_vec((const T*)p.pre + row * p.ld_pre + jg, left);
+        if (p.extra) extra = load_vec((const T*)p.extra + row * p.ld_extra + jg, left);
+        float v[VEC];
+#pragma unroll
+        for (int h = 0; h < VEC / 4; ++h) {
+          const f32x4 q = *(const f32x4*)(mine + r * kRowB + (((jt / 4 + h) ^ r) << 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * h + e] = q[e];
+        }
+        finish<T, KIND>(p, v, bias, pre, extra, row, jg, left);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+}
+
 // A split contraction's parts, added up in their order, and the way out.
 template <typename T, int KIND, int BM, int BN>
 __global__ __launch_bounds__(256) void k_linear_join(const Args p) {
@@ -827,7 +964,30 @@ int launch(Args p, int32_t ntiles, int64_t workspace_bytes, hipStream_t s) {
 }
 
 template <typename T, int KIND>
+int walk(Args p, int32_t ntiles, int tile_rows, hipStream_t s) {
+  if (sizeof(T) != 2 || tile_rows != 128 || p.nk * (int64_t)sizeof(T) > 256 || p.lda >= (1 << 22) || p.ldb >= (1 << 22) ||
+      !dword_aligned(p.a, p.lda, 0, sizeof(T)) || !dword_aligned(p.b, p.ldb, p.b_client, sizeof(T)))
+    return fc_internal_fail(-1, "splits FC_WALK: 16-bit types, tiles of 128 rows, at most 256 bytes of contraction, "
+                                "operands at multiples of 4 bytes");
+  if (p.nj >= kMaxSide) return fc_internal_fail(-1, "bad sizes");
+  p.tiles_j = (int32_t)((p.nj + 127) / 128);
+  // some four blocks for each that the chip holds, so that the last ones are short
+  const int64_t total = (int64_t)ntiles * p.tiles_j;
+  p.walk = (int32_t)std::min<int64_t>(std::max<int64_t>(1, total / 2048), p.tiles_j);
+  const int64_t blocks = (int64_t)ntiles * ((p.tiles_j + p.walk - 1) / p.walk);
+  if (blocks > kMaxBlocks) return fc_internal_fail(-1, "too many tiles");
+  if constexpr (sizeof(T) == 2) {
+    const dim3 grid((unsigned)blocks), block(256);
+    if (p.nk * (int64_t)sizeof(T) <= 128) hipLaunchKernelGGL((k_linear_short<T, KIND, 1>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((k_linear_short<T, KIND, 2>), grid, block, 0, s, p);
+  }
+  return fc_internal_check_launch("k_linear_short");
+}
+
+template <typename T, int KIND>
 int pick(const Args& p, int32_t ntiles, int tile_rows, int64_t workspace_bytes, hipStream_t s) {
+  if constexpr (KIND != kWeight)
+    if (p.splits == FC_WALK) return walk<T, KIND>(p, ntiles, tile_rows, s);
   switch (tile_rows) {
     case 32: return launch<T, KIND, 32, 128, 1, 4>(p, ntiles, workspace_bytes, s);
     case 128: return launch<T, KIND, 128, 128, 2, 2>(p, ntiles, workspace_bytes, s);
@@ -839,7 +999,7 @@ int pick(const Args& p, int32_t ntiles, int tile_rows, int64_t workspace_bytes, 
 
 template <int KIND>
 int dispatch(int dtype, const Args& p, int32_t ntiles, int tile_rows, int64_t workspace_bytes, hipStream_t s) {
-  if (p.splits < 1 || p.splits > 1024) return fc_internal_fail(-1, "bad splits");
+  if ((p.splits < 1 && (KIND == kWeight || p.splits != FC_WALK)) || p.splits > 1024) return fc_internal_fail(-1, "bad splits");
   switch (dtype) {
     case FC_FLOAT32: return pick<float, KIND>(p, ntiles, tile_rows, workspace_bytes, s);
     case FC_BFLOAT16: return pick<bf16, KIND>(p, ntiles, tile_rows, workspace_bytes, s);

@@ -481,7 +481,10 @@ int fc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
  * multiples of 4 bytes), from a table made with that tile_rows; and can split the
  * contraction into `splits` (1..1024) parts, joined in order through a device
  * workspace of fc_linear_workspace_bytes.  Both change speed, and results by the
- * rounding of float32 sums. */
+ * rounding of float32 sums.  fc_linear and fc_linear_backward_input of at most 256 bytes
+ * of contraction take, in 16-bit types, splits FC_WALK with tile_rows 128: blocks that
+ * walk along the columns (operands at multiples of 4 bytes, no workspace). */
+#define FC_WALK (-1)
 
 /* Rows copied to a stride of whole 16-byte vectors, [nclients][rows][dst_stride], zeros
  * behind cols: what 16-bit operands with rows at odd elements are worth where they are

@@ -208,3 +208,18 @@ def test_weight_gradient_of_few_rows_refusals():
   refused(few(dw=NULL), b"null")
   refused(few(dtype=3), b"dtype")
   refused(few(clients=1 << 30, k=1 << 12), b"too many tiles")
+
+
+def test_walk_refusals():
+  lib, b = _lib.load(), _buf()
+  b -= b % 16
+
+  def forward(rows=128, k=8, x=b, ldx=8, ldw=8, dtype=1, client=64):
+    return lib.fc_linear(x, ldx, dtype, b, 1, rows, 1, k, 8, b, client, ldw, NULL, 0, 0, NULL, 0, NULL, 0, b, 8, -1,
+                         NULL, 0, None)
+
+  for kw in (dict(rows=32), dict(rows=256), dict(k=129), dict(k=65, dtype=0), dict(x=b + 2), dict(ldx=9), dict(ldw=9),
+             dict(client=65), dict(ldx=1 << 22)):
+    refused(forward(**kw), b"FC_WALK")
+  refused(lib.fc_linear_backward_weight(b, 8, b, 8, 1, b, 1, 8, 8, b, 64, 8, NULL, 0, 0, 128, -1, NULL, 0, None),
+          b"splits")

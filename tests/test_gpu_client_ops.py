@@ -1132,3 +1132,34 @@ def test_weight_gradient_of_few_rows(gpu, monkeypatch, dtype, k, m, counts):
   for c, (lo, hi) in enumerate(spans(counts)):
     tol = 2 * (hi - lo + 2) * U32 * (dz[lo:hi].double().abs().t() @ x[lo:hi].double().abs()).cpu() * 2
     check(two[c, 1:1 + m * k].view(m, k), 2 * dw[c].double(), tol + U32 * dw[c].double().abs().cpu() * 2, "twice")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("k,m", [(64, 640), (640, 64), (96, 1000), (1000, 96), (128, 300), (300, 128), (31, 515), (515, 31),
+                                 (20, 257), (257, 20), (41, 129), (130, 2), (2, 130)])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_linear_walking_along_the_columns(gpu, monkeypatch, dtype, k, m, act):
+  """Short contractions by blocks that walk: one step and two, whole, in whole vectors and
+  not, columns that end inside a tile and a vector, operands copied and as they lie."""
+  size = torch.finfo(dtype).bits // 8
+  seen = []
+
+  def walks(batch, columns, a, weight):
+    ok = size == 2 and a.shape[1] <= 128 and not (ops._odd(a) or ops._odd(weight))
+    seen.append(ok)
+    return ok
+
+  monkeypatch.setattr(ops, "_walks", walks)
+  monkeypatch.setattr(ops, "_estimate", lambda *a: (1.0 if a[4] else 1e9, 32, 1))
+  rng = np.random.default_rng(k + m)
+  check_linear(gpu, rng, [129, 0, 40], k, m, dtype, act)
+  check_linear(gpu, rng, [300, 1], k, m, dtype, act, shared=True, behind=3)
+  assert any(seen) == (size == 2)
+
+
+def test_linear_walks_by_its_own_rule(gpu):
+  check_linear(gpu, np.random.default_rng(1), [700] * 8, 96, 5004, torch.bfloat16, None)
+  check_linear(gpu, np.random.default_rng(2), [128] * 40, 5002, 64, torch.bfloat16, "relu", shared=True)
+  batch = ops.ClientBatch([700] * 8)
+  x, w = torch.zeros(5600, 96, device=gpu, dtype=torch.bfloat16), torch.zeros(8, 5004, 96, device=gpu, dtype=torch.bfloat16)
+  assert ops._walks(batch, 5004, x, w) and not ops._walks(batch, 5004, x, w[:, :, 1:])
