@@ -348,9 +348,9 @@ def _estimate(tiles, steps, longest, size, aligned):
 
   ``tiles``: output tiles for each of _TILE_COSTS' heights; ``steps`` / ``longest``: the
   mean and the largest number of k-steps of a tile.  Splitting pays where there are
-  fewer tiles than the chip holds: 1 x 4096 by 14336 x 4096 (bfloat16) takes 38 us whole
-  and 26 in four parts; where the tiles fill it, it only costs (8 x 2048 rows, 4096 to
-  8192: 2.1 ms whole, 2.9 in four).
+  fewer tiles than the chip holds: 1 x 4096 by 14336 x 4096 (bfloat16) takes 56 us whole
+  and 29 in four parts; where the tiles fill it, it only costs (64 clients, 20480 rows, 96
+  to 10004: 287 us whole, 1057 in two).
   """
   best = None
   for (rows, (step16, step32, ends, resident)), count in zip(_TILE_COSTS.items(), tiles):
@@ -410,7 +410,7 @@ def _operands(a, b, rows, tiles, steps, longest):
   step's cost (two thirds of the load rate, and the wait is in the step); copied to
   whole vectors first they do not.  Copying pays where a row is read by many tiles: 33
   clients, 9001 rows in all, 1021 to 2050 (float16): 120 + 196 + 183 us as they are,
-  against 100 + 90 + 156 with the copies.
+  against 100 + 90 + 148 with the copies.
   """
   size = a.element_size()
   odd = (_odd(a), _odd(b)) if size == 2 else (0, 0)

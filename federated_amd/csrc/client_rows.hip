@@ -405,7 +405,8 @@ __global__ __launch_bounds__(256) void k_norm_join(const float* part, const int3
 // The k-th largest of the threads' maxima is a lower bound of the k-th largest logit, so
 // only the elements of the few threads whose maximum reaches it are looked at again, and
 // what is at or above it is ranked by counting.  When too many elements tie there, the
-// bound is made exact by a radix select first.
+// bound is made exact by a radix select first.  Bound by the read: 4096 rows of 131072
+// (bfloat16, k 64) in 224 us, 4.8 TB/s.
 // ---------------------------------------------------------------------------
 
 // A row of n elements as N-element vectors at multiples of their size: it starts `head`
@@ -663,6 +664,9 @@ __global__ __launch_bounds__(NT) void k_top_logits(const T* logits, int64_t ld, 
 //   p_k = exp(t_k / tau - L), m = sum p_k;  q = softmax(s / tau)
 //   loss_r = w_r tau^2 sum_k p_k (log p_k - log q_{i_k})
 //   ds_j = w_r tau (m q_j - sum_{k: i_k = j} p_k)
+//
+// Bound by one read of the logits and one write of the gradient: 20480 rows of 10004
+// (float32, k 32) in 328 us, 5.0 TB/s; 8197 of 131072 (bfloat16, k 64) in 921, 4.7 TB/s.
 // ---------------------------------------------------------------------------
 
 constexpr int kDistillMax = 1024;  // teacher entries per row
