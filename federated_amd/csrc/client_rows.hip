@@ -404,8 +404,9 @@ __global__ __launch_bounds__(256) void k_norm_join(const float* part, const int3
 // One read of the row: each thread keeps its elements' maximum, running maximum and sum.
 // The k-th largest of the threads' maxima is a lower bound of the k-th largest logit, so
 // only the elements of the few threads whose maximum reaches it are looked at again, and
-// what is at or above it is ranked by counting.  When too many elements tie there, the
-// bound is made exact by a radix select first.  Bound by the read: 4096 rows of 131072
+// what is at or above it is put in order: by counting for each how many are greater, a
+// few hundred and more by a bitonic network (300,000 rows of 2000, k 300: 10.6 ms, counted
+// 188).  When too many elements tie at the bound, it is made exact by a radix select first.  Bound by the read: 4096 rows of 131072
 // (bfloat16, k 64) in 224 us, 4.8 TB/s.
 // ---------------------------------------------------------------------------
 
@@ -497,7 +498,8 @@ template <typename T, int NT, int VEC>
 __global__ __launch_bounds__(NT) void k_top_logits(const T* logits, int64_t ld, int32_t vocab, int32_t k, float inv_tau,
                                                    int32_t* index, T* values, float* lse) {
   constexpr int W = NT / 64, kProbes = 16 / W;
-  constexpr int kTopCap = NT == 64 ? 512 : 2048;  // candidates ranked in LDS
+  constexpr int kTopCap = NT == 64 ? 512 : 2048;  // candidates put in order in LDS
+  constexpr uint32_t kCounted = 256;              // up to here by counting
   typedef typename VecOf<T, VEC>::type vec;
   __shared__ uint32_t maxima[NT], active[NT];
   __shared__ unsigned long long cand[kTopCap];
@@ -641,6 +643,30 @@ __global__ __launch_bounds__(NT) void k_top_logits(const T* logits, int64_t ld, 
       __syncthreads();
     }
     n = ncand;
+  }
+  if (n > kCounted) {  // in falling order by a bitonic network
+    uint32_t m = 2 * kCounted;
+    while (m < n) m *= 2;
+    for (uint32_t i = n + tid; i < m; i += NT) cand[i] = 0;  // below every candidate
+    for (uint32_t size = 2; size <= m; size *= 2)
+      for (uint32_t stride = size / 2; stride > 0; stride /= 2) {
+        __syncthreads();
+        for (uint32_t q = tid; q < m / 2; q += NT) {
+          const uint32_t i = 2 * q - (q & (stride - 1)), j = i + stride;
+          const unsigned long long a = cand[i], b = cand[j];
+          if ((a < b) == ((i & size) == 0)) {
+            cand[i] = b;
+            cand[j] = a;
+          }
+        }
+      }
+    __syncthreads();
+    for (int i = tid; i < k; i += NT) {
+      const uint32_t at = ~(uint32_t)cand[i];
+      index[row * k + i] = (int32_t)at;
+      values[row * k + i] = x[at];
+    }
+    return;
   }
   // a candidate's rank: how many are greater, counted by 8 lanes
   for (uint32_t i0 = 0; i0 < n; i0 += NT / 8) {
@@ -1040,8 +1066,10 @@ template <typename T>
 int top_launch(const void* logits, int64_t stride, int64_t rows, int64_t vocab, int32_t k, float inv_tau, int32_t* index,
                void* values, float* lse, hipStream_t s) {
   // The bound is close while there are several times as many threads with elements as k,
-  // and a block is no larger than its row keeps busy.  100,000 rows of 10004 (bfloat16, k 16):
-  // 256 threads 297 us a 60,000, 1024 threads 903; 9155 rows of 65536: 251 against 204.
+  // and a block is no larger than its row keeps busy (bfloat16, us): 200,000 rows of 3000, k
+  // 16: 64 threads 462, 256 676; 60,000 of 10004, k 16: 256 threads 303, 1024 924; 18,750 of
+  // 32000, k 300: 256 threads 3500, 1024 801; 600,000 of 1000, k 128: vectors of two 4212,
+  // of eight, which leave half of the threads without, 9661.
   auto go = [&](auto threads, auto vec) {
     constexpr int NT = decltype(threads)::value, VEC = decltype(vec)::value;
     hipLaunchKernelGGL((k_top_logits<T, NT, VEC>), dim3((unsigned)rows), dim3(NT), 0, s, (const T*)logits, stride,
