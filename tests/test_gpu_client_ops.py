@@ -1163,3 +1163,49 @@ def test_linear_walks_by_its_own_rule(gpu):
   batch = ops.ClientBatch([700] * 8)
   x, w = torch.zeros(5600, 96, device=gpu, dtype=torch.bfloat16), torch.zeros(8, 5004, 96, device=gpu, dtype=torch.bfloat16)
   assert ops._walks(batch, 5004, x, w) and not ops._walks(batch, 5004, x, w[:, :, 1:])
+
+
+def test_graph_of_every_path(gpu):
+  """Walking blocks, few rows, split contractions, copied odd rows, wide norms and streamed
+  rows in one captured graph: every replay, on new inputs and with eager work between, gives
+  the eager calls' bits."""
+  rng = np.random.default_rng(12)
+  many, few, one, odd = [ops.ClientBatch(c) for c in ([700] * 8, [8, 0, 3, 5], [1], [900, 0, 773])]
+  bf, h = torch.bfloat16, torch.float16
+  inputs = dict(
+      x1=rand(rng, (5600, 96), bf), w1=rand(rng, (8, 5004, 96), bf, 0.1),
+      x2=rand(rng, (16, 130), torch.float32), d2=rand(rng, (16, 70), torch.float32),
+      x3=rand(rng, (1, 4096), bf), w3=rand(rng, (1, 512, 4096), bf, 0.02),
+      x4=rand(rng, (1673, 1021), h), w4=rand(rng, (3, 515, 1021), h, 0.03), d4=rand(rng, (1673, 515), h),
+      x5=rand(rng, (16, 9001), bf), d5=rand(rng, (16, 9001), bf),
+      s6=rand(rng, (16, 70001), bf), t6=rand(rng, (16, 70001), bf))
+
+  def run(i):
+    out = [ops.linear(i["x1"], i["w1"], None, many)]
+    out += ops.linear_backward_weight(i["d2"], i["x2"], few)
+    out += ops.linear(i["x3"], i["w3"], None, one, activation="silu", preactivation=True)
+    out += [ops.linear(i["x4"], i["w4"], None, odd), ops.linear_backward_input(i["d4"], i["w4"], odd)]
+    out += ops.linear_backward_weight(i["d4"], i["x4"], odd)
+    y, mean, rstd = ops.layer_norm(i["x5"], None, None, few)
+    out += [y, mean, rstd, *ops.layer_norm_backward(i["d5"], i["x5"], mean, rstd, None, few)]
+    index, values, lse = ops.top_logits(i["t6"], 300, 2.0)
+    out += [index, values, lse]
+    out += ops.distillation_with_gradient(i["s6"], index, values, few, temperature=2.0, teacher_lse=lse)
+    return out
+
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    run(inputs)
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    captured = run(inputs)
+  for _ in range(4):
+    for t in inputs.values():
+      t.copy_(rand(rng, tuple(t.shape), t.dtype, float(t.float().std())))
+    want = [t.clone() for t in run(inputs)]
+    graph.replay()
+    torch.cuda.synchronize()
+    for n, (a, b) in enumerate(zip(captured, want)):
+      assert torch.equal(a, b), n
