@@ -1067,9 +1067,10 @@ int top_launch(const void* logits, int64_t stride, int64_t rows, int64_t vocab, 
                void* values, float* lse, hipStream_t s) {
   // The bound is close while there are several times as many threads with elements as k,
   // and a block is no larger than its row keeps busy (bfloat16, us): 200,000 rows of 3000, k
-  // 16: 64 threads 462, 256 676; 60,000 of 10004, k 16: 256 threads 303, 1024 924; 18,750 of
-  // 32000, k 300: 256 threads 3500, 1024 801; 600,000 of 1000, k 128: vectors of two 4212,
-  // of eight, which leave half of the threads without, 9661.
+  // 16: 64 threads 462, 256 676; 60,000 of 10004: 256 threads 303 (k 16), 802 (200), 4063
+  // (300), 4551 (1000), 1024 threads 924, 1394, 2021, 9058: where the bound is close for
+  // neither, the exact select's barriers cost the larger block more.  600,000 of 1000, k 128:
+  // vectors of two 4212, of eight, which leave half of the threads without, 9661.
   auto go = [&](auto threads, auto vec) {
     constexpr int NT = decltype(threads)::value, VEC = decltype(vec)::value;
     hipLaunchKernelGGL((k_top_logits<T, NT, VEC>), dim3((unsigned)rows), dim3(NT), 0, s, (const T*)logits, stride,
@@ -1078,7 +1079,7 @@ int top_launch(const void* logits, int64_t stride, int64_t rows, int64_t vocab, 
   typedef std::integral_constant<int, Elem<T>::kVec> wide;
   if (vocab <= 4096 && k <= 32) go(std::integral_constant<int, 64>(), wide());
   else if (vocab <= 2048) go(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-  else if (vocab <= 32768 && k <= 128) go(std::integral_constant<int, 256>(), wide());
+  else if (vocab <= 8192 || (vocab <= 32768 && (k <= 200 || k > 700))) go(std::integral_constant<int, 256>(), wide());
   else go(std::integral_constant<int, 1024>(), wide());
   return fc_internal_check_launch("k_top_logits");
 }

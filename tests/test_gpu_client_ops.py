@@ -1209,3 +1209,14 @@ def test_graph_of_every_path(gpu):
     torch.cuda.synchronize()
     for n, (a, b) in enumerate(zip(captured, want)):
       assert torch.equal(a, b), n
+
+
+@pytest.mark.parametrize("vocab,k", [(8192, 201), (8193, 200), (8193, 201), (8193, 700), (8193, 701), (2049, 1024), (32769, 701),
+                                     (5000, 600)])
+def test_top_logits_many_of_a_row(gpu, vocab, k):
+  """On both sides of the limits by k, on rows with few distinct values too: many ties."""
+  rng = np.random.default_rng(vocab + k)
+  x = rand(rng, (4, vocab), torch.bfloat16, 2.0)
+  x[2] = torch.round(x[2].float()).to(x.dtype)
+  x[3] = (torch.arange(vocab, device=gpu) % 700).to(x.dtype)
+  check_top(x, k)
