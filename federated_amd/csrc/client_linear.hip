@@ -922,22 +922,24 @@ template <typename T>
 int few_pick(const Args& p, int longest, hipStream_t s) {
   // narrow rows: 16 threads each, so that a wave writes four
   if (p.nj <= 64) return longest <= 8 ? few_launch<T, 8, 16, 256>(p, s) : few_launch<T, 16, 16, 256>(p, s);
-  return longest <= 8 ? few_launch<T, 8, 64, 64>(p, s) : few_launch<T, 16, 64, 128>(p, s);
+  if constexpr (sizeof(T) == 4)  // 16-bit rows beyond 8 are better off in matrix tiles, or in turns
+    if (longest > 8) return few_launch<T, 16, 64, 128>(p, s);
+  return few_launch<T, 8, 64, 64>(p, s);
 }
 
-// Rows copied to a stride of whole 16-byte vectors: [clients][rows][out_ld], zeros behind
-// `cols`.  A thread per vector.
-template <typename T>
-__global__ __launch_bounds__(256) void k_pack_rows(const T* src, int64_t client, int64_t ld, int32_t blocks, int64_t rows,
-                                                   int32_t cols, T* dst, int32_t out_ld) {
-  constexpr int VEC = Elem<T>::kVec;
+// Rows of 16-bit elements copied to a stride of whole 16-byte vectors: [clients][rows]
+// [out_ld], zeros behind `cols`.  A thread per vector.
+typedef f16 T16;  // a copy: 16 bits are 16 bits
+__global__ __launch_bounds__(256) void k_pack_rows(const T16* src, int64_t client, int64_t ld, int32_t blocks, int64_t rows,
+                                                   int32_t cols, T16* dst, int32_t out_ld) {
+  constexpr int VEC = Elem<T16>::kVec;
   const int64_t which = blockIdx.x / blocks, per = out_ld / VEC;
   const int64_t q = (blockIdx.x - which * blocks) * 256 + threadIdx.x;
   if (q >= rows * per) return;
   const int64_t r = q / per;
   const int c = (int)(q - r * per) * VEC;
-  const T* from = src + which * client + r * ld + c;
-  *(typename VecOf<T>::type*)(dst + (which * rows + r) * out_ld + c) = load_vec(from, cols - c);
+  const T16* from = src + which * client + r * ld + c;
+  *(VecOf<T16>::type*)(dst + (which * rows + r) * out_ld + c) = load_vec(from, cols - c);
 }
 
 // Every address of the operand a multiple of 4 bytes: row stride, client stride, base.
@@ -1034,25 +1036,16 @@ int fc_pack_rows(const void* src, int64_t client_stride, int64_t stride, int dty
     return fc_internal_fail(-1, "bad sizes");
   if (rows == 0) return 0;
   if (!src || !dst) return fc_internal_fail(-1, "null pointer");
-  const int64_t vec = dtype == FC_FLOAT32 ? 4 : 8;
+  if (dtype != FC_BFLOAT16 && dtype != FC_FLOAT16) return fc_internal_fail(-1, "bad dtype");
+  constexpr int64_t vec = Elem<T16>::kVec;
   if (dst_stride % vec || (uintptr_t)dst % 16) return fc_internal_fail(-1, "dst is not in whole 16-byte vectors");
   if (rows >= kMaxSide) return fc_internal_fail(-1, "bad sizes");
   const int64_t blocks = (rows * (dst_stride / vec) + 255) / 256;
   if (blocks > kMaxBlocks / nclients) return fc_internal_fail(-1, "too many rows");
   const dim3 grid((unsigned)(blocks * nclients));
   hipStream_t s = (hipStream_t)stream;
-  switch (dtype) {
-    case FC_FLOAT32:
-      hipLaunchKernelGGL((k_pack_rows<float>), grid, dim3(256), 0, s, (const float*)src, client_stride, stride,
-                         (int32_t)blocks, rows, (int32_t)cols, (float*)dst, (int32_t)dst_stride);
-      break;
-    case FC_BFLOAT16:
-    case FC_FLOAT16:  // a copy: 16 bits are 16 bits
-      hipLaunchKernelGGL((k_pack_rows<f16>), grid, dim3(256), 0, s, (const f16*)src, client_stride, stride,
-                         (int32_t)blocks, rows, (int32_t)cols, (f16*)dst, (int32_t)dst_stride);
-      break;
-    default: return fc_internal_fail(-1, "bad dtype");
-  }
+  hipLaunchKernelGGL(k_pack_rows, grid, dim3(256), 0, s, (const T16*)src, client_stride, stride, (int32_t)blocks, rows,
+                     (int32_t)cols, (T16*)dst, (int32_t)dst_stride);
   return fc_internal_check_launch("k_pack_rows");
 }
 

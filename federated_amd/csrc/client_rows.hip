@@ -983,7 +983,7 @@ int norm_dispatch(const NormArgs& p, bool backward, hipStream_t s) {
   // keeps the loads coming (backward, bfloat16, rows of 2500: 3.9 TB/s in 256 x 3 x 4, 3.3 in
   // 256 x 2 x 8; 8000: 4.1 in 1024 x 2 x 4, 3.7 in 512 x 2 x 8).  float32 takes more threads:
   // 1500 in 512 x 1 x 4 4.4 / 4.3 TB/s (forward / backward), in 256 x 2 x 4 4.3 / 3.8.
-  const bool wide = sizeof(T) == 4;
+  constexpr bool wide = sizeof(T) == 4;
   const int quads = (p.dim + 3) / 4;
   if (p.dim < 4) norm_long<T, 64, 1>(p, backward, s);
   else if (quads <= 64) norm_launch<T, 64, 1, 4>(p, backward, s);
@@ -991,9 +991,9 @@ int norm_dispatch(const NormArgs& p, bool backward, hipStream_t s) {
   else if (quads <= 64 * 3) norm_launch<T, 64, 3, 4>(p, backward, s);
   else if (quads <= 64 * 4) norm_launch<T, 64, 4, 4>(p, backward, s);
   else if (quads <= 256 * 2) norm_launch<T, wide ? 512 : 256, wide ? 1 : 2, 4>(p, backward, s);
-  else if (quads <= 256 * 3 && !wide) norm_launch<T, 256, 3, 4>(p, backward, s);
+  else if (quads <= 256 * 3 && !wide) norm_launch<T, wide ? 512 : 256, wide ? 2 : 3, 4>(p, backward, s);
   else if (quads <= 512 * 2) norm_launch<T, 512, 2, 4>(p, backward, s);
-  else if (quads <= 512 * 3 && !wide) norm_launch<T, 512, 3, 4>(p, backward, s);
+  else if (quads <= 512 * 3 && !wide) norm_launch<T, wide ? 1024 : 512, wide ? 2 : 3, 4>(p, backward, s);
   else if (quads <= 1024 * 2) norm_launch<T, 1024, 2, 4>(p, backward, s);
   // Wider rows: forward in registers still (16000: 4.8 TB/s, streamed 2.7); backward, with
   // its two accumulators per column, spills there (float32: 1.1 TB/s, streamed 1.8).
@@ -1046,7 +1046,7 @@ int distill_launch(const DistillArgs& a, int64_t rows, bool loss, hipStream_t s)
   } else if (vecs < 1024 * 4) {
     distill_go<T, 1024, 4>(a, rows, loss, s);
   } else if (vecs < 1024 * 8 && vecs >= 1024 * 7 && sizeof(T) == 4) {  // 9375 rows of 32000: 465 us, streamed 497
-    distill_go<T, 1024, 8>(a, rows, loss, s);
+    distill_go<T, 1024, sizeof(T) == 4 ? 8 : 4>(a, rows, loss, s);
   } else {
     distill_go<T, 1024, 0>(a, rows, loss, s);
   }

@@ -486,9 +486,9 @@ int fc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
  * walk along the columns (operands at multiples of 4 bytes, no workspace). */
 #define FC_WALK (-1)
 
-/* Rows copied to a stride of whole 16-byte vectors, [nclients][rows][dst_stride], zeros
- * behind cols: what 16-bit operands with rows at odd elements are worth where they are
- * read often. */
+/* Rows of 16-bit elements copied to a stride of whole 16-byte vectors,
+ * [nclients][rows][dst_stride], zeros behind cols: what operands with rows at odd elements
+ * are worth where they are read often. */
 int fc_pack_rows(const void* src, int64_t client_stride, int64_t stride, int dtype, int32_t nclients, int64_t rows,
                  int64_t cols, void* dst, int64_t dst_stride, void* stream);
 

@@ -223,3 +223,9 @@ def test_walk_refusals():
     refused(forward(**kw), b"FC_WALK")
   refused(lib.fc_linear_backward_weight(b, 8, b, 8, 1, b, 1, 8, 8, b, 64, 8, NULL, 0, 0, 128, -1, NULL, 0, None),
           b"splits")
+
+
+def test_pack_rows_takes_16_bit_rows_only():
+  lib, b = _lib.load(), ctypes.create_string_buffer(128)
+  at = (ctypes.addressof(b) + 15) // 16 * 16
+  refused(lib.fc_pack_rows(at, 0, 7, 0, 1, 1, 7, at, 8, None), b"dtype")
