@@ -1189,7 +1189,8 @@ int fc_distill(const void* logits, int64_t stride, int dtype, int64_t rows, int6
     return fc_internal_fail(-1, "bad sizes");
   if (k <= 0 || k > kDistillMax) return fc_internal_fail(-1, "bad k");
   if (bad_temperature(temperature)) return fc_internal_fail(-1, "bad temperature");
-  if (!offsets || (!loss && !grad) || (!loss && rows && !lse) || (loss && rows && !row_loss))
+  // without rows every tensor of them may be empty, its pointer null
+  if (!offsets || (rows && ((!loss && !grad) || (!loss && !lse) || (loss && !row_loss))))
     return fc_internal_fail(-1, "null pointer");
   if (loss && dloss) return fc_internal_fail(-1, "dloss goes with the gradient alone");
   hipStream_t s = (hipStream_t)stream;

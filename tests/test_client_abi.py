@@ -229,3 +229,16 @@ def test_pack_rows_takes_16_bit_rows_only():
   lib, b = _lib.load(), ctypes.create_string_buffer(128)
   at = (ctypes.addressof(b) + 15) // 16 * 16
   refused(lib.fc_pack_rows(at, 0, 7, 0, 1, 1, 7, at, 8, None), b"dtype")
+
+
+def test_distillation_without_rows():
+  """No rows and no loss wanted: the gradient of an empty tensor may be a null pointer."""
+  lib, b = _lib.load(), _buf()
+
+  def distill(rows, lse=NULL, grad=NULL, logits=NULL):
+    return lib.fc_distill(logits, 8, 0, rows, 8, b, b, 2, b, b, 1, 1.0, NULL, NULL, NULL, NULL, lse, NULL, grad, 8, None)
+
+  assert distill(0) == 0 and distill(0, lse=b, grad=b, logits=b) == 0
+  refused(distill(1, lse=b, logits=b), b"null")
+  refused(distill(1, grad=b, logits=b), b"null")
+  refused(distill(1, lse=b, grad=b), b"null")

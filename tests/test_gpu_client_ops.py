@@ -1220,3 +1220,21 @@ def test_top_logits_many_of_a_row(gpu, vocab, k):
   x[2] = torch.round(x[2].float()).to(x.dtype)
   x[3] = (torch.arange(vocab, device=gpu) % 700).to(x.dtype)
   check_top(x, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("behind", [0, 3])
+def test_distillation_without_rows(gpu, dtype, behind):
+  """Every form on a batch without rows, over logits of none and over rows behind the batch."""
+  batch = ops.ClientBatch([0, 0])
+  logits = torch.full((behind, 8), 2.0, dtype=dtype, device=gpu)
+  idx = torch.zeros(behind, 3, dtype=torch.int32, device=gpu)
+  val = torch.zeros(behind, 3, device=gpu)
+  loss, lse = ops.distillation(logits, idx, val, batch)
+  assert (loss == 0).all() and loss.shape == (2,) and lse.shape == (behind,)
+  grad = ops.distillation_backward(logits, lse, idx, val, batch)
+  assert grad.shape == (behind, 8) and grad.dtype == dtype and (grad == 0).all()
+  grad = ops.distillation_backward(logits, lse, idx, val, batch, dloss=torch.ones(2, device=gpu), out=logits)
+  assert (grad == 2.0).all()
+  loss, grad = ops.distillation_with_gradient(logits, idx, val, batch)
+  assert (loss == 0).all() and grad.shape == (behind, 8)
