@@ -651,7 +651,7 @@ def distillation_backward(logits, lse, indices, values, batch, temperature=1.0, 
   _vector("lse", lse, batch.num_rows, batch.device)
   if dloss is not None:
     _vector("dloss", dloss, batch.num_clients, batch.device)
-  out = _out("out", out, logits, batch, logits.shape[1], logits, indices, values, lse)
+  out = _out("out", out, logits, batch, logits.shape[1], logits, indices, values, lse, teacher_lse, row_weights, dloss)
   _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, lse, out, False, dloss)
   return out
 
@@ -663,6 +663,6 @@ def distillation_with_gradient(logits, indices, values, batch, temperature=1.0, 
   ``out`` may be ``logits`` itself.
   """
   indices, values = _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights)
-  out = _out("out", out, logits, batch, logits.shape[1], logits, indices, values)
+  out = _out("out", out, logits, batch, logits.shape[1], logits, indices, values, teacher_lse, row_weights)
   loss = _distill(logits, indices, values, batch, temperature, teacher_lse, row_weights, None, out, True, None)
   return loss, out

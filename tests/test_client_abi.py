@@ -242,3 +242,40 @@ def test_distillation_without_rows():
   refused(distill(1, lse=b, logits=b), b"null")
   refused(distill(1, grad=b, logits=b), b"null")
   refused(distill(1, lse=b, grad=b), b"null")
+
+
+def host_batch(counts):
+  """What the argument checks read of a batch, its tensors on the host."""
+  import torch
+  from federated_amd import client_ops as ops
+  batch = object.__new__(ops.ClientBatch)
+  batch.device, batch.num_clients, batch.num_rows = torch.device("cpu"), len(counts), sum(counts)
+  batch.row_client = batch.offsets = torch.zeros(8, dtype=torch.int32)
+  return batch
+
+
+@pytest.mark.parametrize("over", ["teacher_lse", "row_weights", "dloss", "lse"])
+def test_a_gradient_over_the_rows_vectors_is_refused(monkeypatch, over):
+  """Blocks read these while others write gradient rows."""
+  import torch
+  from federated_amd import client_ops as ops
+  calls = []
+  monkeypatch.setattr(ops, "_call", lambda where, name, *args: calls.append(name))
+  batch, buf = host_batch([3, 2]), torch.ones(200)
+  logits, out = torch.zeros(5, 8), buf[:40].view(5, 8)
+  idx, val = torch.zeros(5, 2, dtype=torch.int32), torch.zeros(5, 2)
+  for start in (0, 17, 35):
+    vectors = dict(teacher_lse=buf[40:45], row_weights=buf[50:55], dloss=buf[60:62], lse=buf[70:75])
+    vectors[over] = buf[start:start + (2 if over == "dloss" else 5)]
+    dloss, lse = vectors.pop("dloss"), vectors.pop("lse")
+    with pytest.raises(ValueError, match="shares memory"):
+      ops.distillation_backward(logits, lse, idx, val, batch, dloss=dloss, out=out, **vectors)
+    if over in vectors:
+      with pytest.raises(ValueError, match="shares memory"):
+        ops.distillation_with_gradient(logits, idx, val, batch, out=out, **vectors)
+  assert not calls
+  # beside them: taken
+  vectors = dict(teacher_lse=buf[40:45], row_weights=buf[50:55])
+  assert ops.distillation_backward(logits, buf[70:75], idx, val, batch, dloss=buf[60:62], out=out, **vectors) is out
+  assert ops.distillation_with_gradient(logits, idx, val, batch, out=out, **vectors)[1] is out
+  assert calls == ["fc_distill"] * 2
