@@ -93,15 +93,20 @@ template <> __device__ __forceinline__ f32x4 mma<float>(VecOf<float>::type j, Ve
 }
 
 // 16 bytes per lane from base + off straight to LDS (dword-aligned source): lane l's land
-// at lds + 16 l.  Untracked by the compiler: the caller waits for vmcnt(0).
+// at lds + 16 l.  Untracked by the compiler: the caller waits for vmcnt(0).  M0 is named as
+// changed: a value of the compiler's own in it is set anew (the compiler warns that it
+// would not be kept, which is what is meant).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
-               : "memory");
+               : "memory", "m0");
 }
 
 __device__ __forceinline__ void load_lds16_at(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // The thread's number, to the compiler a new value each time: addresses made from it
 // are not carried in registers through the main loop.

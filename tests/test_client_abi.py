@@ -279,3 +279,20 @@ def test_a_gradient_over_the_rows_vectors_is_refused(monkeypatch, over):
   assert ops.distillation_backward(logits, buf[70:75], idx, val, batch, dloss=buf[60:62], out=out, **vectors) is out
   assert ops.distillation_with_gradient(logits, idx, val, batch, out=out, **vectors)[1] is out
   assert calls == ["fc_distill"] * 2
+
+
+def test_inline_assembly_names_the_scalar_register_it_sets():
+  """A statement that writes M0 says so: the compiler keeps its own values there."""
+  import glob
+  import os
+  import re
+  root = os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__)))
+  writes = 0
+  for path in glob.glob(os.path.join(root, "federated_amd", "csrc", "*")):
+    with open(path) as f:
+      for statement in re.findall(r"asm volatile\(.*?\);\n", f.read(), re.S):
+        code, *rest = statement.split("::")
+        if re.search(r"\bs_mov_b32 m0\b", code):
+          writes += 1
+          assert '"m0"' in "".join(rest), (path, statement)
+  assert writes
