@@ -632,8 +632,9 @@ def distillation(logits, indices, values, batch, temperature=1.0, teacher_lse=No
   ``teacher_lse`` (float32 [rows], at this temperature: p then sums to less than one,
   the rest of the teacher's mass is left out) or, when None, makes p sum to one.
   ``row_weights``: float32 [rows]; None: 1 / (the client's rows), the mean.  A row of
-  weight 0 is not looked at.  ``lse`` (float32 [rows]) is for
-  ``distillation_backward``.
+  weight 0 is not looked at.  ``lse`` (float32 [rows], of the logits at this temperature; NaN
+  where a row was not looked at) is for ``distillation_backward``, whose teacher and
+  weights may be others.
   """
   indices, values = _teacher(logits, indices, values, batch, temperature, teacher_lse, row_weights)
   lse = _stats(logits.shape[0], batch)

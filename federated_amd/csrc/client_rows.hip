@@ -792,7 +792,7 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
   if (!any || weight == 0.0f) {  // nothing to learn from: no loss, no gradient, whatever the logits
     if (LOSS && tid == 0) {
       a.row_loss[row] = 0.0f;
-      if (a.lse) a.lse[row] = 0.0f;
+      if (a.lse) a.lse[row] = NAN;  // not summed: a gradient that looks at the row sums it
     }
     if (GRAD) {
       const vec zero = {};

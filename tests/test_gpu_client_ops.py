@@ -1238,3 +1238,23 @@ def test_distillation_without_rows(gpu, dtype, behind):
   assert (grad == 2.0).all()
   loss, grad = ops.distillation_with_gradient(logits, idx, val, batch)
   assert (loss == 0).all() and grad.shape == (behind, 8)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("vocab", [40, 3001, 70001])
+def test_distillation_gradient_of_rows_the_loss_left_out(gpu, dtype, vocab):
+  """A saved log-sum-exp serves a gradient by other weights and another teacher: rows that
+  the loss did not look at (no weight, nothing but padding) are summed by the gradient."""
+  rng = np.random.default_rng(vocab)
+  counts = [3, 2]
+  batch = ops.ClientBatch(counts)
+  logits = rand(rng, (5, vocab), dtype, 2.0) + 3.0
+  index, values = teacher_rows(rng, 5, vocab, 6, pad=0)
+  bare = index.clone()
+  bare[1] = -1
+  weights = torch.tensor([1.0, 0.5, 0.0, 0.0, 2.0], device=gpu)
+  _, lse = ops.distillation(logits, bare, values, batch, row_weights=weights)
+  _, grad, _, eg = distill_reference(logits, index, values, counts, 1.0)
+  got = ops.distillation_backward(logits, lse, index, values, batch)
+  check(got, grad, eg + unit(dtype) * (grad.abs() + eg) + tiny(dtype), "gradient")
+  assert lse.isnan().tolist() == [False, True, True, True, False]
