@@ -959,21 +959,40 @@ __global__ __launch_bounds__(256) void k_distill_join(const float* row_loss, con
 // Host side.
 // ---------------------------------------------------------------------------
 
+// A launch has fewer than 2^32 threads: `blocks` workgroups of NT in as many launches as
+// that takes, go(first, how many).
+template <int NT, typename Go>
+void in_parts(int64_t blocks, Go go) {
+  constexpr int64_t most = ((1LL << 32) - 1) / NT;
+  for (int64_t first = 0; first < blocks; first += most) go(first, dim3((unsigned)std::min(most, blocks - first)));
+}
+
+// A norm's kernel over its tiles.
+template <int NT>
+void norm_go(void (*kernel)(const NormArgs), const NormArgs& all, hipStream_t s) {
+  in_parts<NT>(all.ntiles, [&](int64_t first, dim3 grid) {
+    NormArgs p = all;
+    p.tiles += first;
+    if (p.part) p.part += first * 2 * p.dim;
+    hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, s, p);
+  });
+}
+
 template <typename T, int TPR, int NV, int VEC>
 void norm_forward(const NormArgs& p, hipStream_t s) {
-  hipLaunchKernelGGL((k_norm<T, TPR, NV, VEC>), dim3(p.ntiles), dim3(TPR > 256 ? TPR : 256), 0, s, p);
+  norm_go<(TPR > 256 ? TPR : 256)>(k_norm<T, TPR, NV, VEC>, p, s);
 }
 
 template <typename T, int TPR, int NV, int VEC>
 void norm_launch(const NormArgs& p, bool backward, hipStream_t s) {
   if (!backward) norm_forward<T, TPR, NV, VEC>(p, s);
-  else hipLaunchKernelGGL((k_norm_backward<T, TPR, NV, VEC>), dim3(p.ntiles), dim3(TPR > 256 ? TPR : 256), 0, s, p);
+  else norm_go<(TPR > 256 ? TPR : 256)>(k_norm_backward<T, TPR, NV, VEC>, p, s);
 }
 
 template <typename T, int NT, int N>
 void norm_long(const NormArgs& p, bool backward, hipStream_t s) {
-  if (backward) hipLaunchKernelGGL((k_norm_backward_long<T, NT, N>), dim3(p.ntiles), dim3(NT), 0, s, p);
-  else hipLaunchKernelGGL((k_norm_long<T, NT, N>), dim3(p.ntiles), dim3(NT), 0, s, p);
+  if (backward) norm_go<NT>(k_norm_backward_long<T, NT, N>, p, s);
+  else norm_go<NT>(k_norm_long<T, NT, N>, p, s);
 }
 
 template <typename T>
@@ -1012,16 +1031,28 @@ int norm_dtype(int dtype, const NormArgs& p, bool backward, hipStream_t s) {
 }
 
 template <typename T, int NT, int NV>
-void distill_go(const DistillArgs& a, int64_t rows, bool loss, hipStream_t s) {
-  const dim3 grid((unsigned)rows), block(NT);
-  const size_t lds = 16 * (size_t)a.k;
-  if constexpr (NV > 0) {
-    hipLaunchKernelGGL((k_distill<T, NT, NV, true, true>), grid, block, lds, s, a);
-  } else {
-    if (loss && a.grad) hipLaunchKernelGGL((k_distill<T, NT, 0, true, true>), grid, block, lds, s, a);
-    else if (loss) hipLaunchKernelGGL((k_distill<T, NT, 0, true, false>), grid, block, lds, s, a);
-    else hipLaunchKernelGGL((k_distill<T, NT, 0, false, true>), grid, block, lds, s, a);
-  }
+void distill_go(const DistillArgs& all, int64_t rows, bool loss, hipStream_t s) {
+  in_parts<NT>(rows, [&](int64_t first, dim3 grid) {
+    DistillArgs a = all;
+    a.logits = (const T*)a.logits + first * a.ld;
+    a.index += first * a.k;
+    a.values += first * a.k;
+    a.row_client += first;
+    if (a.teacher_lse) a.teacher_lse += first;
+    if (a.row_weights) a.row_weights += first;
+    if (a.row_loss) a.row_loss += first;
+    if (a.lse) a.lse += first;
+    if (a.grad) a.grad = (T*)a.grad + first * a.ld_grad;
+    const dim3 block(NT);
+    const size_t lds = 16 * (size_t)a.k;
+    if constexpr (NV > 0) {
+      hipLaunchKernelGGL((k_distill<T, NT, NV, true, true>), grid, block, lds, s, a);
+    } else {
+      if (loss && a.grad) hipLaunchKernelGGL((k_distill<T, NT, 0, true, true>), grid, block, lds, s, a);
+      else if (loss) hipLaunchKernelGGL((k_distill<T, NT, 0, true, false>), grid, block, lds, s, a);
+      else hipLaunchKernelGGL((k_distill<T, NT, 0, false, true>), grid, block, lds, s, a);
+    }
+  });
 }
 
 template <typename T>
@@ -1073,8 +1104,10 @@ int top_launch(const void* logits, int64_t stride, int64_t rows, int64_t vocab, 
   // vectors of two 4212, of eight, which leave half of the threads without, 9661.
   auto go = [&](auto threads, auto vec) {
     constexpr int NT = decltype(threads)::value, VEC = decltype(vec)::value;
-    hipLaunchKernelGGL((k_top_logits<T, NT, VEC>), dim3((unsigned)rows), dim3(NT), 0, s, (const T*)logits, stride,
-                       (int32_t)vocab, k, inv_tau, index, (T*)values, lse);
+    in_parts<NT>(rows, [&](int64_t first, dim3 grid) {
+      hipLaunchKernelGGL((k_top_logits<T, NT, VEC>), grid, dim3(NT), 0, s, (const T*)logits + first * stride, stride,
+                         (int32_t)vocab, k, inv_tau, index + first * k, (T*)values + first * k, lse + first);
+    });
   };
   typedef std::integral_constant<int, Elem<T>::kVec> wide;
   if (vocab <= 4096 && k <= 32) go(std::integral_constant<int, 64>(), wide());
@@ -1085,7 +1118,7 @@ int top_launch(const void* logits, int64_t stride, int64_t rows, int64_t vocab, 
 }
 
 constexpr int64_t kMaxDim = 1 << 24;
-constexpr int64_t kMaxBlocks = (1LL << 32) / 256 - 1;  // a launch has fewer than 2^32 threads
+constexpr int64_t kMaxBlocks = (1LL << 32) / 256 - 1;  // of 256 threads in one launch
 
 bool bad_temperature(float t) { return !(t >= FC_MIN_TEMPERATURE && t <= FC_MAX_TEMPERATURE); }
 
@@ -1207,7 +1240,9 @@ int fc_distill(const void* logits, int64_t stride, int dtype, int64_t rows, int6
     if (const int rc = distill_dtype(dtype, a, rows, loss != nullptr, s)) return rc;
   }
   if (!loss) return 0;
-  hipLaunchKernelGGL(k_distill_join, dim3((unsigned)nclients), dim3(256), 0, s, (const float*)row_loss, offsets, loss);
+  in_parts<256>(nclients, [&](int64_t first, dim3 grid) {
+    hipLaunchKernelGGL(k_distill_join, grid, dim3(256), 0, s, (const float*)row_loss, offsets + first, loss + first);
+  });
   return fc_internal_check_launch("k_distill_join");
 }
 

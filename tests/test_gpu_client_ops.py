@@ -1258,3 +1258,84 @@ def test_distillation_gradient_of_rows_the_loss_left_out(gpu, dtype, vocab):
   got = ops.distillation_backward(logits, lse, index, values, batch)
   check(got, grad, eg + unit(dtype) * (grad.abs() + eg) + tiny(dtype), "gradient")
   assert lse.isnan().tolist() == [False, True, True, True, False]
+
+
+# A launch has fewer than 2^32 threads, so a row or client each past these counts takes another.
+MOST = {64: (2**32 - 1) // 64, 256: (2**32 - 1) // 256}
+
+
+def around(n, at):
+  """Rows to look at: both ends and both sides of a launch's last."""
+  return torch.tensor(sorted({0, 1, 777, at - 2, at - 1, at, at + 1, n - 2, n - 1}), device="cuda")
+
+
+def test_top_logits_of_more_rows_than_a_launch(gpu):
+  """16.8 million rows of 40, k 33: blocks of 256 threads."""
+  n, v, k = MOST[256] + 300, 40, 33
+  gen = torch.Generator(device=gpu).manual_seed(3)
+  x = torch.empty(n, v, dtype=torch.bfloat16, device=gpu).normal_(0.0, 2.0, generator=gen)
+  index, values, lse = ops.top_logits(x, k)
+  rows = around(n, MOST[256])
+  want, want_lse = top_reference(x[rows], k)
+  assert torch.equal(index[rows].long().cpu(), want)
+  assert torch.equal(values[rows], torch.gather(x[rows], 1, index[rows].long()))
+  check(lse[rows], want_lse, (v / 1024 + 48 + 4 * 16) * 2 * U32, "lse")
+  # every row: falling values at the places they are said to be at
+  for lo in range(0, n, 1 << 22):
+    i, val = index[lo:lo + (1 << 22)], values[lo:lo + (1 << 22)]
+    assert bool((val[:, 1:] <= val[:, :-1]).all()) and bool((i >= 0).all()) and bool((i < v).all())
+    assert torch.equal(torch.gather(x[lo:lo + (1 << 22)], 1, i.long()), val)
+    assert bool(lse[lo:lo + (1 << 22)].isfinite().all())
+
+
+def test_distillation_of_more_rows_than_a_launch(gpu):
+  """67 million rows of 8: blocks of one wave; loss alone, gradient alone, both."""
+  n, v = MOST[64] + 500, 8
+  gen = torch.Generator(device=gpu).manual_seed(4)
+  x = torch.empty(n, v, dtype=torch.float16, device=gpu).normal_(0.0, 2.0, generator=gen)
+  index = torch.randint(0, v, (n, 1), generator=gen, device=gpu, dtype=torch.int32)
+  values = torch.zeros(n, 1, device=gpu)
+  lse_t = torch.empty(n, device=gpu).uniform_(0.1, 1.0, generator=gen)
+  weights = torch.ones(n, device=gpu)
+  counts = [MOST[64] - 1, 400, 101]
+  batch = ops.ClientBatch(counts)
+  loss, grad = ops.distillation_with_gradient(x, index, values, batch, teacher_lse=lse_t, row_weights=weights)
+  loss2, lse = ops.distillation(x, index, values, batch, teacher_lse=lse_t, row_weights=weights)
+  assert torch.equal(loss, loss2)
+  back = ops.distillation_backward(x, lse, index, values, batch, teacher_lse=lse_t, row_weights=weights)
+  rows = around(n, MOST[64])
+  want, g, el, eg = distill_reference(x[rows], index[rows], values[rows], [len(rows)], 1.0, lse_t[rows], weights[rows])
+  eg = eg + unit(torch.float16) * (g.abs() + eg) + tiny(torch.float16)
+  check(grad[rows], g, eg, "gradient")
+  check(back[rows], g, eg, "gradient alone")
+  # every row: p (log p - log q) summed over the last two clients, in float64
+  for c, (lo, hi) in list(enumerate(spans(counts)))[1:]:
+    logp = -lse_t[lo:hi].double()
+    logq = torch.log_softmax(x[lo:hi].double(), 1).gather(1, index[lo:hi].long())[:, 0]
+    term = logp.exp() * (logp - logq)
+    tol = float((logp.exp() * (logp.abs() + logq.abs() + 2)).sum()) * (2 * (6 * 32 + 52) * 2 + hi - lo + 8) * U32
+    check(loss[c], term.sum(), tol, "loss")
+  assert bool(lse.isfinite().all()) and bool(grad.isfinite().all())
+
+
+def test_more_clients_than_a_launch(gpu):
+  """16.8 million clients of one row: the losses' join and the norm's tiles."""
+  n, d = MOST[256] + 300, 4
+  gen = torch.Generator(device=gpu).manual_seed(5)
+  batch = ops.ClientBatch(np.ones(n, np.int64))
+  x = torch.empty(n, d, device=gpu).normal_(0.0, 1.0, generator=gen)
+  index = torch.randint(0, d, (n, 1), generator=gen, device=gpu, dtype=torch.int32)
+  loss, lse = ops.distillation(x, index, torch.zeros(n, 1, device=gpu), batch)
+  want = torch.logsumexp(x.double(), 1)
+  size = 1 + x.double().abs().amax(1)
+  assert bool(((lse.double() - want).abs() <= 64 * U32 * size).all())
+  want = want - x.double().gather(1, index.long())[:, 0]
+  assert bool(((loss.double() - want).abs() <= 64 * U32 * size).all())
+  y, mean, rstd = ops.layer_norm(x, None, None, batch)
+  rows = around(n, MOST[256])
+  ref = norm_reference(x[rows], None, None, [len(rows)], 1e-5)
+  tol = norm_tolerances(ref, x[rows], None, d, torch.float32)
+  for name, got in dict(y=y, mean=mean, rstd=rstd).items():
+    check(got[rows], ref[name], tol[name], name)
+  mu = x.double().mean(1)
+  assert bool(((mean.double() - mu).abs() <= 32 * U32 * x.double().abs().amax(1)).all())
