@@ -1339,3 +1339,25 @@ def test_more_clients_than_a_launch(gpu):
     check(got[rows], ref[name], tol[name], name)
   mu = x.double().mean(1)
   assert bool(((mean.double() - mu).abs() <= 32 * U32 * x.double().abs().amax(1)).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+def test_gelu_of_every_value(gpu, dtype):
+  """All values from -13.5 to 13.5 of a 16-bit type, through products by one: relative to each
+  value, in the negative tail too.  The distribution function's relative error stays
+  below (1 + z^2) 2^-19, and what is below 16 least normal float32 may vanish."""
+  z = torch.arange(-2**15, 2**15, dtype=torch.int32).to(torch.int16).view(dtype)
+  z = z[z.isfinite() & (z.abs() <= 13.5)]
+  n = z.numel()
+  batch, one = ops.ClientBatch([n]), torch.ones(1, 1, 1, dtype=dtype, device=gpu)
+  x = z.to(gpu)[:, None]
+  f, slope = ACTS["gelu"]
+  z64 = z.double()
+  e = (1 + z64 * z64) * 2.0**-19
+  least = 16 * 2.0**-126 + tiny(dtype)
+  want = f(z64)
+  check(ops.linear(x, one, None, batch, activation="gelu")[:, 0], want, (unit(dtype) + e) * want.abs() + least, "gelu")
+  want = slope(z64)
+  parts = 0.5 * torch.special.erfc(-z64 / math.sqrt(2)) + z64.abs() * torch.exp(-z64 * z64 / 2) / math.sqrt(2 * math.pi)
+  got = ops.linear_backward_input(torch.ones_like(x), one, batch, preactivation=x, activation="gelu")[:, 0]
+  check(got, want, unit(dtype) * want.abs() + (1 + unit(dtype)) * e * parts + least, "slope")
