@@ -1361,3 +1361,21 @@ def test_gelu_of_every_value(gpu, dtype):
   parts = 0.5 * torch.special.erfc(-z64 / math.sqrt(2)) + z64.abs() * torch.exp(-z64 * z64 / 2) / math.sqrt(2 * math.pi)
   got = ops.linear_backward_input(torch.ones_like(x), one, batch, preactivation=x, activation="gelu")[:, 0]
   check(got, want, unit(dtype) * want.abs() + (1 + unit(dtype)) * e * parts + least, "slope")
+
+
+def test_gelu_of_float32_in_its_tail(gpu):
+  """Relative to each value from -13.5 to 13.5.  The argument z / sqrt 2 carries 1.3 roundings
+  (its product and its constant), which erfc takes z^2 + 1 times; erfc and exp are good to 4
+  units, and two products follow: (12 + 2 z^2) u."""
+  z = torch.linspace(-13.5, 13.5, 400001, dtype=torch.float64).float()
+  batch, one = ops.ClientBatch([z.numel()]), torch.ones(1, 1, 1, device=gpu)
+  x = z.to(gpu)[:, None]
+  f, slope = ACTS["gelu"]
+  z64 = z.double()
+  e = (12 + 2 * z64 * z64) * U32
+  least = 16 * 2.0**-126
+  want = f(z64)
+  check(ops.linear(x, one, None, batch, activation="gelu")[:, 0], want, e * want.abs() + least, "gelu")
+  parts = 0.5 * torch.special.erfc(-z64 / math.sqrt(2)) + z64.abs() * torch.exp(-z64 * z64 / 2) / math.sqrt(2 * math.pi)
+  got = ops.linear_backward_input(torch.ones_like(x), one, batch, preactivation=x, activation="gelu")[:, 0]
+  check(got, slope(z64), e * parts + least, "slope")
