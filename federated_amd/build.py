@@ -30,27 +30,61 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
 CLIENT_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared"] + NO_PACKED_F32
 
 
+def _run(commands, verbose):
+  """The commands, at most as many at once as there are processors."""
+  running, at_once = [], max(1, os.cpu_count() or 1)
+
+  def wait(left):
+    while len(running) > left:
+      cmd, process = running.pop(0)
+      if process.wait():
+        for _, other in running:
+          other.wait()
+        raise subprocess.CalledProcessError(process.returncode, cmd)
+
+  for cmd in commands:
+    wait(at_once - 1)
+    if verbose:
+      print(" ".join(cmd), flush=True)
+    running.append((cmd, subprocess.Popen(cmd)))  # pylint: disable=consider-using-with
+  wait(0)
+
+
+def build_libraries(libraries, verbose=False):
+  """Libraries {path: macros of the codec's file}: all files each, compiled once where alike."""
+  with tempfile.TemporaryDirectory() as d:
+    def compiling(src, flags, defines, name):
+      obj = os.path.join(d, name + ".o")
+      return obj, [HIPCC, "-c"] + [f for f in flags if f != "-shared"] + ["-D" + m for m in defines] + ["-o", obj, src]
+
+    client = [compiling(s, CLIENT_FLAGS, [], os.path.basename(s)) for s in CLIENT_SRCS]
+    codec = [compiling(SRC, FLAGS, defines, "codec%d" % i) for i, defines in enumerate(libraries.values())]
+    _run([cmd for _, cmd in codec + client], verbose)
+    for out, (obj, _) in zip(libraries, codec):
+      tmp = out + ".tmp.%d" % os.getpid()
+      _run([[HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, obj] + [o for o, _ in client]], verbose)
+      os.replace(tmp, out)
+
+
 def build(force=False, verbose=False):
   sources = [SRC, HDR] + CLIENT_SRCS + CLIENT_HDRS
-  if not force and os.path.exists(OUT) and os.path.getmtime(OUT) >= max(os.path.getmtime(s) for s in sources):
-    return OUT
-  tmp = OUT + ".tmp.%d" % os.getpid()
-  with tempfile.TemporaryDirectory() as d:
-    objs, running = [], []
-    for src, flags in [(SRC, FLAGS)] + [(s, CLIENT_FLAGS) for s in CLIENT_SRCS]:
-      objs.append(os.path.join(d, os.path.basename(src) + ".o"))
-      cmd = [HIPCC, "-c"] + [f for f in flags if f != "-shared"] + ["-o", objs[-1], src]
-      if verbose:
-        print(" ".join(cmd), flush=True)
-      running.append((cmd, subprocess.Popen(cmd)))  # pylint: disable=consider-using-with
-    codes = [p.wait() for _, p in running]
-    for (cmd, _), rc in zip(running, codes):
-      if rc:
-        raise subprocess.CalledProcessError(rc, cmd)
-    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp] + objs)
-  os.replace(tmp, OUT)
+  if force or not os.path.exists(OUT) or os.path.getmtime(OUT) < max(os.path.getmtime(s) for s in sources):
+    build_libraries({OUT: []}, verbose)
   return OUT
 
 
+def main(argv):
+  """[--force], or diagnostic libraries libfedcodec_NAME.so: NAME=MACRO[=VALUE][,MACRO...] ..."""
+  variants = {}
+  for arg in argv:
+    name, _, macros = arg.partition("=")
+    if not arg.startswith("--"):
+      variants[os.path.join(HERE, "libfedcodec_%s.so" % name)] = [m for m in macros.split(",") if m]
+  if variants:
+    build_libraries(variants, verbose=True)
+  else:
+    build(force="--force" in argv, verbose=True)
+
+
 if __name__ == "__main__":
-  build(force="--force" in sys.argv, verbose=True)
+  main(sys.argv[1:])
