@@ -58,7 +58,8 @@ class ClientBatch:
     counts = counts.astype(np.int64)
     if counts.min() < 0:
       raise ValueError("row counts must not be negative")
-    if int(counts.sum()) >= (1 << 31) - 1024:
+    # each first: a sum of any may wrap
+    if int(counts.max()) >= (1 << 31) - 1024 or int(counts.sum()) >= (1 << 31) - 1024:
       raise ValueError("a batch holds fewer than 2^31 - 1024 rows")
     self.device = torch.device("cuda" if device is None else device)
     if self.device.type != "cuda":

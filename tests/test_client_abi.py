@@ -296,3 +296,14 @@ def test_inline_assembly_names_the_scalar_register_it_sets():
           writes += 1
           assert '"m0"' in "".join(rest), (path, statement)
   assert writes
+
+
+@pytest.mark.parametrize("counts", [[1 << 62] * 4, [1 << 63, 1 << 63], [(1 << 63) - 1] * 2 + [9], [1 << 30] * 2,
+                                    [(1 << 31) - 1024], [1, -1], [-(1 << 62)] * 4, [1 << 64]], ids=str)
+def test_row_counts_whose_sum_wraps_are_refused(monkeypatch, counts):
+  import torch
+  from federated_amd import client_ops as ops
+  monkeypatch.setattr(_lib, "require_gpu", lambda: None)
+  monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+  with pytest.raises(ValueError):
+    ops.ClientBatch(counts)
