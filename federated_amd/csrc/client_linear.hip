@@ -1125,7 +1125,7 @@ int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, 
                               int64_t dbias_client_stride, int accumulate, int tile_rows, int splits, void* workspace,
                               int64_t workspace_bytes, void* stream) {
   if (nclients <= 0 || in_features <= 0 || out_features <= 0) return fc_internal_fail(-1, "bad sizes");
-  if (!clients || !dweight) return fc_internal_fail(-1, "null pointer");
+  if (!dz || !x || !clients || !dweight) return fc_internal_fail(-1, "null pointer");
   Args p = {};
   p.a = dz; p.lda = dz_stride;
   p.b = x; p.ldb = x_stride;

@@ -523,7 +523,8 @@ int fc_linear_backward_weight(const void* dz, int64_t dz_stride, const void* x, 
                               int64_t workspace_bytes, void* stream);
 
 /* The same for clients of few rows, where the write of dweight is what takes time: any
- * number of rows is right, up to 8 or 16 fast.  longest: the largest client's. */
+ * number of rows is right, up to 8 or 16 fast.  longest: the largest client's; 0: dz and x
+ * may be null. */
 int fc_linear_backward_weight_few(const void* dz, int64_t dz_stride, const void* x, int64_t x_stride, int dtype,
                                   const int32_t* clients, int32_t nclients, int64_t longest, int64_t in_features,
                                   int64_t out_features, float* dweight, int64_t dweight_client_stride,

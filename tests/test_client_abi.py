@@ -307,3 +307,12 @@ def test_row_counts_whose_sum_wraps_are_refused(monkeypatch, counts):
   monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
   with pytest.raises(ValueError):
     ops.ClientBatch(counts)
+
+
+def test_weight_gradient_refuses_missing_operands():
+  """They would be read on the device, by whichever client has rows."""
+  lib, b = _lib.load(), _buf()
+  for dz, x, clients in [(NULL, b, b), (b, NULL, b), (b, b, NULL)]:
+    # the workspace is refused after it, should it be missed: nothing is launched
+    refused(lib.fc_linear_backward_weight(dz, 8, x, 8, 1, clients, 1, 8, 8, b, 64, 8, NULL, 0, 0, 128, 3, NULL, 0, None),
+            b"null")
