@@ -27,6 +27,7 @@ still gets one gradient per client, which is what the codec encodes.
 """
 import ctypes
 import functools
+import math
 import operator
 
 import numpy as np
@@ -389,15 +390,29 @@ def _odd(t):
   return t.data_ptr() & 3 or (t.stride(0) | t.stride(-2)) & 1 or t.stride(-2) >= 1 << 22
 
 
+def _matrices(t, rows):
+  """(how many, rows of each) an operand holds: [rows, width], or [clients, out, in]."""
+  if t.dim() == 2:
+    return 1, rows
+  return (1 if t.stride(0) == 0 else t.shape[0]), t.shape[1]
+
+
+def _packs(t, rows):
+  """Whether one launch copies the operand: below 2^24 blocks of 256 vectors."""
+  clients, per = _matrices(t, rows)
+  return clients * -(-per * ((t.shape[-1] + 7) // 8) // 256) < 1 << 24
+
+
 def _packed(t, rows):
   """``t``'s rows ([rows, width], or [clients, out, in]) at a stride of whole vectors."""
   width = t.shape[-1]
   stride = (width + 7) // 8 * 8
+  clients, per = _matrices(t, rows)
   if t.dim() == 2:
-    clients, per, client_stride = 1, rows, 0
+    client_stride = 0
     out = torch.empty((rows, stride), dtype=t.dtype, device=t.device)
   else:
-    clients, per, client_stride = (1 if t.stride(0) == 0 else t.shape[0]), t.shape[1], t.stride(0)
+    client_stride = t.stride(0)
     out = torch.empty((clients, per, stride), dtype=t.dtype, device=t.device)
   _call(t.device, "fc_pack_rows", _ptr(t), client_stride, t.stride(-2), _DTYPES[t.dtype], clients, per, width, _ptr(out),
         stride)
@@ -415,8 +430,8 @@ def _operands(a, b, rows, tiles, steps, longest):
   """
   size = a.element_size()
   odd = (_odd(a), _odd(b)) if size == 2 else (0, 0)
-  if (odd[0] or odd[1]) and rows:
-    copies = sum(2 * _LAUNCH + n * 4 / 4e6 for o, n in zip(odd, (rows * a.shape[1], _elements(b, rows))) if o)
+  if (odd[0] or odd[1]) and rows and all(_packs(t, rows) for o, t in zip(odd, (a, b)) if o):
+    copies = sum(2 * _LAUNCH + math.prod(_matrices(t, rows)) * t.shape[-1] * 4 / 4e6 for o, t in zip(odd, (a, b)) if o)
     if _estimate(tiles, steps, longest, 2, True)[0] + copies < 2.2 * _estimate(tiles, steps, longest, 2, False)[0]:
       if odd[0]:
         a = _packed(a, rows)
@@ -425,12 +440,6 @@ def _operands(a, b, rows, tiles, steps, longest):
       odd = (0, 0)
   height, splits = _plan(tiles, steps, longest, size, not (odd[0] or odd[1]))
   return a, b, height, splits
-
-
-def _elements(b, rows):
-  if b.dim() == 2:
-    return rows * b.shape[1]
-  return (1 if b.stride(0) == 0 else b.shape[0]) * b.shape[1] * b.shape[2]
 
 
 def _workspace(blocks, rows, splits, device):

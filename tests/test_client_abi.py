@@ -316,3 +316,31 @@ def test_weight_gradient_refuses_missing_operands():
     # the workspace is refused after it, should it be missed: nothing is launched
     refused(lib.fc_linear_backward_weight(dz, 8, x, 8, 1, clients, 1, 8, 8, b, 64, 8, NULL, 0, 0, 128, 3, NULL, 0, None),
             b"null")
+
+
+@pytest.mark.parametrize("which", ["a", "b", "weight"])
+def test_operands_too_large_for_one_copy_are_read_as_they_lie(monkeypatch, which):
+  """Rows at odd elements are copied where that pays, but not more of them than the copy's one
+  launch takes (2^24 - 1 blocks of 256 vectors)."""
+  import torch
+  from federated_amd import client_ops as ops
+  packed = []
+  monkeypatch.setattr(ops, "_packed", lambda t, rows: packed.append(t) or t)
+  monkeypatch.setattr(ops, "_estimate", lambda tiles, steps, longest, size, aligned: (1.0 if aligned else 1e9, 128, 1))
+  lib, at = _lib.load(), _buf() // 16 * 16 + 16
+  half = torch.float16
+  for over in (False, True):
+    rows = (1 << 32) // 126 + (1000 if over else -10000)  # of 126 vectors; a matrix ends inside a block
+    if which == "weight":
+      a, n = torch.empty(9, 8, dtype=half, device="meta"), 9
+      b = torch.empty(4, rows // 4, 1001, dtype=half, device="meta")
+      pack = (b.shape[0], b.shape[1])
+    else:
+      big, small = torch.empty(rows, 1001, dtype=half, device="meta"), torch.empty(rows, 8, dtype=half, device="meta")
+      a, b, n = (big, small, rows) if which == "a" else (small, big, rows)
+      pack = (1, rows)
+    if over:  # as the copy's entry has it
+      refused(lib.fc_pack_rows(at, 0, 1001, 2, pack[0], pack[1], 1001, at, 1008, None), b"too many rows")
+    packed.clear()
+    out = ops._operands(a, b, n, (1, 1, 1), 1, 1)
+    assert bool(packed) != over and out[0] is a and out[1] is b and out[2:] == (128, 1)
