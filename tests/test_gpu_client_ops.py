@@ -1379,3 +1379,61 @@ def test_gelu_of_float32_in_its_tail(gpu):
   parts = 0.5 * torch.special.erfc(-z64 / math.sqrt(2)) + z64.abs() * torch.exp(-z64 * z64 / 2) / math.sqrt(2 * math.pi)
   got = ops.linear_backward_input(torch.ones_like(x), one, batch, preactivation=x, activation="gelu")[:, 0]
   check(got, slope(z64), e * parts + least, "slope")
+
+
+def check_added(rng, counts, k, m, dtype):
+  """Gradients added to what is there, and outputs over their residuals: as without, plus one
+  addition (a split's parts are added to the old value one by one)."""
+  n, c = sum(counts), len(counts)
+  batch = ops.ClientBatch(counts)
+  x, dz = rand(rng, (n, k), dtype), rand(rng, (n, m), dtype, 0.5)
+  w, b = flat_params(rng, c, [(m, k), (m,)], dtype, 1 / math.sqrt(k))
+  old = rand(rng, (c, m * k + m + 2), torch.float32)
+  rows = old.clone()
+  ops.linear_backward_weight(dz, x, batch, dweight=rows[:, 1:1 + m * k].unflatten(1, (m, k)),
+                             dbias=rows[:, 1 + m * k:1 + m * k + m], accumulate=True)
+  assert torch.equal(rows[:, 0], old[:, 0]) and torch.equal(rows[:, -1], old[:, -1])
+  for i, (lo, hi) in enumerate(spans(counts)):
+    d, xx = dz[lo:hi].double().cpu(), x[lo:hi].double().cpu()
+    o, r = old[i, 1:1 + m * k].view(m, k).double().cpu(), rows[i, 1:1 + m * k].view(m, k)
+    mag = d.abs().t() @ xx.abs()
+    check(r, o + d.t() @ xx, (2 * max(1, hi - lo) + 70) * U32 * mag + 70 * U32 * o.abs(), "dw of client %d" % i)
+    o, r = old[i, 1 + m * k:1 + m * k + m].double().cpu(), rows[i, 1 + m * k:1 + m * k + m]
+    mag = d.abs().sum(0)
+    check(r, o + d.sum(0), (2 * max(1, hi - lo) + 70) * U32 * mag + 70 * U32 * o.abs(), "db of client %d" % i)
+  res, below = rand(rng, (n, m), dtype), rand(rng, (n, k), dtype)
+  before = rand(rng, (n, k), dtype)
+  want = ops.linear(x, w, b, batch, activation="silu", residual=res.clone())
+  assert torch.equal(ops.linear(x, w, b, batch, activation="silu", residual=res, out=res), want)
+  want = ops.linear_backward_input(dz, w, batch, preactivation=before, activation="relu", residual=below.clone())
+  assert torch.equal(ops.linear_backward_input(dz, w, batch, preactivation=before, activation="relu", residual=below,
+                                               out=below), want)
+
+
+@pytest.mark.parametrize("rows,splits", [(32, 1), (32, 5), (128, 1), (128, 3), (256, 1), (256, 2), (128, 64)])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_every_plan_adds(gpu, monkeypatch, dtype, rows, splits):
+  monkeypatch.setattr(ops, "_few_rows", lambda *a: False)
+  monkeypatch.setattr(ops, "_plan", lambda tiles, steps, longest, size, aligned: (
+      128 if rows == 256 and (size == 4 or not aligned) else rows, splits))
+  monkeypatch.setattr(ops, "_estimate", lambda tiles, steps, longest, size, aligned: (
+      1e9 if aligned == (splits == 1) else 1.0, rows, splits))
+  rng = np.random.default_rng(rows + splits)
+  check_added(rng, [40, 0, 1, 300], 131, 77, dtype)
+  check_added(rng, [257, 3], 134, 260, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("k,m", [(96, 1000), (41, 129), (128, 64)])
+def test_linear_walking_adds(gpu, monkeypatch, dtype, k, m):
+  monkeypatch.setattr(ops, "_walks", lambda batch, columns, a, weight: a.shape[1] <= 128 and not (
+      ops._odd(a) or ops._odd(weight)))
+  monkeypatch.setattr(ops, "_estimate", lambda *a: (1.0 if a[4] else 1e9, 32, 1))
+  check_added(np.random.default_rng(k + m), [129, 0, 40], k, m, dtype)
+
+
+@pytest.mark.parametrize("vocab,k", [(3000, 5), (10004, 64), (10004, 300), (40000, 128)])
+def test_top_logits_of_float16_rows_far_from_zero(gpu, vocab, k):
+  """Rows around 1000: a value's last three bits lie below the bits the bound is found by."""
+  x = rand(np.random.default_rng(vocab + k), (5, vocab), torch.float16) + 1000.0
+  check_top(x, k, 2.0)
