@@ -23,7 +23,9 @@ buffer are apart), but may be ``residual`` itself.  A batch whose calls were cap
 into a graph has to live as long as the graph.
 
 Forward and backward are separate calls with explicit gradients: a broadcast weight
-still gets one gradient per client, which is what the codec encodes.
+still gets one gradient per client, which is what the codec encodes.  The calls are no
+part of torch's autograd: an input's ``requires_grad`` is not looked at, and outputs carry
+no graph.
 """
 import ctypes
 import functools

@@ -501,8 +501,8 @@ __device__ __forceinline__ Place place_of(const Args& p, int b) {
 }
 
 // Bound by the matrix unit (and its power) where the contraction is long: bfloat16, 8 clients
-// of 2048 rows, 4096 to 8192: 1.14 ms forward with residual and pre-activation, 1.06 input,
-// 1.14 weight gradient, 960 / 1040 / 965 TFLOP/s; the library's plain product of that size
+// of 2048 rows, 4096 to 8192: 1.08 ms forward with residual and pre-activation, 1.08 input,
+// 1.19 weight gradient, 1017 / 1019 / 922 TFLOP/s; the library's plain product of that size
 // class reaches 1407 / 1237 / 1100 by layout.  By memory where it is short or rows are few:
 // one row, 4096 to 14336: 117 MB of weight in 19 us.  Float32 products run at the unit's 153.
 // Tiles: 256 x 256 loads each operand half as often as 128 x 128, 32 x 128 wastes less on
@@ -717,7 +717,7 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
 // 96 to 10004), bound by its outputs' write: a block that makes one tile spends most of its
 // time on its start and end (20480 rows, 64 clients, bfloat16: 287 to 318 us).  So a block
 // keeps its 128 rows of A in LDS and walks along `walk` column tiles, the next one's B
-// loading while this one's outputs leave: 204 us, 2.0 TB/s.  What is left is the chain of
+// loading while this one's outputs leave: 204 us (190 in a trace), 2.1 TB/s.  What is left is the chain of
 // one tile (LDS reads, products, way out) in two blocks a CU; the writes alone, in such
 // tiles at rows of 20008 bytes, take 110.  In float32 the products are the chain, and it
 // gains nothing (64 to 10004: 214 us in tiles, 239 walking).

@@ -531,7 +531,8 @@ __global__ __launch_bounds__(NT) void k_top_logits(const T* logits, int64_t ld, 
   }
   for (; c0 < at_row.end; c0 += kStride) add(at_row.load(c0));
 
-  // 16-bit types: the key's low half follows from its high half
+  // 16-bit types: by the key's high half, from which a bfloat16's low half follows; a float16
+  // keeps its last three bits there, so its bound is up to eight values low (more candidates)
   constexpr int kBits = 8 * (int)sizeof(T);
   const uint32_t best = sm.m == -INFINITY ? 0 : order_key(sm.m);  // nothing but -inf and NaN bounds nothing
   maxima[tid] = best;
@@ -692,7 +693,7 @@ __global__ __launch_bounds__(NT) void k_top_logits(const T* logits, int64_t ld, 
 //   ds_j = w_r tau (m q_j - sum_{k: i_k = j} p_k)
 //
 // Bound by one read of the logits and one write of the gradient: 20480 rows of 10004
-// (float32, k 32) in 328 us, 5.0 TB/s; 8197 of 131072 (bfloat16, k 64) in 921, 4.7 TB/s.
+// (float32, k 32) in 328 us, 5.0 TB/s; 8197 of 131072 (bfloat16, k 64) in 919, 4.7 TB/s.
 // ---------------------------------------------------------------------------
 
 constexpr int kDistillMax = 1024;  // teacher entries per row
@@ -1076,7 +1077,9 @@ int distill_launch(const DistillArgs& a, int64_t rows, bool loss, hipStream_t s)
     distill_go<T, 256, 10>(a, rows, loss, s);
   } else if (vecs < 1024 * 4) {
     distill_go<T, 1024, 4>(a, rows, loss, s);
-  } else if (vecs < 1024 * 8 && vecs >= 1024 * 7 && sizeof(T) == 4) {  // 9375 rows of 32000: 465 us, streamed 497
+  } else if (vecs < 1024 * 8 && vecs >= 1024 * 7 && sizeof(T) == 4) {
+    // 3e8 elements, us held / streamed: rows of 20000 541 / 491, 24000 526 / 490, 28000 497 / 497,
+    // 28700 519 / 515, 30000 506 / 511, 32000 480 / 499, 32700 481 / 522
     distill_go<T, 1024, sizeof(T) == 4 ? 8 : 4>(a, rows, loss, s);
   } else {
     distill_go<T, 1024, 0>(a, rows, loss, s);
@@ -1101,7 +1104,11 @@ int top_launch(const void* logits, int64_t stride, int64_t rows, int64_t vocab, 
   // 16: 64 threads 462, 256 676; 60,000 of 10004: 256 threads 303 (k 16), 802 (200), 4063
   // (300), 4551 (1000), 1024 threads 924, 1394, 2021, 9058: where the bound is close for
   // neither, the exact select's barriers cost the larger block more.  600,000 of 1000, k 128:
-  // vectors of two 4212, of eight, which leave half of the threads without, 9661.
+  // vectors of two 4212, of eight, which leave half of the threads without, 9661.  The limits
+  // at other widths (2e8 elements, 256 / 1024 threads): k 200 6000 wide 408 / 698, 32000 189 /
+  // 208; k 256 1218 / 1047, 586 / 270; k 800 10004 wide 1608 / 1294, 24000 1363 / 579; k 1000
+  // 1622 / 3198, 1372 / 1961: beyond 10,000 wide and between 700 and some 950 the larger
+  // block would be faster.
   auto go = [&](auto threads, auto vec) {
     constexpr int NT = decltype(threads)::value, VEC = decltype(vec)::value;
     in_parts<NT>(rows, [&](int64_t first, dim3 grid) {
