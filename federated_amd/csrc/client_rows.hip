@@ -824,8 +824,10 @@ __global__ __launch_bounds__(NT) void k_distill(const DistillArgs a) {
   }
 
   // The student's softmax: q_j = exp2((s_j - c) scale) / sum.  A saved lse is c = lse tau and
-  // a sum of 1, and costs q an error of |lse| 2^-24: beyond kFar the row is summed again.
-  constexpr float kFar = 1024.0f;
+  // a sum of 1, and its four roundings (m / tau twice, the sum, c) cost q a relative error of
+  // |lse| 2^-22: beyond kFar (1.5e-5 in float32, as the softmax's own; an eighth of float16's
+  // half step) the row is summed again.
+  constexpr float kFar = sizeof(T) == 4 ? 64.0f : 256.0f;
   Softmax sm;
   float lse = LOSS ? 0.0f : a.lse[row];
   const bool scan = LOSS || !(fabsf(lse) <= kFar);

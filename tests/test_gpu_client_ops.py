@@ -1437,3 +1437,28 @@ def test_top_logits_of_float16_rows_far_from_zero(gpu, vocab, k):
   """Rows around 1000: a value's last three bits lie below the bits the bound is found by."""
   x = rand(np.random.default_rng(vocab + k), (5, vocab), torch.float16) + 1000.0
   check_top(x, k, 2.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("offset", [30.0, 60.0, 200.0, -250.0, 500.0, 1000.0])
+@pytest.mark.parametrize("tau", [1.0, 0.5])
+def test_distillation_gradient_alone_at_an_offset(gpu, dtype, offset, tau):
+  """A saved log-sum-exp carries four roundings of its size into q, 2^-22 |lse| relative: as
+  far as 64 for a float32 gradient (1.5e-5), 256 for 16-bit ones (6e-5, an eighth of
+  float16's half step); beyond, the softmax's own roundings alone."""
+  rng = np.random.default_rng(int(abs(offset) + 10 * tau))
+  vocab, n = 501, 40
+  batch = ops.ClientBatch([n])
+  logits = rand(rng, (n, vocab), dtype) + offset
+  index, values = teacher_rows(rng, n, vocab, 4, pad=0)
+  s = logits.double().cpu() / tau
+  q, p = torch.softmax(s, 1), torch.softmax(values.double().cpu() / tau, 1)
+  want = (q.scatter_add(1, index.long().cpu(), -p)) * tau / n
+  _, lse = ops.distillation(logits, index, values, batch, temperature=tau)
+  far = float(torch.logsumexp(s, 1).abs().max()) > (64.0 if dtype == torch.float32 else 256.0)
+  saved = 0.0 if far else 2.0**-22 * torch.logsumexp(s, 1).abs()[:, None]
+  both = (q + p.sum(1, keepdim=True) * (want < 0)) * tau / n
+  tol = (2 * 16 / tau + vocab / 64 + 24 + 16) * 2 * U32 * both + 2 * saved * q * tau / n
+  tol = tol + unit(dtype) * (want.abs() + tol) + tiny(dtype)
+  got = ops.distillation_backward(logits, lse, index, values, batch, temperature=tau)
+  check(got, want, tol, "gradient")
