@@ -717,10 +717,10 @@ __global__ __launch_bounds__(WM * WN * 64, 8 / (WM * WN)) void k_linear(const Ar
 // 96 to 10004), bound by its outputs' write: a block that makes one tile spends most of its
 // time on its start and end (20480 rows, 64 clients, bfloat16: 287 to 318 us).  So a block
 // keeps its 128 rows of A in LDS and walks along `walk` column tiles, the next one's B
-// loading while this one's outputs leave: 204 us (190 in a trace), 2.1 TB/s.  What is left is the chain of
-// one tile (LDS reads, products, way out) in two blocks a CU; the writes alone, in such
-// tiles at rows of 20008 bytes, take 110.  In float32 the products are the chain, and it
-// gains nothing (64 to 10004: 214 us in tiles, 239 walking).
+// loading while this one's outputs leave: 204 us (190 in a trace), 2.1 TB/s.  What is left
+// is the chain of one tile (LDS reads, products, way out) in two blocks a CU; the writes
+// alone, in such tiles at rows of 20008 bytes, take 110.  In float32 the products are the
+// chain, and it gains nothing (64 to 10004: 214 us in tiles, 239 walking).
 template <typename T, int KIND, int STEPS>
 __global__ __launch_bounds__(256, 2) void k_linear_short(const Args p) {
   constexpr bool kB_KC = KIND == kForward;

@@ -543,7 +543,8 @@ int fc_top_logits(const void* logits, int64_t stride, int dtype, int64_t rows, i
  * loss given: loss [nclients] from row_loss [rows] (scratch), lse (nullable) out, grad
  * (nullable; may be logits) in the same pass.  loss NULL: grad from the saved lse,
  * scaled by dloss [nclients] (nullable); rows of weight 0 or of nothing but padding save
- * a NaN, and a gradient that looks at such a row sums it.  row_weights NULL: 1 / the client's rows. */
+ * a NaN, and a gradient that looks at such a row sums it.  row_weights NULL: 1 / the
+ * client's rows. */
 int fc_distill(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t vocab, const int32_t* index,
                const float* values, int32_t k, const int32_t* row_client, const int32_t* offsets, int32_t nclients,
                float temperature, const float* teacher_lse, const float* row_weights, const float* dloss,
